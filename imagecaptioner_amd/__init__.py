@@ -8,4 +8,5 @@ The pipeline itself runs only on the GPU (imagecaptioner_amd/csrc); importing th
 package does not need one, constructing a TagPipe does.
 """
 from ._abi import Config  # noqa: F401
+from .replies import TagGrammar  # noqa: F401
 from .tagpipe import BatchResult, TagPipe, TagPipeError, load_library  # noqa: F401

@@ -151,6 +151,27 @@ class tp_replies(C.Structure):
                 ("sources", C.POINTER(C.c_uint8)), ("status", C.POINTER(C.c_uint8)), ("has_score", C.POINTER(C.c_uint8)), ("opaque", C.c_void_p)]
 
 
+TP_T_F32, TP_T_F16, TP_T_BF16 = 0, 1, 2
+
+
+class tp_logits(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("type", C.c_int32), ("rows", C.c_uint64), ("vocab", C.c_uint32), ("history_cap", C.c_uint32),
+                ("logits", C.c_void_p), ("stride", C.c_uint64), ("history", C.c_void_p), ("history_stride", C.c_uint64), ("history_len", C.c_void_p),
+                ("prompt_len", C.c_void_p), ("repetition", C.c_void_p), ("frequency", C.c_void_p), ("presence", C.c_void_p), ("bias", C.c_void_p),
+                ("bias_stride", C.c_uint64), ("bias_row", C.c_void_p), ("mask", C.c_void_p), ("mask_stride", C.c_uint64), ("mask_row", C.c_void_p),
+                ("n_bias", C.c_uint32), ("n_masks", C.c_uint32), ("stream", C.c_void_p)]
+
+
+class tp_grammar_config(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("n_tokens", C.c_uint32), ("tokens", C.c_void_p), ("token_offsets", C.c_void_p), ("end_token", C.c_int32),
+                ("min_tags", C.c_uint32), ("max_tags", C.c_uint32), ("spaces", C.c_uint32), ("tags", C.c_void_p), ("tag_offsets", C.c_void_p), ("n_tags", C.c_uint64)]
+
+
+class tp_grammar_info(C.Structure):
+    _fields_ = [("n_tokens", C.c_uint32), ("n_prefixes", C.c_uint32), ("n_tags", C.c_uint32), ("longest_token", C.c_uint32), ("longest_list", C.c_uint32),
+                ("reserved", C.c_uint32), ("n_entries", C.c_uint64)]
+
+
 TP_REPLY_OK, TP_REPLY_NO_TAGS, TP_REPLY_ORDER, TP_REPLY_FAILED = 0, 1, 2, 3
 
 

@@ -15,6 +15,7 @@
 
 #include "../../include/tagpipe.h"
 #include "tp_launch.h"
+#include "tp_reply.h"
 #include "tp_pipeline.h"
 #include "tp_tables.hpp"
 
@@ -250,6 +251,41 @@ struct tp_ctx {
     }
     bool no_overlap = false;         // TAGPIPE_NO_OVERLAP=1: the host-pointer run copies in, computes and copies out in turn (testing aid)
 };
+
+// A grammar (tp_grammar_create) in device memory; it holds nothing of the context it was made from.
+struct tp_grammar {
+    int device = 0;
+    tp_grammar_info info{};
+    DevGrammar dev{};
+    std::vector<void*> owned;
+    ~tp_grammar();
+};
+
+namespace {
+
+// Makes `device` current for a scope and puts the caller's device back.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        int now = 0;
+        HIP_OK(hipGetDevice(&now));
+        if (now == device) return;
+        HIP_OK(hipSetDevice(device));
+        before = now;
+    }
+    OnDevice(const OnDevice&) = delete;
+    ~OnDevice() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
+}  // namespace
+
+tp_grammar::~tp_grammar() {
+    int now = 0;
+    const bool known = hipGetDevice(&now) == hipSuccess;
+    (void)hipSetDevice(device);
+    for (void* p : owned) (void)hipFree(p);
+    if (known) (void)hipSetDevice(now);
+}
 
 namespace {
 
@@ -1785,6 +1821,109 @@ int tp_format_review_rows(const tp_ctx* ctx, const tp_result* res, int format, c
             return true;
         };
         return format_rows_parallel(n_files, nl, row_for, out, capacity, out_offsets, needed);
+    });
+}
+
+// ---- writing the replies ------------------------------------------------------------------------------------------------------
+
+uint64_t tp_choose_workspace(uint64_t rows, uint32_t vocab) { return choose_workspace(rows, vocab); }
+uint64_t tp_lines_workspace(uint64_t rows) { return lines_workspace(rows); }
+
+int tp_shape_logits(tp_ctx* ctx, const tp_logits* io, void* out, uint64_t out_stride) {
+    if (!ctx) return fail(TP_E_INVALID_ARG, "null argument");
+    if (const char* e = check_shape(io, out, out_stride)) return fail(TP_E_INVALID_ARG, e);
+    if (io->rows == 0) return TP_OK;
+    return guarded([&]() {
+        OnDevice d(ctx->device);
+        HIP_OK(launch_shape(*io, out, out_stride));
+        return (int)TP_OK;
+    });
+}
+
+int tp_choose_tokens(tp_ctx* ctx, const tp_logits* io, const float* temperature, const float* uniform, int32_t* tokens, float* logprob,
+                     void* workspace, uint64_t workspace_bytes) {
+    if (!ctx) return fail(TP_E_INVALID_ARG, "null argument");
+    if (const char* e = check_choose(io, temperature, uniform, tokens, logprob, workspace, workspace_bytes)) return fail(TP_E_INVALID_ARG, e);
+    if (io->rows == 0) return TP_OK;
+    return guarded([&]() {
+        OnDevice d(ctx->device);
+        HIP_OK(launch_choose(*io, temperature, uniform, tokens, logprob, (ChoicePart*)workspace));
+        return (int)TP_OK;
+    });
+}
+
+tp_grammar* tp_grammar_create(tp_ctx* ctx, const tp_grammar_config* cfg) {
+    if (!ctx) { fail(TP_E_INVALID_ARG, "null argument"); return nullptr; }
+    if (const char* e = check_grammar_config(cfg)) { fail(TP_E_INVALID_ARG, e); return nullptr; }
+    tp_grammar* made = nullptr;
+    const int rc = guarded([&]() {
+        std::unique_ptr<tp_grammar> g(new tp_grammar());
+        std::vector<std::string> tags;
+        if (cfg->tags) {
+            for (uint64_t t = 0; t < cfg->n_tags; ++t) tags.emplace_back((const char*)cfg->tags + cfg->tag_offsets[t], (size_t)(cfg->tag_offsets[t + 1] - cfg->tag_offsets[t]));
+        } else {
+            tags = reply_tags(ctx->ht);
+        }
+        HostGrammar h;
+        compile_grammar(*cfg, std::move(tags), h);
+        g->device = ctx->device;
+        g->info = h.info;
+        OnDevice d(ctx->device);
+        g->dev.begin = upload(g->owned, h.begin);
+        g->dev.token = upload(g->owned, h.token);
+        g->dev.move = upload(g->owned, h.move);
+        g->dev.text = upload(g->owned, h.text);
+        g->dev.text_begin = upload(g->owned, h.text_begin);
+        g->dev.n_tokens = h.info.n_tokens;
+        g->dev.n_places = h.info.n_prefixes + 2;
+        g->dev.min_tags = h.min_tags;
+        g->dev.max_tags = h.max_tags;
+        made = g.release();
+        return (int)TP_OK;
+    });
+    return rc == TP_OK ? made : nullptr;
+}
+
+void tp_grammar_destroy(tp_grammar* g) { delete g; }
+
+int tp_grammar_get_info(const tp_grammar* g, tp_grammar_info* out) {
+    if (!g || !out) return fail(TP_E_INVALID_ARG, "null argument");
+    *out = g->info;
+    return TP_OK;
+}
+
+int tp_grammar_mask(const tp_grammar* g, const int32_t* states, uint64_t rows, uint32_t* mask, uint64_t mask_stride, void* stream) {
+    if (!g) return fail(TP_E_INVALID_ARG, "null argument");
+    if (const char* e = check_mask(g->dev.n_tokens, states, rows, mask, mask_stride)) return fail(TP_E_INVALID_ARG, e);
+    if (rows == 0) return TP_OK;
+    return guarded([&]() {
+        OnDevice d(g->device);
+        HIP_OK(launch_grammar_mask(g->dev, states, rows, mask, mask_stride, (hipStream_t)stream));
+        return (int)TP_OK;
+    });
+}
+
+int tp_grammar_step(const tp_grammar* g, const tp_logits* io, const float* temperature, const float* uniform, int32_t* states, int32_t* tokens,
+                    float* logprob, int append) {
+    if (!g) return fail(TP_E_INVALID_ARG, "null argument");
+    if (const char* e = check_step(g->dev.n_tokens, io, temperature, uniform, states, tokens, logprob, append)) return fail(TP_E_INVALID_ARG, e);
+    if (io->rows == 0) return TP_OK;
+    return guarded([&]() {
+        OnDevice d(g->device);
+        HIP_OK(launch_grammar_step(g->dev, *io, temperature, uniform, states, tokens, logprob, append));
+        return (int)TP_OK;
+    });
+}
+
+int tp_grammar_lines(const tp_grammar* g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t rows,
+                     uint8_t* arena, uint64_t capacity, uint64_t* offsets, void* workspace, uint64_t workspace_bytes, void* stream) {
+    if (!g) return fail(TP_E_INVALID_ARG, "null argument");
+    if (const char* e = check_lines(tokens, stride, width, begin, len, rows, arena, capacity, offsets, workspace, workspace_bytes)) return fail(TP_E_INVALID_ARG, e);
+    if (rows == 0) return TP_OK;
+    return guarded([&]() {
+        OnDevice d(g->device);
+        HIP_OK(launch_grammar_lines(g->dev, tokens, stride, width, begin, len, rows, arena, capacity, offsets, workspace, (hipStream_t)stream));
+        return (int)TP_OK;
     });
 }
 

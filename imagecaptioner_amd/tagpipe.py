@@ -9,8 +9,8 @@ import os
 
 import numpy as np
 
-from ._abi import (tp_replies, TP_E_CAPACITY, TP_OK, VERDICT_DTYPE, Config, tp_audit, tp_config, tp_counters, tp_device_io, tp_result, tp_table_info,
-                   tp_timing)
+from ._abi import (tp_replies, TP_E_CAPACITY, TP_OK, VERDICT_DTYPE, Config, tp_audit, tp_config, tp_counters, tp_device_io, tp_grammar_config,
+                   tp_grammar_info, tp_logits, tp_result, tp_table_info, tp_timing)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtagpipe_hip.so")
@@ -22,6 +22,8 @@ EXPORTS = (
     "tp_triage_lines", "tp_run_merged", "tp_format_fired_rules", "tp_needtag_text", "tp_format_side_files",
     "tp_decode_joytag_replies", "tp_release_replies", "tp_run_replies", "tp_set_audit", "tp_get_audit", "tp_audit_header", "tp_format_audit_rows", "tp_review_csv_header", "tp_format_review_rows",
     "tp_fallback_caption", "tp_error_needtag_text",
+    "tp_shape_logits", "tp_choose_workspace", "tp_choose_tokens", "tp_grammar_create", "tp_grammar_destroy", "tp_grammar_get_info", "tp_grammar_mask",
+    "tp_grammar_step", "tp_lines_workspace", "tp_grammar_lines",
 )
 
 
@@ -88,6 +90,21 @@ def load_library():
                                         C.c_void_p, C.c_uint64, C.c_void_p, C.POINTER(C.c_uint64)]
     L.tp_fallback_caption.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.POINTER(C.c_uint64)]
     L.tp_error_needtag_text.restype = C.c_char_p
+    L.tp_shape_logits.argtypes = [C.c_void_p, C.POINTER(tp_logits), C.c_void_p, C.c_uint64]
+    L.tp_choose_workspace.argtypes = [C.c_uint64, C.c_uint32]
+    L.tp_choose_workspace.restype = C.c_uint64
+    L.tp_choose_tokens.argtypes = [C.c_void_p, C.POINTER(tp_logits), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64]
+    L.tp_grammar_create.argtypes = [C.c_void_p, C.POINTER(tp_grammar_config)]
+    L.tp_grammar_create.restype = C.c_void_p
+    L.tp_grammar_destroy.argtypes = [C.c_void_p]
+    L.tp_grammar_destroy.restype = None
+    L.tp_grammar_get_info.argtypes = [C.c_void_p, C.POINTER(tp_grammar_info)]
+    L.tp_grammar_mask.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]
+    L.tp_grammar_step.argtypes = [C.c_void_p, C.POINTER(tp_logits), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]
+    L.tp_lines_workspace.argtypes = [C.c_uint64]
+    L.tp_lines_workspace.restype = C.c_uint64
+    L.tp_grammar_lines.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
+                                   C.c_uint64, C.c_void_p]
     _LIB = L
     return L
 
@@ -460,6 +477,26 @@ class TagPipe:
             self._L.tp_set_audit(self._h, 0)
         return self._collect(res, audit)
 
+    # ---- writing the replies (torch tensors on the context's device; see replies.py) ----------------
+    def shape_logits(self, logits, *, out=None, **rules):
+        """tp_shape_logits: penalties for repeated tokens, biases and allowed-token masks on logits [rows, vocab] (float32, float16 or
+        bfloat16).  `rules` are those of replies.logit_rules.  `out` may be `logits` itself (in place); a new tensor otherwise."""
+        return replies.shape_logits(self, logits, out, rules)
+
+    def choose_tokens(self, logits, *, temperature=None, uniform=None, **rules):
+        """tp_choose_tokens: (tokens int32 [rows], log-probabilities float32 [rows]) of the shaped logits, which are not written.
+        temperature float32 [rows] (0: the largest) and uniform float32 [rows] in [0, 1) make it a sample; without them it is the largest."""
+        return replies.choose_tokens(self, logits, temperature, uniform, rules)
+
+    def tag_grammar(self, tokens, end_token, *, min_tags=3, max_tags=42, spaces=False, tags=None):
+        """tp_grammar_create: the tag lines of this context's tables (or of `tags`) over a model's token list (texts, bytes or str)."""
+        return replies.TagGrammar(self, tokens, end_token, min_tags, max_tags, spaces, tags)
+
+    def run_tokens(self, grammar, tokens, lengths=None, begin=None):
+        """Written replies through the pipeline without leaving the device: TagGrammar.lines on the rows of `tokens`, then
+        tp_run_lines_device on the texts.  Returns a BatchResult, as run_lines of the same texts does."""
+        return replies.run_tokens(self, grammar, tokens, lengths, begin)
+
     # ---- device-resident run ---------------------------------------------------------------------
     def run_lines_device(self, io: tp_device_io, noalloc=False):
         """tp_run_lines_device: every pointer in `io` is a device pointer.  Returns the caption byte count;
@@ -472,3 +509,6 @@ class TagPipe:
             err.required = nbytes.value
             raise err
         return nbytes.value
+
+
+from . import replies  # noqa: E402  (it needs the names above)

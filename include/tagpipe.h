@@ -489,6 +489,143 @@ int tp_format_review_rows(const tp_ctx* ctx, const tp_result* res, int format, c
                           const uint8_t* caption_paths, const uint64_t* caption_offsets, const char* thresholds_used, const char* vocab_file,
                           uint8_t* out, uint64_t capacity, uint64_t* out_offsets, uint64_t* needed);
 
+/*
+ * Writing the replies.  The line ingest above parses a language model's answer (Program.cs:574-587); a caller whose
+ * captioning model runs on the same GPU has that model's logits in device memory, one row per reply and one column per
+ * token.  The functions below write the answer under the rules the pipeline will read it by, token by token, so that
+ * no refusal, no unknown tag and no cut-off line has to be dropped afterwards:
+ *
+ *   tp_shape_logits   penalties for repeated tokens, a bias and a mask of allowed tokens on the logits
+ *   tp_choose_tokens  the same without writing the logits: the token that is chosen, and its log-probability
+ *   tp_grammar_mask   the mask of the tokens that keep a row's text a tag line of this context's tables
+ *   tp_grammar_step   shaping, choice among the grammar's tokens and the move to the next state, in one launch
+ *   tp_grammar_lines  the written tokens as text: the arena and offsets tp_run_lines_device takes
+ *
+ * Conventions.  Every pointer in these structs and argument lists is a device pointer on the context's device unless
+ * it is said to be host memory.  Work is enqueued on `stream` (a hipStream_t, NULL = default stream); no call
+ * allocates, copies to the host or waits, so all but tp_grammar_create may be captured into a HIP graph.  The caller's current
+ * device is left as it was.  A workspace holds nothing between calls and needs no initial contents, but calls that may
+ * overlap (two streams, two graphs replayed at once) need one each.  Outputs must not overlap inputs except where a
+ * call says so.  Zero rows: nothing is done.  A grammar does not refer to the context it was made from.
+ */
+#define TP_T_F32  0
+#define TP_T_F16  1
+#define TP_T_BF16 2
+
+/*
+ * One row per reply.  With l the logit of token t in row r, in 32-bit arithmetic and in this order:
+ *   x = l;  t stands in the row's history:              x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *           n times at or behind prompt_len[r], n > 0:  x = x - frequency[r] * n, then x = x - presence[r]
+ *           the row has a bias:                         x = x + bias[t]
+ *           the row has a mask and t's bit is 0:        x = -infinity, whatever l is (l need not be read)
+ * A history entry outside [0, vocab) is skipped.  Lengths are taken as 0 below 0 and as history_cap above it.
+ */
+typedef struct tp_logits {
+    uint32_t struct_size;         /* sizeof(tp_logits) */
+    int32_t  type;                /* TP_T_* of logits (and of tp_shape_logits' output) */
+    uint64_t rows;
+    uint32_t vocab;               /* tokens, 1 .. 2^24 */
+    uint32_t history_cap;         /* entries a row of the history has room for, at most 2^31 - 1 */
+    const void* logits;           /* row r starts at element r * stride */
+    uint64_t stride;              /* elements, at least vocab; any alignment of an element's own size */
+    int32_t* history;             /* row r's tokens: history[r * history_stride + k], k < history_len[r]; NULL: no history */
+    uint64_t history_stride;      /* elements, at least history_cap */
+    int32_t* history_len;         /* rows; NULL: every row holds history_cap tokens */
+    const int32_t* prompt_len;    /* rows; entries before it count as repeated but not for frequency and presence; NULL: 0 */
+    const float* repetition;      /* rows, NULL: 1; greater than 0 */
+    const float* frequency;       /* rows, NULL: 0 */
+    const float* presence;        /* rows, NULL: 0 */
+    const float* bias;            /* n_bias rows of vocab entries; NULL: none */
+    uint64_t bias_stride;         /* elements, at least vocab */
+    const int32_t* bias_row;      /* rows: which bias; outside [0, n_bias): none for this row.  NULL: bias 0 for every row */
+    const uint32_t* mask;         /* n_masks rows of (vocab + 31) / 32 words: token t is allowed when bit t % 32 of word t / 32 is 1; NULL: none */
+    uint64_t mask_stride;         /* words, at least (vocab + 31) / 32 */
+    const int32_t* mask_row;      /* rows: which mask; outside [0, n_masks): none for this row.  NULL: mask 0 for every row */
+    uint32_t n_bias, n_masks;
+    void* stream;
+} tp_logits;
+
+/*
+ * out[r * out_stride + t] = x, rounded once to the logits' type.  `out` may be `logits` with the same stride (in place);
+ * it must not overlap them otherwise.  Elements of `out` behind a row's vocab entries are left as they were.
+ */
+int tp_shape_logits(tp_ctx* ctx, const tp_logits* io, void* out, uint64_t out_stride);
+
+/*
+ * The token of every row.  z = x / temperature[r] where temperature[r] > 0, else z = x.  Without a temperature (NULL
+ * array, 0, negative, NaN) the token is the largest x, ties to the lowest token.  With one it is the lowest token whose
+ * cumulative weight exceeds uniform[r] * (the sum of all weights), weights exp(z - max z) in token order, summed in 64
+ * bits; uniform[r] in [0, 1), NULL: as temperature NULL.  Values of uniform outside [0, 1) give the first or last token of a weight above 0.
+ * A z of NaN counts as -infinity.  Where +infinity stands, the tokens that have it share the weight.
+ * logprob[r] = z - max z - ln(sum of weights) of the chosen token.  A row without a z above -infinity gets token -1 and
+ * log-probability -infinity.  logprob may be NULL.  workspace: tp_choose_workspace bytes (host function), aligned to 16.
+ */
+uint64_t tp_choose_workspace(uint64_t rows, uint32_t vocab);
+int tp_choose_tokens(tp_ctx* ctx, const tp_logits* io, const float* temperature, const float* uniform, int32_t* tokens, float* logprob,
+                     void* workspace, uint64_t workspace_bytes);
+
+/*
+ * The grammar of a tag line over a model's token list:  tag ", " tag ", " ... tag <end>,  between min_tags and max_tags
+ * tags.  A tag is one the pipeline keeps: with a vocabulary file a member of it that ShouldDropTag lets pass
+ * (Program.cs:1121-1133), without one any such string of the context's tables; or one of the caller's own `tags`.
+ * Tags may repeat (tp_logits' penalties are there for that).  A token may be any piece of text; one that holds two commas is never allowed.
+ * Refused (TP_E_CONFIG): no tags; a token list without a token of its own for every single byte that the lines use,
+ * because a line could then come to a place with no way on.  All pointers are host memory and are not kept.
+ *
+ * A row's state is two int32: the place its text has come to, and how many tags it has finished (commas written).  Places: k = the
+ * k-th of the sorted distinct prefixes of the tags (bytes, ascending; 0 = the empty one, where a line and every tag
+ * begins); n_prefixes = behind a tag's comma; n_prefixes + 1 = the end is written.  {0, 0} starts a line.  Nothing is
+ * allowed behind the end or in a place outside [0, n_prefixes + 1].
+ */
+typedef struct tp_grammar tp_grammar;
+typedef struct tp_grammar_config {
+    uint32_t struct_size;          /* sizeof(tp_grammar_config) */
+    uint32_t n_tokens;             /* 1 .. 2^24 */
+    const uint8_t*  tokens;        /* token t is tokens[token_offsets[t] .. token_offsets[t + 1]); an empty one is never allowed */
+    const uint64_t* token_offsets; /* n_tokens + 1 */
+    int32_t  end_token;            /* ends a line; its text counts as empty */
+    uint32_t min_tags, max_tags;   /* 1 <= min_tags <= max_tags <= 65535; three tags is what a line needs not to fall back (Program.cs:297) */
+    uint32_t spaces;               /* 1: the '_' of a tag is written ' ' (NormalizeTag takes it back, Program.cs:1153) */
+    const uint8_t*  tags;          /* the caller's own tags, laid out like the tokens; NULL: the context's */
+    const uint64_t* tag_offsets;   /* n_tags + 1 */
+    uint64_t n_tags;
+} tp_grammar_config;
+typedef struct tp_grammar_info {
+    uint32_t n_tokens, n_prefixes; /* places 0 .. n_prefixes + 1 */
+    uint32_t n_tags;               /* distinct tags */
+    uint32_t longest_token;        /* bytes */
+    uint32_t longest_list;         /* most tokens that may follow any one place */
+    uint32_t reserved;
+    uint64_t n_entries;            /* all places' tokens */
+} tp_grammar_info;
+tp_grammar* tp_grammar_create(tp_ctx* ctx, const tp_grammar_config* cfg);   /* NULL on failure */
+void tp_grammar_destroy(tp_grammar* g);                                       /* after the work that uses it is done */
+int tp_grammar_get_info(const tp_grammar* g, tp_grammar_info* out);
+
+/* mask: per row (n_tokens + 31) / 32 words as tp_logits' mask takes them, row r at r * mask_stride; bits behind the last token are 0. */
+int tp_grammar_mask(const tp_grammar* g, const int32_t* states, uint64_t rows, uint32_t* mask, uint64_t mask_stride, void* stream);
+
+/*
+ * tp_choose_tokens with the grammar's tokens of every row's state as the mask (io's mask must be NULL; io->vocab must be n_tokens), then the
+ * state moves on and, with append = 1, the token goes to the end of the row's history and history_len is raised (both must then be
+ * given; a row whose history is full gets no token).  A row without a token (-1: its line is at the end, or no allowed token has an
+ * x above -infinity) keeps its state and its history.  io->logits NULL: `tokens` is an input, the caller's own choice; a token that the
+ * grammar does not allow there moves the row to place -1, token -1 does nothing; logprob is not written.
+ */
+int tp_grammar_step(const tp_grammar* g, const tp_logits* io, const float* temperature, const float* uniform, int32_t* states,
+                    int32_t* tokens, float* logprob, int append);
+
+/*
+ * The texts of rows of tokens, back to back: row r's is arena[offsets[r] .. offsets[r + 1]).  Row r's tokens are
+ * tokens[r * stride + k], from begin[r] (NULL: 0) to below len[r] (NULL: width; both taken as 0 below 0 and as width above it); one outside
+ * [0, n_tokens) has no text.  A row's text must stay below 4 GiB.  Nothing is written at or behind `capacity`: offsets[rows] is the size needed, and a caller that
+ * cannot bound it compares the two.  16 zero bytes behind the last text are written where they fit, so that the arena can go to
+ * tp_run_lines_device as it is.  workspace: tp_lines_workspace bytes (host function), aligned to 16.
+ */
+uint64_t tp_lines_workspace(uint64_t rows);
+int tp_grammar_lines(const tp_grammar* g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t rows,
+                     uint8_t* arena, uint64_t capacity, uint64_t* offsets, void* workspace, uint64_t workspace_bytes, void* stream);
+
 int tp_get_last_timing(const tp_ctx* ctx, tp_timing* out);
 
 #ifdef __cplusplus
