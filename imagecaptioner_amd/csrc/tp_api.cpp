@@ -1870,10 +1870,13 @@ tp_grammar* tp_grammar_create(tp_ctx* ctx, const tp_grammar_config* cfg) {
         g->info = h.info;
         OnDevice d(ctx->device);
         g->dev.begin = upload(g->owned, h.begin);
-        g->dev.token = upload(g->owned, h.token);
-        g->dev.move = upload(g->owned, h.move);
+        std::vector<uint2> pairs(h.token.size());
+        for (size_t e = 0; e < pairs.size(); ++e) { pairs[e].x = (uint32_t)h.token[e]; pairs[e].y = h.move[e]; }
+        g->dev.entry = upload(g->owned, pairs);
+        pairs.resize(h.info.n_tokens);
+        for (size_t t = 0; t < pairs.size(); ++t) { pairs[t].x = h.text_begin[t]; pairs[t].y = h.text_begin[t + 1] - h.text_begin[t]; }
+        g->dev.span = upload(g->owned, pairs);
         g->dev.text = upload(g->owned, h.text);
-        g->dev.text_begin = upload(g->owned, h.text_begin);
         g->dev.n_tokens = h.info.n_tokens;
         g->dev.n_places = h.info.n_prefixes + 2;
         g->dev.min_tags = h.min_tags;

@@ -48,7 +48,8 @@ const char* check_lines(const int32_t* tokens, uint64_t stride, uint32_t width, 
 constexpr uint32_t LOGIT_CHUNK = 8192;
 constexpr uint64_t MAX_REPLY_ROWS = (uint64_t)1 << 31;
 inline uint32_t logit_chunks(uint32_t vocab) { return (vocab + LOGIT_CHUNK - 1) / LOGIT_CHUNK; }
-struct ChoicePart { float best; int32_t token; double sum; };   // of one chunk: max z, the lowest token that has it, sum of exp(z - max z)
+constexpr int CHUNK_SEGMENTS = 16;
+struct ChoicePart { float best; int32_t token; float sum[CHUNK_SEGMENTS]; };   // of one chunk: the largest x, the lowest token that has it, the weights' sums of its segments
 uint64_t choose_workspace(uint64_t rows, uint32_t vocab);
 uint64_t lines_workspace(uint64_t rows);
 

@@ -1,6 +1,7 @@
 // Launchers of the kernels that write replies (tp_reply.hip), used by the C ABI layer (tp_api.cpp).
 #pragma once
 #include <hip/hip_runtime_api.h>
+#include <hip/hip_vector_types.h>
 #include <stdint.h>
 
 #include "../../include/tagpipe.h"
@@ -10,11 +11,10 @@ namespace tp {
 
 // A compiled grammar in device memory.
 struct DevGrammar {
-    const uint32_t* begin;        // HostGrammar's arrays
-    const int32_t* token;
-    const uint32_t* move;
-    const uint8_t* text;
-    const uint32_t* text_begin;
+    const uint32_t* begin;        // HostGrammar::begin
+    const uint2* entry;           // per entry: token, move
+    const uint8_t* text;          // the tokens' bytes
+    const uint2* span;            // per token: first byte, bytes
     uint32_t n_tokens, n_places;  // places 0 .. n_places - 1 (the end among them)
     uint32_t min_tags, max_tags;
 };

@@ -170,8 +170,10 @@ def test_masked_places_may_hold_anything(pipe, name):
 
 
 def check_choice(token, logprob, xs, sizes, temperature, uniform):
-    """The token against the 64-bit distribution.  z is off by e = (5 + 1) half steps of the largest intermediate over T, a weight exp(z - m) by 2 e + the
-    difference's half step + expf's (2 steps at most: 4 half steps), each relative; u * sum may fall on the other side of a border by that share of the sum."""
+    """The token against the 64-bit distribution.  z = x / T is off by e = (5 + 1) half steps of the largest intermediate over T.  A weight is 2^((x - m) * k): the
+    difference, the product and k (log2 e and its quotient by T: two) are off by four half steps relative, which moves the weight by 4 half steps times |ln w|;
+    the power itself is off by one step (two half steps), and a sum of 512 weights in 32 bits by its nine levels.  u * sum may fall on the other side of
+    a border by that share of the sum."""
     for r, x in enumerate(xs):
         t = float(temperature[r]) if temperature is not None and uniform is not None and temperature[r] > 0 else 0.0
         got, lp = int(token[r]), float(logprob[r])
@@ -183,7 +185,7 @@ def check_choice(token, logprob, xs, sizes, temperature, uniform):
         e = 6 * HALF32 * (sizes[r][fine].max() if fine.any() else 0) / (t or 1.0)
         spread = np.abs(z[fine] - z[fine].max()) if fine.any() else np.zeros(1)
         live = spread[spread < 104]                                       # expf is 0 below -104
-        share = 2 * e + HALF32 * (live.max() if len(live) else 0) + 4 * HALF32
+        share = 2 * e + 4 * HALF32 * (live.max() if len(live) else 0) + (2 + 9) * HALF32
         assert 0 <= got < len(x) and w[got] > 0, r
         if t > 0:
             cum, total = np.cumsum(w), w.sum()
