@@ -46,8 +46,8 @@ bool fits(uint64_t rows, uint64_t stride, uint64_t bytes) { return stride == 0 |
 }  // namespace
 
 uint64_t choose_workspace(uint64_t rows, uint32_t vocab) {
-    const uint64_t c = logit_chunks(vocab);
-    return c > 1 && rows <= MAX_REPLY_ROWS ? rows * c * sizeof(ChoicePart) : 0;
+    // a vocabulary that any launch's window holds needs none
+    return vocab > 8 * REPLY_SEGMENT && rows <= MAX_REPLY_ROWS ? (rows * reply_segments(vocab) * sizeof(ChoicePart) + 15) / 16 * 16 : 0;
 }
 
 uint64_t lines_workspace(uint64_t rows) { return rows <= MAX_REPLY_ROWS ? (rows + 4) / 4 * 16 + (rows / 256 + 4) * 8 : 0; }

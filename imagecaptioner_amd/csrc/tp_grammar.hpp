@@ -43,13 +43,11 @@ const char* check_step(uint32_t n_tokens, const tp_logits* io, const float* temp
 const char* check_lines(const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t rows, const uint8_t* arena, uint64_t capacity, const uint64_t* offsets,
                         const void* workspace, uint64_t workspace_bytes);
 
-// Tokens of one block of the logit kernels; a row of more is shared by several blocks, whose partial results the
-// choice's second launch joins.
-constexpr uint32_t LOGIT_CHUNK = 8192;
 constexpr uint64_t MAX_REPLY_ROWS = (uint64_t)1 << 31;
-inline uint32_t logit_chunks(uint32_t vocab) { return (vocab + LOGIT_CHUNK - 1) / LOGIT_CHUNK; }
-constexpr int CHUNK_SEGMENTS = 16;
-struct ChoicePart { float best; int32_t token; float sum[CHUNK_SEGMENTS]; };   // of one chunk: the largest x, the lowest token that has it, the weights' sums of its segments
+// The choice of a token joins segments of a row: of each the largest x, and the sum of the weights against it.
+constexpr uint32_t REPLY_SEGMENT = 1024;
+constexpr uint32_t reply_segments(uint32_t vocab) { return (vocab + REPLY_SEGMENT - 1) / REPLY_SEGMENT; }
+struct ChoicePart { float best, sum; };
 uint64_t choose_workspace(uint64_t rows, uint32_t vocab);
 uint64_t lines_workspace(uint64_t rows);
 

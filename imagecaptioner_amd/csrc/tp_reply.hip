@@ -2,6 +2,8 @@
 // and steps, and the written tokens as text.  The formulas are in include/tagpipe.h.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "tp_reply.h"
 #include "tp_launch.h"
 
@@ -13,20 +15,56 @@ constexpr uint32_t SEEN = 0x80000000u;         // a token's count word: stands i
 constexpr float NEG_INF = -__builtin_inff();
 
 // ---- element types --------------------------------------------------------------------------------------------------------
+// Pointers into device memory as the kernels hold them: told to be global memory, so that their accesses are global ones with
+// the row's start in scalar registers.
+template <class E>
+using Glob = const E __attribute__((address_space(1)))*;
+template <class E>
+__device__ inline Glob<E> glob(const E* p) { return (Glob<E>)p; }
+typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+template <class E> struct At;                     // four words at an address that is only a multiple of an element's size
+template <> struct At<uint16_t> { typedef Words4 W __attribute__((aligned(2))); };
+template <> struct At<uint32_t> { typedef Words4 W __attribute__((aligned(4))); };
+
 // Logits of every type are worked on in 32 bits; the one rounding back to 16 bits (to nearest, ties to even) is the store of
-// tp_shape_logits.
+// tp_shape_logits.  S: an element's bits; VEC: groups of four words that eight elements take.
 struct TF32 {
-    using S = float;
-    static __device__ float up(S v) { return v; }
-    static __device__ S down(float v) { return v; }
+    using S = uint32_t;
+    static constexpr int VEC = 2;
+    static __device__ float up(S v) { return __builtin_bit_cast(float, v); }
+    static __device__ S down(float v) { return __builtin_bit_cast(uint32_t, v); }
+    static __device__ void up8(const Words4 (&d)[2], float (&x)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = up(d[j >> 2][j & 3]);
+    }
+    static __device__ void down8(const float (&x)[8], Words4 (&d)[2]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j >> 2][j & 3] = down(x[j]);
+    }
 };
-struct TF16 {
-    using S = _Float16;
-    static __device__ float up(S v) { return (float)v; }
-    static __device__ S down(float v) { return (_Float16)v; }
+template <class T>
+struct Pairs {                                      // two elements a word
+    static __device__ void up8(const Words4 (&d)[1], float (&x)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            x[j] = T::up((uint16_t)d[0][j >> 1]);
+            x[j + 1] = T::up((uint16_t)(d[0][j >> 1] >> 16));
+        }
+    }
+    static __device__ void down8(const float (&x)[8], Words4 (&d)[1]) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) d[0][j >> 1] = (uint32_t)T::down(x[j]) | (uint32_t)T::down(x[j + 1]) << 16;
+    }
 };
-struct TBF16 {
+struct TF16 : Pairs<TF16> {
     using S = uint16_t;
+    static constexpr int VEC = 1;
+    static __device__ float up(S v) { return (float)__builtin_bit_cast(_Float16, v); }
+    static __device__ S down(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+};
+struct TBF16 : Pairs<TBF16> {
+    using S = uint16_t;
+    static constexpr int VEC = 1;
     static __device__ float up(S v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
     static __device__ S down(float v) {
         const uint32_t u = __builtin_bit_cast(uint32_t, v);
@@ -37,36 +75,38 @@ struct TBF16 {
 
 // ---- one row's rules ------------------------------------------------------------------------------------------------------
 struct RowRules {
-    const int32_t* history;       // null: nothing to count
+    Glob<int32_t> history;        // `len` of them
     uint32_t len, prompt;
     float rep, freq, pres;
-    const float* bias;            // null: none
-    const uint8_t* mask;          // the mask row's bytes, null: none
+    Glob<float> bias;             // null: none
+    Glob<uint8_t> mask;           // the mask row's bytes, null: none
 };
 
 __device__ inline uint32_t clamp_len(int32_t n, uint32_t cap) { return n < 0 ? 0u : (uint32_t)n > cap ? cap : (uint32_t)n; }
 
 __device__ inline RowRules row_rules(const tp_logits& a, uint64_t row) {
     RowRules r;
-    r.len = a.history ? (a.history_len ? clamp_len(a.history_len[row], a.history_cap) : a.history_cap) : 0u;
+    r.len = a.history ? (a.history_len ? clamp_len(glob(a.history_len)[row], a.history_cap) : a.history_cap) : 0u;
     if (!a.repetition && !a.frequency && !a.presence) r.len = 0;       // nothing asks what the history holds
-    r.history = a.history + row * a.history_stride;
-    r.prompt = a.prompt_len ? clamp_len(a.prompt_len[row], a.history_cap) : 0u;
-    r.rep = a.repetition ? a.repetition[row] : 1.0f;
-    r.freq = a.frequency ? a.frequency[row] : 0.0f;
-    r.pres = a.presence ? a.presence[row] : 0.0f;
+    r.history = glob(a.history) + row * a.history_stride;
+    r.prompt = a.prompt_len ? clamp_len(glob(a.prompt_len)[row], a.history_cap) : 0u;
+    r.rep = a.repetition ? glob(a.repetition)[row] : 1.0f;
+    r.freq = a.frequency ? glob(a.frequency)[row] : 0.0f;
+    r.pres = a.presence ? glob(a.presence)[row] : 0.0f;
     r.bias = nullptr;
     if (a.bias) {
-        const uint32_t b = a.bias_row ? (uint32_t)a.bias_row[row] : 0u;
-        if (b < a.n_bias) r.bias = a.bias + (uint64_t)b * a.bias_stride;
+        const uint32_t b = a.bias_row ? (uint32_t)glob(a.bias_row)[row] : 0u;
+        if (b < a.n_bias) r.bias = glob(a.bias) + (uint64_t)b * a.bias_stride;
     }
     r.mask = nullptr;
     if (a.mask) {
-        const uint32_t m = a.mask_row ? (uint32_t)a.mask_row[row] : 0u;
-        if (m < a.n_masks) r.mask = (const uint8_t*)(a.mask + (uint64_t)m * a.mask_stride);
+        const uint32_t m = a.mask_row ? (uint32_t)glob(a.mask_row)[row] : 0u;
+        if (m < a.n_masks) r.mask = (Glob<uint8_t>)(glob(a.mask) + (uint64_t)m * a.mask_stride);
     }
     return r;
 }
+template <class T>
+__device__ inline Glob<typename T::S> logit_row(const tp_logits& a, uint64_t row) { return glob((const typename T::S*)a.logits) + row * a.stride; }
 
 // The penalties of a token whose count word is c.  -ffp-contract=off: every operation rounds by itself, as the formula says.
 __device__ inline float penalised(float x, uint32_t c, const RowRules& r) {
@@ -112,6 +152,15 @@ __device__ inline double wave_sum(double v) {
     return v;
 }
 // sum of the lanes up to and including this one
+__device__ inline uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 __device__ inline double wave_scan(double v) {
     const int lane = (int)(threadIdx.x & 63);
     for (int d = 1; d < 64; d <<= 1) {
@@ -164,193 +213,293 @@ __device__ inline bool block_any(bool v) {
     }
 }
 
-// ---- shaping of a dense row, in windows -----------------------------------------------------------------------------------------
-// THREADS threads take a window of THREADS * VECS * 8 tokens of one row, VECS vectors of eight each, whose loads stand in flight while the
-// history is worked on.  Of the history only the tokens inside the window count: their counts are taken in an LDS table (a word
-// per token; only the words that are hit are cleared), then one thread per distinct token works the penalties out, with the token's logit
-// of its own load, and leaves the result in the token's word and a bit in a bitmap.  A vector then looks at one byte of the bitmap:
-// the penalties' arithmetic, a division among it, is done once per repeated token instead of once per token of the row, and a
-// window that the history does not reach stops after the first look.  A vector whose eight mask bits are all 0 is not loaded.
-template <int THREADS, int VECS>
-struct Window {
-    static constexpr uint32_t TOKENS = THREADS * VECS * 8;
-    struct Lds {
-        alignas(16) uint32_t word[TOKENS];
-        alignas(16) uint32_t seen[TOKENS / 32];
-    };
-    // the first token of this thread's vector v within the window
-    static __device__ uint32_t at(int v) { return (uint32_t)v * THREADS * 8 + threadIdx.x * 8; }
+// ---- a row in segments ----------------------------------------------------------------------------------------------------------
+constexpr uint32_t SEGMENT = REPLY_SEGMENT;
+constexpr int VECS = (int)(SEGMENT / (64 * 8));
+extern __shared__ uint32_t dynamic_lds[];
 
-    // whether the history has a token inside the window of `inside` tokens from w0; if so their penalised logits stand in LDS
-    template <class T>
-    static __device__ bool repeated(const RowRules& r, const typename T::S* l, uint32_t w0, uint32_t inside, Lds& s) {
-        if (!r.len) return false;
-        const uint32_t tid = threadIdx.x, h0 = tid < r.len ? (uint32_t)r.history[tid] - w0 : 0xFFFFFFFFu;
-        bool any = h0 < inside;
-        if (any) s.word[h0] = 0;
-        for (uint32_t k = tid + THREADS; k < r.len; k += THREADS) {
-            const uint32_t t = (uint32_t)r.history[k] - w0;
-            if (t < inside) { s.word[t] = 0; any = true; }
-        }
-        for (uint32_t k = tid; k < TOKENS / 32; k += THREADS) s.seen[k] = 0;
-        if (!block_any<THREADS>(any)) return false;
-        auto count = [&](uint32_t k, uint32_t t) { if (t < inside) { if (k >= r.prompt) atomicAdd(&s.word[t], 1u); else atomicOr(&s.word[t], SEEN); } };
-        count(tid, h0);
-        for (uint32_t k = tid + THREADS; k < r.len; k += THREADS) count(k, (uint32_t)r.history[k] - w0);
-        block_sync<THREADS>();
-        auto claim = [&](uint32_t t) {
-            if (t >= inside) return;
-            const uint32_t bit = 1u << (t & 31);
-            if (!(atomicOr(&s.seen[t >> 5], bit) & bit)) s.word[t] = __builtin_bit_cast(uint32_t, penalised(T::up(l[t]), s.word[t], r));
-        };
-        claim(h0);
-        for (uint32_t k = tid + THREADS; k < r.len; k += THREADS) claim((uint32_t)r.history[k] - w0);
-        block_sync<THREADS>();
-        return true;
-    }
-
-    template <class T>
-    static __device__ void shaped(const tp_logits& a, const RowRules& r, uint64_t row, uint32_t w0, Lds& s, float (&x)[VECS][8]) {
-        using S = typename T::S;
-        const S* l = (const S*)a.logits + row * a.stride + w0;
-        const uint32_t n = a.vocab - w0;                                   // tokens from here to the row's end
-        uint32_t allowed[VECS];
-        S raw[VECS][8] = {};
-#pragma unroll
-        for (int v = 0; v < VECS; ++v) allowed[v] = at(v) < n ? (r.mask ? r.mask[(w0 + at(v)) >> 3] : 0xFFu) : 0u;
-#pragma unroll
-        for (int v = 0; v < VECS; ++v) {
-            if (!allowed[v]) continue;
-            if (at(v) + 8 <= n) {
-                __builtin_memcpy(raw[v], l + at(v), sizeof raw[v]);           // rows may start at any element
-            } else {
-                allowed[v] &= 0xFFu >> (8 - (n - at(v)));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) if (at(v) + j < n) raw[v][j] = l[at(v) + j];
-            }
-        }
-        const bool hits = repeated<T>(r, l, w0, n < TOKENS ? n : TOKENS, s);
-#pragma unroll
-        for (int v = 0; v < VECS; ++v) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[v][j] = T::up(raw[v][j]);
-            const uint32_t hit = hits ? ((const uint8_t*)s.seen)[at(v) >> 3] : 0u;
-            if (hit) {
-                float y[8];
-                __builtin_memcpy(y, __builtin_assume_aligned(s.word + at(v), 16), sizeof y);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[v][j] = hit >> j & 1 ? y[j] : x[v][j];
-            }
-            if (r.bias && allowed[v]) {
-                float b[8];
-                if (at(v) + 8 <= n) {
-                    __builtin_memcpy(b, r.bias + w0 + at(v), sizeof b);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) b[j] = at(v) + j < n ? r.bias[w0 + at(v) + j] : 0.0f;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[v][j] = x[v][j] + b[j];
-            }
-            if (allowed[v] != 0xFFu) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[v][j] = allowed[v] >> j & 1 ? x[v][j] : NEG_INF;
-            }
-        }
-    }
-};
-
-constexpr int CHUNK_THREADS = 512;
-constexpr int CHUNK_VECS = (int)(LOGIT_CHUNK / (CHUNK_THREADS * 8));
-using Chunk = Window<CHUNK_THREADS, CHUNK_VECS>;
-static_assert(Chunk::TOKENS == LOGIT_CHUNK, "a chunk is whole vectors");
-
+// A wave's segment of a row: two vectors of eight tokens a lane.  `at`: the lane's first token within the window, 512 less than its second vector's.
 template <class T>
-__global__ __launch_bounds__(CHUNK_THREADS) void k_shape(tp_logits a, uint64_t block0, uint32_t chunks, void* out, uint64_t out_stride) {
+struct Held {
+    Words4 d[VECS][T::VEC];
+    uint32_t allowed[VECS];                                                   // a vector's mask bits, 0 behind the row's end
+};
+__device__ inline uint32_t lane_at(uint32_t segment) { return segment * SEGMENT + (threadIdx.x & 63) * 8; }
+
+// `n`: tokens from the window's start to the row's end.  A segment that the end cuts is loaded token by token where a vector is cut.
+template <class T>
+__device__ inline void load_segment(const RowRules& r, Glob<typename T::S> row, uint32_t w0, uint32_t n, uint32_t segment, Held<T>& h) {
     using S = typename T::S;
-    __shared__ Chunk::Lds s;
-    const uint64_t b = block0 + blockIdx.x, row = b / chunks;
-    const uint32_t c0 = (uint32_t)(b % chunks) * LOGIT_CHUNK;
-    float x[CHUNK_VECS][8];
-    Chunk::shaped<T>(a, row_rules(a, row), row, c0, s, x);
-    S* o = (S*)out + row * out_stride + c0;
-    const uint32_t n = a.vocab - c0;
+    using V = const typename At<S>::W __attribute__((address_space(1)));
+    const uint32_t at = lane_at(segment);
 #pragma unroll
-    for (int v = 0; v < CHUNK_VECS; ++v) {
-        const uint32_t at = Chunk::at(v);
-        S raw[8];
+    for (int v = 0; v < VECS; ++v) {
+        h.allowed[v] = 0xFFu;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) raw[j] = T::down(x[v][j]);
-        if (at + 8 <= n) {
-            __builtin_memcpy(o + at, raw, sizeof raw);
+        for (int g = 0; g < T::VEC; ++g) h.d[v][g] = Words4{0, 0, 0, 0};
+    }
+    if ((segment + 1) * SEGMENT <= n) {
+        if (r.mask) {
+#pragma unroll
+            for (int v = 0; v < VECS; ++v) h.allowed[v] = r.mask[(w0 + at + v * 512) >> 3];
+#pragma unroll
+            for (int v = 0; v < VECS; ++v)
+                if (h.allowed[v])
+#pragma unroll
+                    for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((V*)(row + at + v * 512))[g];
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) if (at + j < n) o[at + j] = raw[j];
+            for (int v = 0; v < VECS; ++v)
+#pragma unroll
+                for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((V*)(row + at + v * 512))[g];
+        }
+        return;
+    }
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+        const uint32_t t = at + v * 512;
+        if (t >= n) { h.allowed[v] = 0; continue; }
+        if (r.mask) h.allowed[v] = r.mask[(w0 + t) >> 3];
+        if (t + 8 <= n) {
+#pragma unroll
+            for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((V*)(row + t))[g];
+            continue;
+        }
+        h.allowed[v] &= 0xFFu >> (8 - (n - t));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t bits = t + j < n ? (uint32_t)row[t + j] : 0u;
+            if constexpr (sizeof(S) == 4) h.d[v][j >> 2][j & 3] = bits;
+            else h.d[v][0][j >> 1] |= bits << (16 * (j & 1));
+        }
+    }
+}
+// the bias, and -infinity where `take` has no bit
+__device__ inline void finish_segment(const RowRules& r, uint32_t w0, uint32_t n, uint32_t segment, const uint32_t (&take)[VECS], float (&x)[VECS][8]) {
+    using V = const At<uint32_t>::W __attribute__((address_space(1)));
+    const uint32_t at = lane_at(segment);
+    if (r.bias) {
+        if ((segment + 1) * SEGMENT <= n) {
+            Words4 b[VECS][2];
+#pragma unroll
+            for (int v = 0; v < VECS; ++v) { b[v][0] = ((V*)(r.bias + w0 + at + v * 512))[0]; b[v][1] = ((V*)(r.bias + w0 + at + v * 512))[1]; }
+#pragma unroll
+            for (int v = 0; v < VECS; ++v)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[v][j] = x[v][j] + __builtin_bit_cast(float, (uint32_t)b[v][j >> 2][j & 3]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VECS; ++v)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) if (at + v * 512 + j < n) x[v][j] = x[v][j] + r.bias[w0 + at + v * 512 + j];
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < VECS; ++v)
+        if (take[v] != 0xFFu) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[v][j] = take[v] >> j & 1 ? x[v][j] : NEG_INF;
+        }
+}
+
+// ---- shaping ------------------------------------------------------------------------------------------------------------------------
+// Bound by reading and writing the logits once.  A block takes 8192 tokens of one row, a segment a wave; the loads stand in flight while the
+// block counts the history in an LDS table of a word per token, of which it clears all and every thread looks at some of the
+// row's whole history.  The penalties are worked out where a token's word is not 0.  (The choice below keeps only as many words as
+// the history has entries and works each repeated token out once; here, with the vector units idle, its longer chain of
+// barriers costs more than it saves: 77 against 54 us for 256 x 131071 float32 with 1500 entries of history.)
+constexpr int SHAPE_WAVES = 8;
+constexpr uint32_t SHAPE_TOKENS = SHAPE_WAVES * SEGMENT;
+
+template <class T>
+__global__ __launch_bounds__(SHAPE_WAVES * 64) void k_shape(tp_logits a, uint64_t block0, uint32_t chunks, void* out, uint64_t out_stride) {
+    using S = typename T::S;
+    using V = typename At<S>::W __attribute__((address_space(1)));
+    constexpr uint32_t THREADS = SHAPE_WAVES * 64;
+    __shared__ alignas(16) uint32_t cnt[SHAPE_TOKENS];
+    const uint64_t b = block0 + blockIdx.x, row = b / chunks;
+    const uint32_t w0 = (uint32_t)(b % chunks) * SHAPE_TOKENS, n = a.vocab - w0, tid = threadIdx.x;
+    const uint32_t g = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), at = lane_at(g);
+    auto* o = (S __attribute__((address_space(1)))*)((S*)out + row * out_stride + w0);
+    const RowRules r = row_rules(a, row);
+    Held<T> h;
+    load_segment<T>(r, logit_row<T>(a, row) + w0, w0, n, g, h);
+    if (r.len) {
+        for (uint32_t k = tid * 4; k < SHAPE_TOKENS; k += THREADS * 4) *(uint4*)(cnt + k) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        const uint32_t inside = n < SHAPE_TOKENS ? n : SHAPE_TOKENS;
+        for (uint32_t k = tid; k < r.len; k += THREADS) {
+            const uint32_t t = (uint32_t)r.history[k] - w0;
+            if (t < inside) { if (k >= r.prompt) atomicAdd(&cnt[t], 1u); else atomicOr(&cnt[t], SEEN); }
+        }
+        __syncthreads();
+    }
+    if (g * SEGMENT >= n) return;
+    float x[VECS][8];
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+        T::up8(h.d[v], x[v]);
+        if (r.len) {
+            uint32_t c[8];
+            __builtin_memcpy(c, __builtin_assume_aligned(cnt + at + v * 512, 16), sizeof c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[v][j] = penalised(x[v][j], c[j], r);
+        }
+    }
+    finish_segment(r, w0, n, g, h.allowed, x);
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+        const uint32_t t = at + v * 512;
+        Words4 d[T::VEC];
+        T::down8(x[v], d);
+        if ((g + 1) * SEGMENT <= n || t + 8 <= n) {
+#pragma unroll
+            for (int k = 0; k < T::VEC; ++k) ((V*)(o + t))[k] = d[k];
+        } else if (t < n) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) if (t + j < n) o[t + j] = T::down(x[v][j]);
         }
     }
 }
 
-// ---- the choice -------------------------------------------------------------------------------------------------------------
-// The first launch reads the logits once: per chunk the largest x and, against it, the sums of the weights of 16 segments of 512
-// tokens.  The second joins a row's chunks with one wave: the token's chunk by a scan of the chunks' sums, its segment
-// by a scan of the segments', and the token itself in the one segment, which the wave shapes again (1 KB of the row).  A row of
-// one chunk does both in the first launch.  Segment sums are 32-bit sums of at most 512 weights in a tree of 9 levels; everything above is summed in 64.
-constexpr int SEGMENT = 512;
-using Segment = Window<64, 1>;
-static_assert(Segment::TOKENS == SEGMENT && CHUNK_SEGMENTS * SEGMENT == LOGIT_CHUNK && CHUNK_VECS * CHUNK_THREADS / 64 == CHUNK_SEGMENTS, "a wave's vector of a chunk is a segment");
+// ---- repeated tokens of a window ------------------------------------------------------------------------------------------------
+// For the choice, which the vector units bound: the tokens of the history inside a window of a row are marked in a bitmap, a prefix sum over
+// its words ranks them, and the distinct ones' counts are taken in an array as long as the history has room for.  One
+// thread per distinct token then works its x out, with a load of the token's own logit, and puts it in the count's place.  The
+// vectors leave these tokens out: the penalties' arithmetic, a division among it, is done once per repeated token instead
+// of once per token of the row.  The first segment's loads are in flight meanwhile.
+template <int WAVES, int SEGS>
+struct Window {
+    static constexpr int THREADS = WAVES * 64;
+    static constexpr uint32_t TOKENS = (uint32_t)WAVES * SEGS * SEGMENT, WORDS = TOKENS / 32;
+    static constexpr int MINE = (int)((WORDS + THREADS - 1) / THREADS);    // bitmap words of a thread
+    struct Lds {
+        alignas(16) uint32_t seen[WORDS];
+        uint32_t claimed[WORDS];
+        uint32_t rank[WORDS + 1];                                             // distinct tokens before the word
+        uint32_t wave[WAVES];
+    };
+    // `value`, in dynamic LDS: the distinct tokens' x, in token order; as many words as the history has entries, or the window tokens
 
-struct ChunkLds {
-    float max[CHUNK_THREADS / 64];
-    uint32_t first;
-    ChoicePart part;
+    static __device__ uint32_t tid() { return threadIdx.x % THREADS; }
+    static __device__ uint32_t rank_of(const Lds& l, uint32_t t) { return l.rank[t >> 5] + (uint32_t)__popc(l.seen[t >> 5] & ((1u << (t & 31)) - 1)); }
+
+    // How many distinct tokens of the window of `inside` tokens from w0 the history has; their x stand in `value`.
+    template <class T>
+    static __device__ uint32_t repeated(const RowRules& r, Glob<typename T::S> row, uint32_t w0, uint32_t inside, Lds& l, uint32_t* value) {
+        if (!r.len) return 0;
+        const uint32_t words = (inside + SEGMENT - 1) / SEGMENT * (SEGMENT / 32);      // the bitmap's, in whole segments
+        const uint32_t h0 = tid() < r.len ? (uint32_t)r.history[tid()] - w0 : 0xFFFFFFFFu;   // the thread's first token stays in a register
+        for (uint32_t k = tid(); k < words; k += THREADS) l.seen[k] = l.claimed[k] = 0;
+        block_sync<THREADS>();
+        bool any = false;
+        for (uint32_t k = tid(), t = h0; k < r.len;) {
+            if (t < inside) { atomicOr(&l.seen[t >> 5], 1u << (t & 31)); any = true; }
+            k += THREADS;
+            t = k < r.len ? (uint32_t)r.history[k] - w0 : 0xFFFFFFFFu;
+        }
+        if (!block_any<THREADS>(any)) return 0;
+        uint32_t n[MINE], mine = 0;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) { n[i] = tid() * MINE + i < words ? (uint32_t)__popc(l.seen[tid() * MINE + i]) : 0u; mine += n[i]; }
+        const uint32_t incl = wave_scan(mine);
+        uint32_t before = incl - mine, distinct = 0;
+        if constexpr (WAVES > 1) {
+            if ((tid() & 63) == 63) l.wave[tid() >> 6] = incl;
+            block_sync<THREADS>();
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) { if (w < (int)(tid() >> 6)) before += l.wave[w]; distinct += l.wave[w]; }
+        } else {
+            distinct = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+        }
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) if (tid() * MINE + i < words) { l.rank[tid() * MINE + i] = before; before += n[i]; }
+        if (tid() == 0) l.rank[words] = distinct;
+        for (uint32_t k = tid(); k < distinct; k += THREADS) value[k] = 0;
+        block_sync<THREADS>();
+        for (uint32_t k = tid(), t = h0; k < r.len;) {
+            if (t < inside) { if (k >= r.prompt) atomicAdd(&value[rank_of(l, t)], 1u); else atomicOr(&value[rank_of(l, t)], SEEN); }
+            k += THREADS;
+            t = k < r.len ? (uint32_t)r.history[k] - w0 : 0xFFFFFFFFu;
+        }
+        block_sync<THREADS>();
+        for (uint32_t k = tid(), t = h0; k < r.len;) {
+            if (t < inside) {
+                const uint32_t bit = 1u << (t & 31);
+                if (!(atomicOr(&l.claimed[t >> 5], bit) & bit)) {
+                    const uint32_t i = rank_of(l, t);
+                    float x = penalised(T::up(row[t]), value[i], r);
+                    if (r.bias) x = x + r.bias[w0 + t];
+                    if (r.mask && !(r.mask[(w0 + t) >> 3] >> (t & 7) & 1)) x = NEG_INF;
+                    value[i] = __builtin_bit_cast(uint32_t, x);
+                }
+            }
+            k += THREADS;
+            t = k < r.len ? (uint32_t)r.history[k] - w0 : 0xFFFFFFFFu;
+        }
+        block_sync<THREADS>();
+        return distinct;
+    }
+
 };
 
-// The chunk's part of the choice; `out` is complete for the whole block after the next barrier.
-__device__ void chunk_part(float (&x)[CHUNK_VECS][8], float t, uint32_t c0, ChunkLds& l, ChoicePart* out) {
-    const int wave = (int)(threadIdx.x >> 6);
-    float best = NEG_INF;
+// ---- the choice -------------------------------------------------------------------------------------------------------------
+// The first launch reads the logits once and leaves of every segment the largest x and the sum of the weights against it; a wave does
+// that by itself.  The second joins a row with one wave: the token's segment by a scan of the segments' shares, and the token in that segment, which
+// the wave shapes again (1024 tokens of the row).  A row of one window does both in the first launch.  A segment's sum is a 32-bit sum of 1024
+// weights in a tree of 10 levels; everything above is summed in 64.
+using OneSegment = Window<1, 1>;
+constexpr int CHOICE_WAVES = 16, MOST_SEGS = 8;                               // waves of a block, segments of a wave at the most
+using Chunk = Window<CHOICE_WAVES, MOST_SEGS>;
+
+template <class T>
+__device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32_t n, uint32_t g, const Held<T>& h, float k, uint32_t distinct, const Chunk::Lds& l, const uint32_t* value) {
+    float x[VECS][8], best = NEG_INF;
+    uint32_t take[VECS], i0 = 0, i1 = 0;
 #pragma unroll
-    for (int v = 0; v < CHUNK_VECS; ++v)
+    for (int v = 0; v < VECS; ++v) take[v] = h.allowed[v];
+    if (distinct) {
+        i0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)l.rank[g * (SEGMENT / 32)]);
+        i1 = (uint32_t)__builtin_amdgcn_readfirstlane((int)l.rank[(g + 1) * (SEGMENT / 32)]);
+        if (i1 > i0) {
+#pragma unroll
+            for (int v = 0; v < VECS; ++v) take[v] &= ~(uint32_t)((const uint8_t*)l.seen)[(lane_at(g) + v * 512) >> 3];
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) T::up8(h.d[v], x[v]);
+    finish_segment(r, w0, n, g, take, x);
+#pragma unroll
+    for (int v = 0; v < VECS; ++v)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             x[v][j] = countable(x[v][j]);
             best = fmaxf(best, x[v][j]);
         }
+    for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) best = fmaxf(best, countable(__builtin_bit_cast(float, value[i])));
     best = wave_max(best);
-    if ((threadIdx.x & 63) == 0) l.max[wave] = best;
-    if (threadIdx.x == 0) l.first = 0xFFFFFFFFu;
-    __syncthreads();
-    best = l.max[0];
+    if (!(best > NEG_INF)) return ChoicePart{best, 0.0f};
+    float sum = 0.0f;
 #pragma unroll
-    for (int w = 1; w < CHUNK_THREADS / 64; ++w) best = fmaxf(best, l.max[w]);
-    best = read_lane(best, 0);                                            // the same in every lane: the cases below are branches of the wave
-    const float k = weight_scale(t);
-#pragma unroll
-    for (int v = 0; v < CHUNK_VECS; ++v) {
+    for (int v = 0; v < VECS; ++v) {
         float w[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = best > NEG_INF ? weight(x[v][j], best, k) : 0.0f;
-        const float sum = wave_sum(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-        if ((threadIdx.x & 63) == 0) out->sum[v * (CHUNK_THREADS / 64) + wave] = sum;
+        for (int j = 0; j < 8; ++j) w[j] = weight(x[v][j], best, k);
+        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     }
-    if (t == 0.0f) {                                                      // the lowest token of the largest x
-        uint32_t first = 0xFFFFFFFFu;
-#pragma unroll
-        for (int v = CHUNK_VECS - 1; v >= 0; --v)
-#pragma unroll
-            for (int j = 7; j >= 0; --j) if (x[v][j] == best) first = c0 + Chunk::at(v) + j;
-        if (first != 0xFFFFFFFFu) atomicMin(&l.first, first);
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) { out->best = best; out->token = (int32_t)l.first; }
+    for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) sum += weight(countable(__builtin_bit_cast(float, value[i])), best, k);
+    return ChoicePart{best, wave_sum(sum)};
 }
 
-// Joins a row's chunks: all lanes of one wave.
-template <class T>
-__device__ void join_row(const tp_logits& a, uint64_t row, uint32_t chunks, const ChoicePart* p, float t, const float* uniform, int32_t* tokens, float* logprob, Segment::Lds& s) {
+// Joins a row's segments: all lanes of one wave.  Tables: Chunk where the row's own window stands in LDS (`distinct` of it), OneSegment
+// where the segment's repeated tokens are still to be found.
+template <class T, class Tables>
+__device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, uint32_t segments, const ChoicePart* p, float t, const float* uniform, int32_t* tokens,
+                         float* logprob, uint32_t distinct, typename Tables::Lds& l, uint32_t* value) {
+    constexpr bool HERE = Tables::TOKENS > SEGMENT;
     const uint32_t lane = threadIdx.x & 63;
     float best = NEG_INF;
-    for (uint32_t c = lane; c < chunks; c += 64) best = fmaxf(best, p[c].best);
+    for (uint32_t c = lane; c < segments; c += 64) best = fmaxf(best, p[c].best);
     best = wave_max(best);
     if (!(best > NEG_INF)) {
         if (lane == 0) {
@@ -360,110 +509,124 @@ __device__ void join_row(const tp_logits& a, uint64_t row, uint32_t chunks, cons
         return;
     }
     const float k = weight_scale(t);
-    auto share = [&](uint32_t c) {
-        if (c >= chunks || !(p[c].best > NEG_INF)) return 0.0;
-        double w = 0.0;
-#pragma unroll
-        for (int i = 0; i < CHUNK_SEGMENTS; ++i) w += (double)p[c].sum[i];
-        return w * (double)weight(p[c].best, best, k);
-    };
+    auto share = [&](uint32_t c) { return c < segments && p[c].best > NEG_INF ? (double)p[c].sum * (double)weight(p[c].best, best, k) : 0.0; };
     double sum = 0.0;
-    uint32_t greedy = 0xFFFFFFFFu;
-    for (uint32_t c = lane; c < chunks; c += 64) {
-        sum += share(c);
-        if (p[c].best == best && (uint32_t)p[c].token < greedy) greedy = (uint32_t)p[c].token;
-    }
+    for (uint32_t c = lane; c < segments; c += 64) sum += share(c);
     sum = wave_sum(sum);
-    if (t == 0.0f) {
-        for (int d = 32; d; d >>= 1) {
-            const uint32_t o = (uint32_t)__shfl_xor((int)greedy, d, 64);
-            greedy = o < greedy ? o : greedy;
+    // Greedy: the first segment that has the largest x.  Sampled: the first whose cumulative share exceeds the target; where there is none (rounding,
+    // or a `uniform` of 1 or more) the last of a share above 0, and so within the segment.
+    double target = t > 0.0f ? (double)uniform[row] * sum : 0.0, carry = 0.0, before = 0.0;
+    uint32_t segment = 0;
+    bool found = false;
+    for (uint32_t c0 = 0; c0 < segments && !found; c0 += 64) {
+        const double w = share(c0 + lane), incl = carry + wave_scan(w);
+        const uint64_t live = __ballot(w > 0.0);
+        const uint64_t over = t > 0.0f ? __ballot(w > 0.0 && incl > target) : __ballot(c0 + lane < segments && p[c0 + lane].best == best);
+        if (over || (live && t > 0.0f)) {
+            found = over != 0;
+            const int to = found ? __builtin_ctzll(over) : 63 - __builtin_clzll(live);
+            segment = c0 + (uint32_t)to;
+            before = __shfl(incl - w, to, 64);
         }
-        if (lane == 0) {
-            tokens[row] = (int32_t)greedy;
-            if (logprob) logprob[row] = (float)-log(sum);
-        }
-        return;
+        carry = __shfl(incl, 63, 64);
     }
-    // Where rounding, or a `uniform` of 1 or more, leaves no place whose cumulative weight exceeds the target, the last place
-    // of a weight above 0 is taken, at every level.
-    double target = (double)uniform[row] * sum;
-    uint32_t chunk = 0;
-    {
-        double carry = 0.0, before = 0.0;
-        bool found = false;
-        for (uint32_t c0 = 0; c0 < chunks && !found; c0 += 64) {
-            const double w = share(c0 + lane), incl = carry + wave_scan(w);
-            const uint64_t live = __ballot(w > 0.0), over = __ballot(w > 0.0 && incl > target);
-            if (live) {
-                found = over != 0;
-                const int at = found ? __builtin_ctzll(over) : 63 - __builtin_clzll(live);
-                chunk = c0 + (uint32_t)at;
-                before = __shfl(incl - w, at, 64);
+    const float segment_best = p[segment].best;
+    target = (target - before) / (double)weight(segment_best, best, k);
+    const uint32_t w0 = segment * SEGMENT, n = a.vocab - w0, l0 = HERE ? w0 : 0;             // l0: the segment's start within the tables
+    const auto from = logit_row<T>(a, row) + w0;
+    Held<T> h;
+    load_segment<T>(r, from, w0, n, 0, h);
+    if constexpr (!HERE) distinct = OneSegment::repeated<T>(r, from, w0, n < SEGMENT ? n : SEGMENT, l, value);
+    uint32_t at = 0;
+    float x_at = best;
+    bool done = false;
+    double run = 0.0;
+    float xs[VECS][8];
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) T::up8(h.d[v], xs[v]);
+    finish_segment(r, w0, n, 0, h.allowed, xs);
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+        if (done) continue;
+        float (&x)[8] = xs[v];
+        const uint32_t t0 = l0 + lane_at(0) + v * 512, hit = distinct ? (uint32_t)((const uint8_t*)l.seen)[t0 >> 3] : 0u;
+        if (hit) {
+            uint32_t i = Tables::rank_of(l, t0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) if (hit >> j & 1) x[j] = __builtin_bit_cast(float, value[i++]);
+        }
+        uint32_t first = 8, last = 8;
+        float x_first = best, x_last = best;
+        if (t > 0.0f) {
+            float w[8];
+            double mine = 0.0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j] = weight(countable(x[j]), segment_best, k);
+                mine += (double)w[j];
             }
-            carry = __shfl(incl, 63, 64);
-        }
-        target = (target - before) / (double)weight(p[chunk].best, best, k);
-    }
-    uint32_t segment;
-    {
-        const double w = lane < CHUNK_SEGMENTS ? (double)p[chunk].sum[lane] : 0.0, incl = wave_scan(w);
-        const uint64_t live = __ballot(w > 0.0), over = __ballot(w > 0.0 && incl > target);
-        segment = (uint32_t)(over ? __builtin_ctzll(over) : 63 - __builtin_clzll(live));
-        target -= __shfl(incl - w, (int)segment, 64);
-    }
-    const float chunk_best = p[chunk].best;
-    const uint32_t w0 = chunk * LOGIT_CHUNK + segment * SEGMENT;
-    float x[1][8];
-    Segment::shaped<T>(a, row_rules(a, row), row, w0, s, x);
-    double cum = 0.0;
-    float w[8];
+            const double incl = run + wave_scan(mine);
+            double cum = incl - mine;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        w[j] = weight(countable(x[0][j]), chunk_best, k);
-        cum += (double)w[j];
-    }
-    double run = wave_scan(cum) - cum;
-    uint32_t first = 8, last = 8;
-    float x_first = 0.0f, x_last = 0.0f;
+            for (int j = 0; j < 8; ++j) {
+                cum += (double)w[j];
+                if (w[j] > 0.0f) {
+                    last = (uint32_t)j; x_last = x[j];
+                    if (first == 8 && cum > target) { first = (uint32_t)j; x_first = x[j]; }
+                }
+            }
+            run = __shfl(incl, 63, 64);
+        } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        run += (double)w[j];
-        if (w[j] > 0.0f) {
-            last = (uint32_t)j; x_last = x[0][j];
-            if (first == 8 && run > target) { first = (uint32_t)j; x_first = x[0][j]; }
+            for (int j = 7; j >= 0; --j) if (x[j] == best) first = (uint32_t)j;
         }
+        const uint64_t over = __ballot(first < 8), live = __ballot(last < 8);
+        if (!over && !live) continue;
+        done = over != 0;
+        const int to = done ? __builtin_ctzll(over) : 63 - __builtin_clzll(live);
+        at = (uint32_t)v * 512 + (uint32_t)to * 8 + (uint32_t)__shfl((int)(done ? first : last), to, 64);
+        x_at = __shfl(done ? x_first : x_last, to, 64);
     }
-    const uint64_t over = __ballot(first < 8), live = __ballot(last < 8);
-    const uint32_t at = (uint32_t)(over ? __builtin_ctzll(over) : 63 - __builtin_clzll(live));
-    if (lane == at) {
-        tokens[row] = (int32_t)(w0 + lane * 8 + (over ? first : last));
-        if (logprob) logprob[row] = log_probability(over ? x_first : x_last, best, t, sum);
+    if (lane == 0) {
+        tokens[row] = (int32_t)(w0 + at);
+        if (logprob) logprob[row] = log_probability(x_at, best, t, sum);
     }
 }
 
 template <class T>
-__global__ __launch_bounds__(CHUNK_THREADS) void k_choose(tp_logits a, uint64_t block0, uint32_t chunks, const float* temperature, const float* uniform,
-                                                          int32_t* tokens, float* logprob, ChoicePart* parts) {
-    __shared__ union { Chunk::Lds chunk; Segment::Lds segment; } s;
-    __shared__ ChunkLds l;
+__global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_eu(8))) void k_choose(tp_logits a, uint64_t block0, uint32_t chunks, uint32_t segs, const float* temperature,
+                                                                                                     const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
+    __shared__ Chunk::Lds l;
+    __shared__ ChoicePart here[CHOICE_WAVES * MOST_SEGS];
     const uint64_t b = block0 + blockIdx.x, row = b / chunks;
-    const uint32_t c0 = (uint32_t)(b % chunks) * LOGIT_CHUNK;
-    float x[CHUNK_VECS][8];
-    Chunk::shaped<T>(a, row_rules(a, row), row, c0, s.chunk, x);
-    const float t = temperature_of(temperature, uniform, row);
-    chunk_part(x, t, c0, l, chunks > 1 ? parts + b : &l.part);
+    const uint32_t window = segs * CHOICE_WAVES * SEGMENT, w0 = (uint32_t)(b % chunks) * window, n = a.vocab - w0, segments = reply_segments(a.vocab);
+    const float t = temperature_of(temperature, uniform, row), k = weight_scale(t);
+    const RowRules r = row_rules(a, row);
+    const auto from = logit_row<T>(a, row) + w0;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * CHOICE_WAVES, reply_segments(n));
+    Held<T> now, next;
+    if (wave < last) load_segment<T>(r, from, w0, n, wave, now);
+    const uint32_t distinct = Chunk::repeated<T>(r, from, w0, std::min(n, window), l, dynamic_lds);
+    for (uint32_t g = wave; g < last; g += CHOICE_WAVES) {
+        if (g + CHOICE_WAVES < last) load_segment<T>(r, from, w0, n, g + CHOICE_WAVES, next);   // the next one's loads are in flight while this one is worked on
+        const ChoicePart p = segment_part<T>(r, w0, n, g, now, k, distinct, l, dynamic_lds);
+        if ((threadIdx.x & 63) == 0) {
+            if (chunks > 1) parts[row * segments + w0 / SEGMENT + g] = p; else here[g] = p;
+        }
+        now = next;
+    }
     if (chunks > 1) return;
     __syncthreads();
-    if (threadIdx.x < 64) join_row<T>(a, row, 1, &l.part, t, uniform, tokens, logprob, s.segment);
+    if (threadIdx.x < 64) join_row<T, Chunk>(a, r, row, segments, here, t, uniform, tokens, logprob, distinct, l, dynamic_lds);
 }
 
 template <class T>
-__global__ __launch_bounds__(64) void k_choose_join(tp_logits a, uint64_t row0, uint32_t chunks, const float* temperature, const float* uniform,
-                                                    int32_t* tokens, float* logprob, const ChoicePart* parts) {
-    __shared__ Segment::Lds s;
+__global__ __launch_bounds__(64) void k_choose_join(tp_logits a, uint64_t row0, const float* temperature, const float* uniform, int32_t* tokens, float* logprob,
+                                                    const ChoicePart* parts) {
+    __shared__ OneSegment::Lds l;
     const uint64_t row = row0 + blockIdx.x;
-    join_row<T>(a, row, chunks, parts + row * chunks, temperature_of(temperature, uniform, row), uniform, tokens, logprob, s);
+    const uint32_t segments = reply_segments(a.vocab);
+    join_row<T, OneSegment>(a, row_rules(a, row), row, segments, parts + row * segments, temperature_of(temperature, uniform, row), uniform, tokens, logprob, 0, l, dynamic_lds);
 }
 
 // ---- the grammar ----------------------------------------------------------------------------------------------------------------
@@ -564,13 +727,17 @@ struct Step {
     // x of the m entries from e0: entry i of the piece is thread i % THREADS's number i / THREADS; -infinity where it may not be taken
     template <class T>
     static __device__ void shaped(const DevGrammar& g, const tp_logits& a, const RowRules& r, uint64_t row, uint32_t tags, uint32_t e0, uint32_t m, Lds& s, uint2 (&en)[EACH], float (&x)[EACH]) {
-        const typename T::S* l = (const typename T::S*)a.logits + row * a.stride;
+        const auto l = logit_row<T>(a, row);
+        const auto entries = (Glob<unsigned long long>)(glob((const unsigned long long*)g.entry) + e0);
         const uint32_t tid = threadIdx.x;
         bool ok[EACH];
         typename T::S raw[EACH];
         float b[EACH];
 #pragma unroll
-        for (int v = 0; v < EACH; ++v) en[v] = (uint32_t)v * THREADS + tid < m ? g.entry[e0 + v * THREADS + tid] : make_uint2(0xFFFFFFFFu, 0);
+        for (int v = 0; v < EACH; ++v) {
+            const unsigned long long e = (uint32_t)v * THREADS + tid < m ? entries[v * THREADS + tid] : 0xFFFFFFFFull;
+            en[v] = make_uint2((uint32_t)e, (uint32_t)(e >> 32));
+        }
 #pragma unroll
         for (int v = 0; v < EACH; ++v) {
             ok[v] = en[v].x != 0xFFFFFFFFu && may(en[v].y, tags, g);
@@ -825,25 +992,38 @@ hipError_t by_type(int32_t type, F&& f) {
 }  // namespace
 
 hipError_t launch_shape(const tp_logits& io, void* out, uint64_t out_stride) {
-    const uint32_t chunks = logit_chunks(io.vocab);
+    const uint32_t chunks = (io.vocab + SHAPE_TOKENS - 1) / SHAPE_TOKENS;
     return by_type(io.type, [&](auto tag) {
         using T = decltype(tag);
         return in_ranges(io.rows * chunks, [&](uint64_t b, unsigned n) {
-            hipLaunchKernelGGL(k_shape<T>, dim3(n), dim3(CHUNK_THREADS), 0, (hipStream_t)io.stream, io, b, chunks, out, out_stride);
+            hipLaunchKernelGGL(k_shape<T>, dim3(n), dim3(SHAPE_WAVES * 64), 0, (hipStream_t)io.stream, io, b, chunks, out, out_stride);
         });
     });
 }
 
+// Segments a wave of the choice takes, one after another.  More of them let fewer blocks read the row's history, and a row that
+// is one block's needs no second launch; fewer let a small call use more compute units: as many as still give every compute unit
+// its two blocks.  A window must also keep its repeated tokens in 64 KB of LDS.
+static uint32_t window_segments(const tp_logits& io) {
+    for (uint32_t segs = MOST_SEGS; segs > 1; segs /= 2) {
+        const uint64_t tokens = (uint64_t)CHOICE_WAVES * segs * SEGMENT;
+        if (tokens > 16384 && io.history && io.history_cap > 4096) continue;
+        if (tokens / 2 < io.vocab && io.rows * ((io.vocab + tokens - 1) / tokens) >= 512) return segs;
+    }
+    return 1;
+}
+
 hipError_t launch_choose(const tp_logits& io, const float* temperature, const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
-    const uint32_t chunks = logit_chunks(io.vocab);
+    const uint32_t segs = window_segments(io), window = segs * CHOICE_WAVES * SEGMENT, chunks = (io.vocab + window - 1) / window;
+    const uint32_t lds = io.history ? std::min(io.history_cap, window) * 4 : 0, lds_one = io.history ? std::min(io.history_cap, SEGMENT) * 4 : 0;
     return by_type(io.type, [&](auto tag) {
         using T = decltype(tag);
         hipError_t e = in_ranges(io.rows * chunks, [&](uint64_t b, unsigned n) {
-            hipLaunchKernelGGL(k_choose<T>, dim3(n), dim3(CHUNK_THREADS), 0, (hipStream_t)io.stream, io, b, chunks, temperature, uniform, tokens, logprob, parts);
+            hipLaunchKernelGGL(k_choose<T>, dim3(n), dim3(CHOICE_WAVES * 64), lds, (hipStream_t)io.stream, io, b, chunks, segs, temperature, uniform, tokens, logprob, parts);
         });
         if (e != hipSuccess || chunks == 1) return e;
         return in_ranges(io.rows, [&](uint64_t b, unsigned n) {
-            hipLaunchKernelGGL(k_choose_join<T>, dim3(n), dim3(64), 0, (hipStream_t)io.stream, io, b, chunks, temperature, uniform, tokens, logprob, parts);
+            hipLaunchKernelGGL(k_choose_join<T>, dim3(n), dim3(64), lds_one, (hipStream_t)io.stream, io, b, temperature, uniform, tokens, logprob, parts);
         });
     });
 }

@@ -172,7 +172,7 @@ def test_masked_places_may_hold_anything(pipe, name):
 def check_choice(token, logprob, xs, sizes, temperature, uniform):
     """The token against the 64-bit distribution.  z = x / T is off by e = (5 + 1) half steps of the largest intermediate over T.  A weight is 2^((x - m) * k): the
     difference, the product and k (log2 e and its quotient by T: two) are off by four half steps relative, which moves the weight by 4 half steps times |ln w|;
-    the power itself is off by one step (two half steps), and a sum of 512 weights in 32 bits by its nine levels.  u * sum may fall on the other side of
+    the power itself is off by one step (two half steps), and a sum of 1024 weights in 32 bits by its ten levels.  u * sum may fall on the other side of
     a border by that share of the sum."""
     for r, x in enumerate(xs):
         t = float(temperature[r]) if temperature is not None and uniform is not None and temperature[r] > 0 else 0.0
@@ -185,7 +185,7 @@ def check_choice(token, logprob, xs, sizes, temperature, uniform):
         e = 6 * HALF32 * (sizes[r][fine].max() if fine.any() else 0) / (t or 1.0)
         spread = np.abs(z[fine] - z[fine].max()) if fine.any() else np.zeros(1)
         live = spread[spread < 104]                                       # expf is 0 below -104
-        share = 2 * e + 4 * HALF32 * (live.max() if len(live) else 0) + (2 + 9) * HALF32
+        share = 2 * e + 4 * HALF32 * (live.max() if len(live) else 0) + (2 + 10) * HALF32
         assert 0 <= got < len(x) and w[got] > 0, r
         if t > 0:
             cum, total = np.cumsum(w), w.sum()
@@ -195,6 +195,25 @@ def check_choice(token, logprob, xs, sizes, temperature, uniform):
             assert z[got] >= z.max() - 2 * e, (r, got)
         want = (0.0 if z[got] == z.max() else z[got] - z.max()) - math.log(w.sum())
         assert abs(lp - want) <= 2 * e + 2 * share + 2 * HALF32 * abs(want), (r, lp, want)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 50021), (3, 9000), (1, 200001), (520, 17000)])
+def test_long_histories(pipe, rows, vocab):
+    """More history than a launch keeps of it at once, most of it distinct."""
+    rng = np.random.default_rng(rows)
+    logits, l = make_logits(rng, rows, vocab, torch.float16)
+    rules = Rules(rng, rows, vocab, history=20000 if rows < 500 else 4200, bias=1)
+    rules.history[:, ::2] = rng.integers(0, vocab, size=rules.history[:, ::2].shape)
+    rules.args["history"] = dev(rules.history)
+    temperature, uniform = choice_numbers(rng, rows)
+    some = range(rows) if rows < 500 else [0, 1, 2, 259, 519]
+    got = pipe.shape_logits(logits, **rules.args)
+    token, logprob = (v.cpu().numpy() for v in pipe.choose_tokens(logits, temperature=dev(temperature), uniform=dev(uniform), **rules.args))
+    if rows < 500:
+        check_shaped(got, l, rules, torch.float16)
+    xs, sizes, _ = zip(*(rules.plain(l[r], r) for r in some))
+    some = list(some)
+    check_choice(token[some], logprob[some], xs, sizes, temperature[some], uniform[some])
 
 
 def choice_numbers(rng, rows):
