@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "tp_reply.h"
 #include "tp_launch.h"
@@ -84,25 +85,25 @@ struct RowRules {
 
 __device__ inline uint32_t clamp_len(int32_t n, uint32_t cap) { return n < 0 ? 0u : (uint32_t)n > cap ? cap : (uint32_t)n; }
 
+// Every rule is one load from where it stands or from a zero, and none waits for another: a row's block begins with one round of
+// memory latency instead of one per rule.
+__device__ const uint32_t no_rule[1] = {0};
 __device__ inline RowRules row_rules(const tp_logits& a, uint64_t row) {
+    const auto none = glob((const float*)no_rule);
+    const auto none_i = glob((const int32_t*)no_rule);
+    const int32_t len = *(a.history_len ? glob(a.history_len) + row : none_i), prompt = *(a.prompt_len ? glob(a.prompt_len) + row : none_i);
+    const float rep = *(a.repetition ? glob(a.repetition) + row : none), freq = *(a.frequency ? glob(a.frequency) + row : none), pres = *(a.presence ? glob(a.presence) + row : none);
+    const uint32_t bias = (uint32_t)*(a.bias_row ? glob(a.bias_row) + row : none_i), mask = (uint32_t)*(a.mask_row ? glob(a.mask_row) + row : none_i);
     RowRules r;
-    r.len = a.history ? (a.history_len ? clamp_len(glob(a.history_len)[row], a.history_cap) : a.history_cap) : 0u;
-    if (!a.repetition && !a.frequency && !a.presence) r.len = 0;       // nothing asks what the history holds
+    const bool asked = a.history && (a.repetition || a.frequency || a.presence);       // else nothing asks what the history holds
+    r.len = asked ? (a.history_len ? clamp_len(len, a.history_cap) : a.history_cap) : 0u;
     r.history = glob(a.history) + row * a.history_stride;
-    r.prompt = a.prompt_len ? clamp_len(glob(a.prompt_len)[row], a.history_cap) : 0u;
-    r.rep = a.repetition ? glob(a.repetition)[row] : 1.0f;
-    r.freq = a.frequency ? glob(a.frequency)[row] : 0.0f;
-    r.pres = a.presence ? glob(a.presence)[row] : 0.0f;
-    r.bias = nullptr;
-    if (a.bias) {
-        const uint32_t b = a.bias_row ? (uint32_t)glob(a.bias_row)[row] : 0u;
-        if (b < a.n_bias) r.bias = glob(a.bias) + (uint64_t)b * a.bias_stride;
-    }
-    r.mask = nullptr;
-    if (a.mask) {
-        const uint32_t m = a.mask_row ? (uint32_t)glob(a.mask_row)[row] : 0u;
-        if (m < a.n_masks) r.mask = (Glob<uint8_t>)(glob(a.mask) + (uint64_t)m * a.mask_stride);
-    }
+    r.prompt = clamp_len(prompt, a.history_cap);
+    r.rep = a.repetition ? rep : 1.0f;
+    r.freq = freq;
+    r.pres = pres;
+    r.bias = a.bias && bias < a.n_bias ? glob(a.bias) + (uint64_t)bias * a.bias_stride : nullptr;
+    r.mask = a.mask && mask < a.n_masks ? (Glob<uint8_t>)(glob(a.mask) + (uint64_t)mask * a.mask_stride) : nullptr;
     return r;
 }
 template <class T>
@@ -218,80 +219,87 @@ constexpr uint32_t SEGMENT = REPLY_SEGMENT;
 constexpr int VECS = (int)(SEGMENT / (64 * 8));
 extern __shared__ uint32_t dynamic_lds[];
 
-// A wave's segment of a row: two vectors of eight tokens a lane.  `at`: the lane's first token within the window, 512 less than its second vector's.
+// A wave's segment of a row: two vectors of eight tokens a lane, the lane's second 512 tokens behind its first.  A vector that the row's end cuts is loaded
+// from eight tokens before the end instead, so that every lane loads alike; its first `cut` tokens belong to the vector before and
+// are left out by their bits of `take`.  (TINY: a vocabulary of fewer than eight tokens, loaded one by one.)
 template <class T>
 struct Held {
     Words4 d[VECS][T::VEC];
-    uint32_t allowed[VECS];                                                   // a vector's mask bits, 0 behind the row's end
+    uint32_t take[VECS];                                                      // tokens that are this lane's, inside the row and allowed by the mask
 };
 __device__ inline uint32_t lane_at(uint32_t segment) { return segment * SEGMENT + (threadIdx.x & 63) * 8; }
+// how far the vector at t reaches over the end of n tokens: 0 not, 8 it lies behind it
+__device__ inline uint32_t cut_of(uint32_t t, uint32_t n) { return t + 8 <= n ? 0u : t < n ? t + 8 - n : 8u; }
 
-// `n`: tokens from the window's start to the row's end.  A segment that the end cuts is loaded token by token where a vector is cut.
-template <class T>
+template <class E>
+using Vec = const typename At<E>::W __attribute__((address_space(1)));
+
+// `n`: tokens from the window's start to the row's end
+template <class T, bool TINY>
 __device__ inline void load_segment(const RowRules& r, Glob<typename T::S> row, uint32_t w0, uint32_t n, uint32_t segment, Held<T>& h) {
     using S = typename T::S;
-    using V = const typename At<S>::W __attribute__((address_space(1)));
     const uint32_t at = lane_at(segment);
+    if constexpr (TINY) {
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) {
-        h.allowed[v] = 0xFFu;
+        for (int v = 0; v < VECS; ++v) {
+            const uint32_t t = at + v * 512, cut = cut_of(t, n);
+            const uint32_t bits = r.mask ? (uint32_t)r.mask[0] : 0xFFu;
+            h.take[v] = cut < 8 ? bits << cut & 0xFFu : 0u;
 #pragma unroll
-        for (int g = 0; g < T::VEC; ++g) h.d[v][g] = Words4{0, 0, 0, 0};
-    }
-    if ((segment + 1) * SEGMENT <= n) {
-        if (r.mask) {
+            for (int g = 0; g < T::VEC; ++g) h.d[v][g] = Words4{0, 0, 0, 0};
 #pragma unroll
-            for (int v = 0; v < VECS; ++v) h.allowed[v] = r.mask[(w0 + at + v * 512) >> 3];
-#pragma unroll
-            for (int v = 0; v < VECS; ++v)
-                if (h.allowed[v])
-#pragma unroll
-                    for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((V*)(row + at + v * 512))[g];
-        } else {
-#pragma unroll
-            for (int v = 0; v < VECS; ++v)
-#pragma unroll
-                for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((V*)(row + at + v * 512))[g];
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t e = cut < 8 && (uint32_t)j >= cut ? (uint32_t)row[j - cut] : 0u;
+                if constexpr (sizeof(S) == 4) h.d[v][j >> 2][j & 3] = e;
+                else h.d[v][0][j >> 1] |= e << (16 * (j & 1));
+            }
         }
         return;
     }
+    if (r.mask) {
+        uint32_t bits[VECS];
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) {
-        const uint32_t t = at + v * 512;
-        if (t >= n) { h.allowed[v] = 0; continue; }
-        if (r.mask) h.allowed[v] = r.mask[(w0 + t) >> 3];
-        if (t + 8 <= n) {
+        for (int v = 0; v < VECS; ++v) bits[v] = r.mask[(w0 + std::min(at + v * 512, n - 1)) >> 3];
 #pragma unroll
-            for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((V*)(row + t))[g];
-            continue;
+        for (int v = 0; v < VECS; ++v) {
+            const uint32_t t = at + v * 512;
+            h.take[v] = bits[v] << cut_of(t, n) & 0xFFu;
+            if (h.take[v])
+#pragma unroll
+                for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((Vec<S>*)(row + (int32_t)std::min((int32_t)t, (int32_t)n - 8)))[g];
         }
-        h.allowed[v] &= 0xFFu >> (8 - (n - t));
+    } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t bits = t + j < n ? (uint32_t)row[t + j] : 0u;
-            if constexpr (sizeof(S) == 4) h.d[v][j >> 2][j & 3] = bits;
-            else h.d[v][0][j >> 1] |= bits << (16 * (j & 1));
+        for (int v = 0; v < VECS; ++v) {
+            const uint32_t t = at + v * 512;
+            h.take[v] = 0xFFu << cut_of(t, n) & 0xFFu;
+#pragma unroll
+            for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((Vec<S>*)(row + (int32_t)std::min((int32_t)t, (int32_t)n - 8)))[g];
         }
     }
 }
 // the bias, and -infinity where `take` has no bit
+template <bool TINY>
 __device__ inline void finish_segment(const RowRules& r, uint32_t w0, uint32_t n, uint32_t segment, const uint32_t (&take)[VECS], float (&x)[VECS][8]) {
-    using V = const At<uint32_t>::W __attribute__((address_space(1)));
     const uint32_t at = lane_at(segment);
     if (r.bias) {
-        if ((segment + 1) * SEGMENT <= n) {
+        if constexpr (TINY) {
+#pragma unroll
+            for (int v = 0; v < VECS; ++v)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) if (take[v] >> j & 1) x[v][j] = x[v][j] + r.bias[j - cut_of(at + v * 512, n)];
+        } else {
             Words4 b[VECS][2];
 #pragma unroll
-            for (int v = 0; v < VECS; ++v) { b[v][0] = ((V*)(r.bias + w0 + at + v * 512))[0]; b[v][1] = ((V*)(r.bias + w0 + at + v * 512))[1]; }
+            for (int v = 0; v < VECS; ++v) {
+                auto* from = (Vec<uint32_t>*)(r.bias + w0 + (int32_t)std::min((int32_t)(at + v * 512), (int32_t)n - 8));
+                b[v][0] = from[0];
+                b[v][1] = from[1];
+            }
 #pragma unroll
             for (int v = 0; v < VECS; ++v)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[v][j] = x[v][j] + __builtin_bit_cast(float, (uint32_t)b[v][j >> 2][j & 3]);
-        } else {
-#pragma unroll
-            for (int v = 0; v < VECS; ++v)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) if (at + v * 512 + j < n) x[v][j] = x[v][j] + r.bias[w0 + at + v * 512 + j];
         }
     }
 #pragma unroll
@@ -302,6 +310,31 @@ __device__ inline void finish_segment(const RowRules& r, uint32_t w0, uint32_t n
         }
 }
 
+// A row's history as a block of THREADS threads goes through it: HELD entries a thread in registers, loaded before
+// anything else is, the others again from memory in every pass.
+template <int THREADS, int HELD>
+struct History {
+    uint32_t token[HELD];                                                     // as they stand there: nothing waits for them here
+    __device__ inline void load(const RowRules& r, uint32_t w0) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+            const uint32_t k = threadIdx.x % THREADS + i * THREADS;
+            token[i] = k < r.len ? (uint32_t)r.history[k] : w0 - 1;              // no token: a distance of 2^32 - 1
+        }
+    }
+    // f(whether the entry counts for frequency and presence, distance from w0), for distances below `inside`
+    template <class F>
+    __device__ inline void each(const RowRules& r, uint32_t w0, uint32_t inside, F&& f) const {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (token[i] - w0 < inside) f(threadIdx.x % THREADS + i * THREADS >= r.prompt, token[i] - w0);
+        for (uint32_t k = threadIdx.x % THREADS + HELD * THREADS; k < r.len; k += THREADS) {
+            const uint32_t h = (uint32_t)r.history[k] - w0;
+            if (h < inside) f(k >= r.prompt, h);
+        }
+    }
+};
+
 // ---- shaping ------------------------------------------------------------------------------------------------------------------------
 // Bound by reading and writing the logits once.  A block takes 8192 tokens of one row, a segment a wave; the loads stand in flight while the
 // block counts the history in an LDS table of a word per token, of which it clears all and every thread looks at some of the
@@ -311,27 +344,25 @@ __device__ inline void finish_segment(const RowRules& r, uint32_t w0, uint32_t n
 constexpr int SHAPE_WAVES = 8;
 constexpr uint32_t SHAPE_TOKENS = SHAPE_WAVES * SEGMENT;
 
-template <class T>
-__global__ __launch_bounds__(SHAPE_WAVES * 64) void k_shape(tp_logits a, uint64_t block0, uint32_t chunks, void* out, uint64_t out_stride) {
+template <class T, bool TINY>
+__global__ __launch_bounds__(SHAPE_WAVES * 64) __attribute__((amdgpu_waves_per_eu(8))) void k_shape(tp_logits a, uint64_t row0, void* out, uint64_t out_stride) {
     using S = typename T::S;
     using V = typename At<S>::W __attribute__((address_space(1)));
     constexpr uint32_t THREADS = SHAPE_WAVES * 64;
     __shared__ alignas(16) uint32_t cnt[SHAPE_TOKENS];
-    const uint64_t b = block0 + blockIdx.x, row = b / chunks;
-    const uint32_t w0 = (uint32_t)(b % chunks) * SHAPE_TOKENS, n = a.vocab - w0, tid = threadIdx.x;
-    const uint32_t g = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), at = lane_at(g);
+    const uint64_t row = row0 + blockIdx.y;
+    const uint32_t w0 = blockIdx.x * SHAPE_TOKENS, n = a.vocab - w0;
+    const uint32_t g = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), at = lane_at(g);
     auto* o = (S __attribute__((address_space(1)))*)((S*)out + row * out_stride + w0);
     const RowRules r = row_rules(a, row);
+    History<THREADS, 4> history;
+    history.load(r, w0);
     Held<T> h;
-    load_segment<T>(r, logit_row<T>(a, row) + w0, w0, n, g, h);
+    load_segment<T, TINY>(r, logit_row<T>(a, row) + w0, w0, n, g, h);
     if (r.len) {
-        for (uint32_t k = tid * 4; k < SHAPE_TOKENS; k += THREADS * 4) *(uint4*)(cnt + k) = make_uint4(0, 0, 0, 0);
+        for (uint32_t k = threadIdx.x * 4; k < SHAPE_TOKENS; k += THREADS * 4) *(uint4*)(cnt + k) = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        const uint32_t inside = n < SHAPE_TOKENS ? n : SHAPE_TOKENS;
-        for (uint32_t k = tid; k < r.len; k += THREADS) {
-            const uint32_t t = (uint32_t)r.history[k] - w0;
-            if (t < inside) { if (k >= r.prompt) atomicAdd(&cnt[t], 1u); else atomicOr(&cnt[t], SEEN); }
-        }
+        history.each(r, w0, std::min(n, SHAPE_TOKENS), [&](bool counted, uint32_t t) { if (counted) atomicAdd(&cnt[t], 1u); else atomicOr(&cnt[t], SEEN); });
         __syncthreads();
     }
     if (g * SEGMENT >= n) return;
@@ -340,24 +371,32 @@ __global__ __launch_bounds__(SHAPE_WAVES * 64) void k_shape(tp_logits a, uint64_
     for (int v = 0; v < VECS; ++v) {
         T::up8(h.d[v], x[v]);
         if (r.len) {
-            uint32_t c[8];
-            __builtin_memcpy(c, __builtin_assume_aligned(cnt + at + v * 512, 16), sizeof c);
+            const uint32_t t = at + v * 512, cut = cut_of(t, n);
+            if (cut == 0) {
+                uint32_t c[8];
+                __builtin_memcpy(c, __builtin_assume_aligned(cnt + t, 16), sizeof c);
+                if (c[0] | c[1] | c[2] | c[3] | c[4] | c[5] | c[6] | c[7]) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[v][j] = penalised(x[v][j], c[j], r);
+                    for (int j = 0; j < 8; ++j) x[v][j] = penalised(x[v][j], c[j], r);
+                }
+            } else if (cut < 8) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) if ((uint32_t)j >= cut) x[v][j] = penalised(x[v][j], cnt[t + j - cut], r);
+            }
         }
     }
-    finish_segment(r, w0, n, g, h.allowed, x);
+    finish_segment<TINY>(r, w0, n, g, h.take, x);
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
-        const uint32_t t = at + v * 512;
+        const uint32_t t = at + v * 512, cut = cut_of(t, n);
         Words4 d[T::VEC];
         T::down8(x[v], d);
-        if ((g + 1) * SEGMENT <= n || t + 8 <= n) {
+        if (cut == 0) {
 #pragma unroll
             for (int k = 0; k < T::VEC; ++k) ((V*)(o + t))[k] = d[k];
-        } else if (t < n) {
+        } else if (cut < 8) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) if (t + j < n) o[t + j] = T::down(x[v][j]);
+            for (int j = 0; j < 8; ++j) if ((uint32_t)j >= cut) o[t + j - cut] = T::down(x[v][j]);
         }
     }
 }
@@ -385,19 +424,14 @@ struct Window {
     static __device__ uint32_t rank_of(const Lds& l, uint32_t t) { return l.rank[t >> 5] + (uint32_t)__popc(l.seen[t >> 5] & ((1u << (t & 31)) - 1)); }
 
     // How many distinct tokens of the window of `inside` tokens from w0 the history has; their x stand in `value`.
-    template <class T>
-    static __device__ uint32_t repeated(const RowRules& r, Glob<typename T::S> row, uint32_t w0, uint32_t inside, Lds& l, uint32_t* value) {
+    template <class T, class H>
+    static __device__ uint32_t repeated(const RowRules& r, const H& history, Glob<typename T::S> row, uint32_t w0, uint32_t inside, Lds& l, uint32_t* value) {
         if (!r.len) return 0;
         const uint32_t words = (inside + SEGMENT - 1) / SEGMENT * (SEGMENT / 32);      // the bitmap's, in whole segments
-        const uint32_t h0 = tid() < r.len ? (uint32_t)r.history[tid()] - w0 : 0xFFFFFFFFu;   // the thread's first token stays in a register
         for (uint32_t k = tid(); k < words; k += THREADS) l.seen[k] = l.claimed[k] = 0;
         block_sync<THREADS>();
         bool any = false;
-        for (uint32_t k = tid(), t = h0; k < r.len;) {
-            if (t < inside) { atomicOr(&l.seen[t >> 5], 1u << (t & 31)); any = true; }
-            k += THREADS;
-            t = k < r.len ? (uint32_t)r.history[k] - w0 : 0xFFFFFFFFu;
-        }
+        history.each(r, w0, inside, [&](bool, uint32_t t) { atomicOr(&l.seen[t >> 5], 1u << (t & 31)); any = true; });
         if (!block_any<THREADS>(any)) return 0;
         uint32_t n[MINE], mine = 0;
 #pragma unroll
@@ -417,30 +451,21 @@ struct Window {
         if (tid() == 0) l.rank[words] = distinct;
         for (uint32_t k = tid(); k < distinct; k += THREADS) value[k] = 0;
         block_sync<THREADS>();
-        for (uint32_t k = tid(), t = h0; k < r.len;) {
-            if (t < inside) { if (k >= r.prompt) atomicAdd(&value[rank_of(l, t)], 1u); else atomicOr(&value[rank_of(l, t)], SEEN); }
-            k += THREADS;
-            t = k < r.len ? (uint32_t)r.history[k] - w0 : 0xFFFFFFFFu;
-        }
+        history.each(r, w0, inside, [&](bool counted, uint32_t t) { if (counted) atomicAdd(&value[rank_of(l, t)], 1u); else atomicOr(&value[rank_of(l, t)], SEEN); });
         block_sync<THREADS>();
-        for (uint32_t k = tid(), t = h0; k < r.len;) {
-            if (t < inside) {
-                const uint32_t bit = 1u << (t & 31);
-                if (!(atomicOr(&l.claimed[t >> 5], bit) & bit)) {
-                    const uint32_t i = rank_of(l, t);
-                    float x = penalised(T::up(row[t]), value[i], r);
-                    if (r.bias) x = x + r.bias[w0 + t];
-                    if (r.mask && !(r.mask[(w0 + t) >> 3] >> (t & 7) & 1)) x = NEG_INF;
-                    value[i] = __builtin_bit_cast(uint32_t, x);
-                }
-            }
-            k += THREADS;
-            t = k < r.len ? (uint32_t)r.history[k] - w0 : 0xFFFFFFFFu;
-        }
+        history.each(r, w0, inside, [&](bool, uint32_t t) {
+            const uint32_t bit = 1u << (t & 31);
+            if (atomicOr(&l.claimed[t >> 5], bit) & bit) return;
+            const uint32_t i = rank_of(l, t);
+            const float logit = T::up(row[t]), b = r.bias ? r.bias[w0 + t] : 0.0f;
+            float x = penalised(logit, value[i], r);
+            if (r.bias) x = x + b;
+            if (r.mask && !(r.mask[(w0 + t) >> 3] >> (t & 7) & 1)) x = NEG_INF;
+            value[i] = __builtin_bit_cast(uint32_t, x);
+        });
         block_sync<THREADS>();
         return distinct;
     }
-
 };
 
 // ---- the choice -------------------------------------------------------------------------------------------------------------
@@ -452,23 +477,26 @@ using OneSegment = Window<1, 1>;
 constexpr int CHOICE_WAVES = 16, MOST_SEGS = 8;                               // waves of a block, segments of a wave at the most
 using Chunk = Window<CHOICE_WAVES, MOST_SEGS>;
 
-template <class T>
+template <class T, bool TINY>
 __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32_t n, uint32_t g, const Held<T>& h, float k, uint32_t distinct, const Chunk::Lds& l, const uint32_t* value) {
     float x[VECS][8], best = NEG_INF;
     uint32_t take[VECS], i0 = 0, i1 = 0;
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) take[v] = h.allowed[v];
+    for (int v = 0; v < VECS; ++v) take[v] = h.take[v];
     if (distinct) {
         i0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)l.rank[g * (SEGMENT / 32)]);
         i1 = (uint32_t)__builtin_amdgcn_readfirstlane((int)l.rank[(g + 1) * (SEGMENT / 32)]);
         if (i1 > i0) {
 #pragma unroll
-            for (int v = 0; v < VECS; ++v) take[v] &= ~(uint32_t)((const uint8_t*)l.seen)[(lane_at(g) + v * 512) >> 3];
+            for (int v = 0; v < VECS; ++v) {
+                const uint32_t t = lane_at(g) + v * 512;
+                take[v] &= ~((uint32_t)((const uint8_t*)l.seen)[t >> 3] << cut_of(t, n));
+            }
         }
     }
 #pragma unroll
     for (int v = 0; v < VECS; ++v) T::up8(h.d[v], x[v]);
-    finish_segment(r, w0, n, g, take, x);
+    finish_segment<TINY>(r, w0, n, g, take, x);
 #pragma unroll
     for (int v = 0; v < VECS; ++v)
 #pragma unroll
@@ -493,7 +521,7 @@ __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32
 
 // Joins a row's segments: all lanes of one wave.  Tables: Chunk where the row's own window stands in LDS (`distinct` of it), OneSegment
 // where the segment's repeated tokens are still to be found.
-template <class T, class Tables>
+template <class T, class Tables, bool TINY>
 __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, uint32_t segments, const ChoicePart* p, float t, const float* uniform, int32_t* tokens,
                          float* logprob, uint32_t distinct, typename Tables::Lds& l, uint32_t* value) {
     constexpr bool HERE = Tables::TOKENS > SEGMENT;
@@ -535,8 +563,14 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     const uint32_t w0 = segment * SEGMENT, n = a.vocab - w0, l0 = HERE ? w0 : 0;             // l0: the segment's start within the tables
     const auto from = logit_row<T>(a, row) + w0;
     Held<T> h;
-    load_segment<T>(r, from, w0, n, 0, h);
-    if constexpr (!HERE) distinct = OneSegment::repeated<T>(r, from, w0, n < SEGMENT ? n : SEGMENT, l, value);
+    if constexpr (HERE) {
+        load_segment<T, TINY>(r, from, w0, n, 0, h);
+    } else {
+        History<64, 8> history;
+        history.load(r, w0);
+        load_segment<T, TINY>(r, from, w0, n, 0, h);
+        distinct = OneSegment::repeated<T>(r, history, from, w0, std::min(n, SEGMENT), l, value);
+    }
     uint32_t at = 0;
     float x_at = best;
     bool done = false;
@@ -544,12 +578,13 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     float xs[VECS][8];
 #pragma unroll
     for (int v = 0; v < VECS; ++v) T::up8(h.d[v], xs[v]);
-    finish_segment(r, w0, n, 0, h.allowed, xs);
+    finish_segment<TINY>(r, w0, n, 0, h.take, xs);
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
         if (done) continue;
         float (&x)[8] = xs[v];
-        const uint32_t t0 = l0 + lane_at(0) + v * 512, hit = distinct ? (uint32_t)((const uint8_t*)l.seen)[t0 >> 3] : 0u;
+        const uint32_t t0 = l0 + lane_at(0) + v * 512, cut = cut_of(lane_at(0) + v * 512, n);
+        const uint32_t hit = distinct && cut < 8 ? (uint32_t)((const uint8_t*)l.seen)[t0 >> 3] << cut & 0xFFu : 0u;
         if (hit) {
             uint32_t i = Tables::rank_of(l, t0);
 #pragma unroll
@@ -584,7 +619,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         if (!over && !live) continue;
         done = over != 0;
         const int to = done ? __builtin_ctzll(over) : 63 - __builtin_clzll(live);
-        at = (uint32_t)v * 512 + (uint32_t)to * 8 + (uint32_t)__shfl((int)(done ? first : last), to, 64);
+        at = (uint32_t)v * 512 + (uint32_t)to * 8 + (uint32_t)__shfl((int)((done ? first : last) - cut), to, 64);
         x_at = __shfl(done ? x_first : x_last, to, 64);
     }
     if (lane == 0) {
@@ -593,31 +628,39 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     }
 }
 
-template <class T>
-__global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_eu(8))) void k_choose(tp_logits a, uint64_t block0, uint32_t chunks, uint32_t segs, const float* temperature,
+template <class T, bool TINY>
+__global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_eu(8))) void k_choose(tp_logits a, uint64_t row0, uint32_t segs, const float* temperature,
                                                                                                      const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
     __shared__ Chunk::Lds l;
     __shared__ ChoicePart here[CHOICE_WAVES * MOST_SEGS];
-    const uint64_t b = block0 + blockIdx.x, row = b / chunks;
-    const uint32_t window = segs * CHOICE_WAVES * SEGMENT, w0 = (uint32_t)(b % chunks) * window, n = a.vocab - w0, segments = reply_segments(a.vocab);
+    const uint64_t row = row0 + blockIdx.y;
+    const uint32_t chunks = gridDim.x, window = segs * CHOICE_WAVES * SEGMENT, w0 = blockIdx.x * window, n = a.vocab - w0, segments = reply_segments(a.vocab);
     const float t = temperature_of(temperature, uniform, row), k = weight_scale(t);
     const RowRules r = row_rules(a, row);
     const auto from = logit_row<T>(a, row) + w0;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * CHOICE_WAVES, reply_segments(n));
-    Held<T> now, next;
-    if (wave < last) load_segment<T>(r, from, w0, n, wave, now);
-    const uint32_t distinct = Chunk::repeated<T>(r, from, w0, std::min(n, window), l, dynamic_lds);
-    for (uint32_t g = wave; g < last; g += CHOICE_WAVES) {
-        if (g + CHOICE_WAVES < last) load_segment<T>(r, from, w0, n, g + CHOICE_WAVES, next);   // the next one's loads are in flight while this one is worked on
-        const ChoicePart p = segment_part<T>(r, w0, n, g, now, k, distinct, l, dynamic_lds);
+    History<CHOICE_WAVES * 64, 2> history;
+    history.load(r, w0);
+    // two segments in turn: one's loads are in flight while the other is worked on (and stay in the registers they were sent to)
+    Held<T> even, odd;
+    if (wave < last) load_segment<T, TINY>(r, from, w0, n, wave, even);
+    const uint32_t distinct = Chunk::repeated<T>(r, history, from, w0, std::min(n, window), l, dynamic_lds);
+    ChoicePart* out = parts + row * segments + w0 / SEGMENT;
+    auto part = [&](uint32_t g, const Held<T>& h) {
+        const ChoicePart p = segment_part<T, TINY>(r, w0, n, g, h, k, distinct, l, dynamic_lds);
         if ((threadIdx.x & 63) == 0) {
-            if (chunks > 1) parts[row * segments + w0 / SEGMENT + g] = p; else here[g] = p;
+            if (chunks > 1) out[g] = p; else here[g] = p;
         }
-        now = next;
+    };
+    for (uint32_t g = wave; g < last; g += 2 * CHOICE_WAVES) {
+        if (g + CHOICE_WAVES < last) load_segment<T, TINY>(r, from, w0, n, g + CHOICE_WAVES, odd);
+        part(g, even);
+        if (g + 2 * CHOICE_WAVES < last) load_segment<T, TINY>(r, from, w0, n, g + 2 * CHOICE_WAVES, even);
+        if (g + CHOICE_WAVES < last) part(g + CHOICE_WAVES, odd);
     }
     if (chunks > 1) return;
     __syncthreads();
-    if (threadIdx.x < 64) join_row<T, Chunk>(a, r, row, segments, here, t, uniform, tokens, logprob, distinct, l, dynamic_lds);
+    if (threadIdx.x < 64) join_row<T, Chunk, TINY>(a, r, row, segments, here, t, uniform, tokens, logprob, distinct, l, dynamic_lds);
 }
 
 template <class T>
@@ -626,7 +669,7 @@ __global__ __launch_bounds__(64) void k_choose_join(tp_logits a, uint64_t row0, 
     __shared__ OneSegment::Lds l;
     const uint64_t row = row0 + blockIdx.x;
     const uint32_t segments = reply_segments(a.vocab);
-    join_row<T, OneSegment>(a, row_rules(a, row), row, segments, parts + row * segments, temperature_of(temperature, uniform, row), uniform, tokens, logprob, 0, l, dynamic_lds);
+    join_row<T, OneSegment, false>(a, row_rules(a, row), row, segments, parts + row * segments, temperature_of(temperature, uniform, row), uniform, tokens, logprob, 0, l, dynamic_lds);
 }
 
 // ---- the grammar ----------------------------------------------------------------------------------------------------------------
@@ -984,19 +1027,36 @@ hipError_t in_ranges(uint64_t blocks, F&& launch) {
     return hipSuccess;
 }
 
+// the same for a grid of `columns` blocks a row: f(first row, rows)
+template <class F>
+hipError_t in_row_ranges(uint64_t rows, uint32_t columns, F&& launch) {
+    const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(65535, MAX_BLOCKS / columns));
+    for (uint64_t r = 0; r < rows; r += most) {
+        launch(r, (unsigned)std::min(most, rows - r));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
 template <class F>
 hipError_t by_type(int32_t type, F&& f) {
     return type == TP_T_F32 ? f(TF32{}) : type == TP_T_F16 ? f(TF16{}) : f(TBF16{});
+}
+// f(type, whether the vocabulary is smaller than a vector)
+template <class F>
+hipError_t by_type_and_size(const tp_logits& io, F&& f) {
+    return by_type(io.type, [&](auto tag) { return io.vocab < 8 ? f(tag, std::true_type{}) : f(tag, std::false_type{}); });
 }
 
 }  // namespace
 
 hipError_t launch_shape(const tp_logits& io, void* out, uint64_t out_stride) {
     const uint32_t chunks = (io.vocab + SHAPE_TOKENS - 1) / SHAPE_TOKENS;
-    return by_type(io.type, [&](auto tag) {
+    return by_type_and_size(io, [&](auto tag, auto tiny) {
         using T = decltype(tag);
-        return in_ranges(io.rows * chunks, [&](uint64_t b, unsigned n) {
-            hipLaunchKernelGGL(k_shape<T>, dim3(n), dim3(SHAPE_WAVES * 64), 0, (hipStream_t)io.stream, io, b, chunks, out, out_stride);
+        return in_row_ranges(io.rows, chunks, [&](uint64_t r, unsigned n) {
+            hipLaunchKernelGGL((k_shape<T, decltype(tiny)::value>), dim3(chunks, n), dim3(SHAPE_WAVES * 64), 0, (hipStream_t)io.stream, io, r, out, out_stride);
         });
     });
 }
@@ -1016,10 +1076,10 @@ static uint32_t window_segments(const tp_logits& io) {
 hipError_t launch_choose(const tp_logits& io, const float* temperature, const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
     const uint32_t segs = window_segments(io), window = segs * CHOICE_WAVES * SEGMENT, chunks = (io.vocab + window - 1) / window;
     const uint32_t lds = io.history ? std::min(io.history_cap, window) * 4 : 0, lds_one = io.history ? std::min(io.history_cap, SEGMENT) * 4 : 0;
-    return by_type(io.type, [&](auto tag) {
+    return by_type_and_size(io, [&](auto tag, auto tiny) {
         using T = decltype(tag);
-        hipError_t e = in_ranges(io.rows * chunks, [&](uint64_t b, unsigned n) {
-            hipLaunchKernelGGL(k_choose<T>, dim3(n), dim3(CHOICE_WAVES * 64), lds, (hipStream_t)io.stream, io, b, chunks, segs, temperature, uniform, tokens, logprob, parts);
+        hipError_t e = in_row_ranges(io.rows, chunks, [&](uint64_t r, unsigned n) {
+            hipLaunchKernelGGL((k_choose<T, decltype(tiny)::value>), dim3(chunks, n), dim3(CHOICE_WAVES * 64), lds, (hipStream_t)io.stream, io, r, segs, temperature, uniform, tokens, logprob, parts);
         });
         if (e != hipSuccess || chunks == 1) return e;
         return in_ranges(io.rows, [&](uint64_t b, unsigned n) {
