@@ -1876,6 +1876,7 @@ tp_grammar* tp_grammar_create(tp_ctx* ctx, const tp_grammar_config* cfg) {
         pairs.resize(h.info.n_tokens);
         for (size_t t = 0; t < pairs.size(); ++t) { pairs[t].x = h.text_begin[t]; pairs[t].y = h.text_begin[t + 1] - h.text_begin[t]; }
         g->dev.span = upload(g->owned, pairs);
+        h.text.resize(h.text.size() + 8);                                  // k_line_text reads eight bytes at a time
         g->dev.text = upload(g->owned, h.text);
         g->dev.n_tokens = h.info.n_tokens;
         g->dev.n_places = h.info.n_prefixes + 2;

@@ -47,10 +47,10 @@ bool fits(uint64_t rows, uint64_t stride, uint64_t bytes) { return stride == 0 |
 
 uint64_t choose_workspace(uint64_t rows, uint32_t vocab) {
     // a vocabulary that any launch's window holds needs none
-    return vocab > 8 * REPLY_SEGMENT && rows <= MAX_REPLY_ROWS ? (rows * reply_segments(vocab) * sizeof(ChoicePart) + 15) / 16 * 16 : 0;
+    return vocab > 16 * REPLY_SEGMENT && rows <= MAX_REPLY_ROWS ? (rows * reply_segments(vocab) * sizeof(ChoicePart) + 15) / 16 * 16 : 0;
 }
 
-uint64_t lines_workspace(uint64_t rows) { return rows <= MAX_REPLY_ROWS ? (rows + 4) / 4 * 16 + (rows / 256 + 4) * 8 : 0; }
+uint64_t lines_workspace(uint64_t rows) { return rows <= MAX_REPLY_ROWS ? (rows + 4) / 4 * 16 + (rows / 16 + 4) * 8 : 0; }
 
 const char* check_grammar_config(const tp_grammar_config* cfg) {
     if (!cfg || cfg->struct_size != sizeof(tp_grammar_config)) return "tp_grammar_config is null or has the wrong struct_size";

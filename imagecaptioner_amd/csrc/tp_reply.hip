@@ -172,25 +172,39 @@ __device__ inline double wave_scan(double v) {
 }
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------
-// exp((x - best) / T) as 2^((x - best) * k), k = log2(e) / T.  The difference is taken first: it is small where the weight counts,
-// so that the rounding of k and of the product (each half a step, relative) moves a weight by less than |ln w| steps of 2^-23, where dividing
-// every x by T would move it by as many steps as z is large.  k stays a normal number, so that neither 0 * k nor -infinity * k is a NaN.
+// A token's weight is 2^(x * k - c), k = log2(e) / T rounded once for the row and c = best * k rounded once for the tokens that are summed
+// together: one fused multiply-add and one power.  c is no more than a common scale, known exactly to whoever joins sums of
+// different c, so that a weight is off by the rounding of k and of the fma's one result, each half a step relative in the exponent.
+// k stays a normal number, so that neither 0 * k nor -infinity * k is a NaN.  Where c overflows, neighbouring numbers already lie so far apart that only
+// the largest x weighs anything.
 __device__ inline float weight_scale(float t) {
     return t > 0.0f ? fminf(fmaxf(1.44269504088896341f / t, 1.17549435e-38f), 3.40282347e38f) : 1.44269504088896341f;
 }
-__device__ inline float weight(float x, float best, float k) {
-    if (best == -NEG_INF) return x == best ? 1.0f : 0.0f;
-    return __builtin_amdgcn_exp2f((x - best) * k);
-}
+struct Scale {
+    float k, c, best;
+    bool equal;                   // weigh by equality with the largest
+    __device__ Scale(float best_, float k_) : k(k_), c(best_ * k_), best(best_), equal(!(fabsf(best_ * k_) < __builtin_inff())) {}
+    __device__ float weight(float x) const { return equal ? (x == best ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(__builtin_fmaf(x, k, -c)); }
+    // what a sum of the weights of another scale (of the same k) counts for in this one's
+    __device__ double of(float other_best) const { return equal || !(other_best > NEG_INF) ? (other_best == best ? 1.0 : 0.0) : (double)__builtin_amdgcn_exp2f(other_best * k - c); }
+    // ln of the weight's share of `sum`: of the weight as it was summed, so that a token that is alone has 0 exactly; of its exponent where that is
+    // next to nothing
+    __device__ float log_share(float x, double sum) const {
+        const float w = weight(x);
+        return (float)(w > 1e-30f ? log((double)w / sum) : ((double)x * (double)k - (double)c) * 0.69314718055994531 - log(sum));
+    }
+};
 __device__ inline float temperature_of(const float* temperature, const float* uniform, uint64_t row) {
     const float t = temperature && uniform ? temperature[row] : 0.0f;
     return t > 0.0f ? t : 0.0f;
 }
-__device__ inline float log_probability(float x, float best, float t, double sum) {
-    return (float)((x == best ? 0.0 : ((double)x - (double)best) / (t > 0.0f ? (double)t : 1.0)) - log(sum));
-}
 // a NaN counts as -infinity in a choice
-__device__ inline float countable(float x) { return fmaxf(x, NEG_INF); }
+__device__ inline float countable(float x) { return x == x ? x : NEG_INF; }
+__device__ inline float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 
 // What a barrier of THREADS threads is: a single wave needs none, since its LDS accesses happen in order; the compiler must
 // only keep them so.  (One wave of a larger block may then work on its own.)
@@ -314,6 +328,7 @@ __device__ inline void finish_segment(const RowRules& r, uint32_t w0, uint32_t n
 // anything else is, the others again from memory in every pass.
 template <int THREADS, int HELD>
 struct History {
+    static constexpr int HELD_ENTRIES = HELD;
     uint32_t token[HELD];                                                     // as they stand there: nothing waits for them here
     __device__ inline void load(const RowRules& r, uint32_t w0) {
 #pragma unroll
@@ -322,15 +337,15 @@ struct History {
             token[i] = k < r.len ? (uint32_t)r.history[k] : w0 - 1;              // no token: a distance of 2^32 - 1
         }
     }
-    // f(whether the entry counts for frequency and presence, distance from w0), for distances below `inside`
+    // f(whether the entry counts for frequency and presence, distance from w0, number among the held or -1), for distances below `inside`
     template <class F>
     __device__ inline void each(const RowRules& r, uint32_t w0, uint32_t inside, F&& f) const {
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
-            if (token[i] - w0 < inside) f(threadIdx.x % THREADS + i * THREADS >= r.prompt, token[i] - w0);
+            if (token[i] - w0 < inside) f(threadIdx.x % THREADS + i * THREADS >= r.prompt, token[i] - w0, i);
         for (uint32_t k = threadIdx.x % THREADS + HELD * THREADS; k < r.len; k += THREADS) {
             const uint32_t h = (uint32_t)r.history[k] - w0;
-            if (h < inside) f(k >= r.prompt, h);
+            if (h < inside) f(k >= r.prompt, h, -1);
         }
     }
 };
@@ -362,7 +377,7 @@ __global__ __launch_bounds__(SHAPE_WAVES * 64) __attribute__((amdgpu_waves_per_e
     if (r.len) {
         for (uint32_t k = threadIdx.x * 4; k < SHAPE_TOKENS; k += THREADS * 4) *(uint4*)(cnt + k) = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        history.each(r, w0, std::min(n, SHAPE_TOKENS), [&](bool counted, uint32_t t) { if (counted) atomicAdd(&cnt[t], 1u); else atomicOr(&cnt[t], SEEN); });
+        history.each(r, w0, std::min(n, SHAPE_TOKENS), [&](bool counted, uint32_t t, int) { if (counted) atomicAdd(&cnt[t], 1u); else atomicOr(&cnt[t], SEEN); });
         __syncthreads();
     }
     if (g * SEGMENT >= n) return;
@@ -429,9 +444,17 @@ struct Window {
         if (!r.len) return 0;
         const uint32_t words = (inside + SEGMENT - 1) / SEGMENT * (SEGMENT / 32);      // the bitmap's, in whole segments
         for (uint32_t k = tid(); k < words; k += THREADS) l.seen[k] = l.claimed[k] = 0;
+        typename T::S held[H::HELD_ENTRIES];                                    // the held entries' own logits and biases, wanted at the end
+        float held_bias[H::HELD_ENTRIES];
+#pragma unroll
+        for (int i = 0; i < H::HELD_ENTRIES; ++i) {
+            const uint32_t t = history.token[i] - w0;
+            held[i] = t < inside ? row[t] : (typename T::S)0;
+            held_bias[i] = t < inside && r.bias ? r.bias[w0 + t] : 0.0f;
+        }
         block_sync<THREADS>();
         bool any = false;
-        history.each(r, w0, inside, [&](bool, uint32_t t) { atomicOr(&l.seen[t >> 5], 1u << (t & 31)); any = true; });
+        history.each(r, w0, inside, [&](bool, uint32_t t, int) { atomicOr(&l.seen[t >> 5], 1u << (t & 31)); any = true; });
         if (!block_any<THREADS>(any)) return 0;
         uint32_t n[MINE], mine = 0;
 #pragma unroll
@@ -451,14 +474,21 @@ struct Window {
         if (tid() == 0) l.rank[words] = distinct;
         for (uint32_t k = tid(); k < distinct; k += THREADS) value[k] = 0;
         block_sync<THREADS>();
-        history.each(r, w0, inside, [&](bool counted, uint32_t t) { if (counted) atomicAdd(&value[rank_of(l, t)], 1u); else atomicOr(&value[rank_of(l, t)], SEEN); });
+        history.each(r, w0, inside, [&](bool counted, uint32_t t, int) { if (counted) atomicAdd(&value[rank_of(l, t)], 1u); else atomicOr(&value[rank_of(l, t)], SEEN); });
         block_sync<THREADS>();
-        history.each(r, w0, inside, [&](bool, uint32_t t) {
+        history.each(r, w0, inside, [&](bool, uint32_t t, int at) {
             const uint32_t bit = 1u << (t & 31);
             if (atomicOr(&l.claimed[t >> 5], bit) & bit) return;
             const uint32_t i = rank_of(l, t);
-            const float logit = T::up(row[t]), b = r.bias ? r.bias[w0 + t] : 0.0f;
-            float x = penalised(logit, value[i], r);
+            typename T::S logit = 0;
+            float b = 0.0f;
+            if (at < 0) {
+                logit = row[t];
+                if (r.bias) b = r.bias[w0 + t];
+            }
+#pragma unroll
+            for (int h = 0; h < H::HELD_ENTRIES; ++h) if (at == h) { logit = held[h]; b = held_bias[h]; }
+            float x = penalised(T::up(logit), value[i], r);
             if (r.bias) x = x + b;
             if (r.mask && !(r.mask[(w0 + t) >> 3] >> (t & 7) & 1)) x = NEG_INF;
             value[i] = __builtin_bit_cast(uint32_t, x);
@@ -497,26 +527,43 @@ __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32
 #pragma unroll
     for (int v = 0; v < VECS; ++v) T::up8(h.d[v], x[v]);
     finish_segment<TINY>(r, w0, n, g, take, x);
+    auto sums = [&]() {
+        best = NEG_INF;
 #pragma unroll
-    for (int v = 0; v < VECS; ++v)
+        for (int v = 0; v < VECS; ++v)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[v][j] = countable(x[v][j]);
-            best = fmaxf(best, x[v][j]);
+            for (int j = 0; j < 8; j += 2) best = max3(best, x[v][j], x[v][j + 1]);
+        for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) best = fmaxf(best, countable(__builtin_bit_cast(float, value[i])));
+        best = wave_max(best);
+        const Scale scale(best, k);
+        float sum = 0.0f;
+        if (best == NEG_INF) return sum;
+        if (!scale.equal) {
+#pragma unroll
+            for (int v = 0; v < VECS; ++v) {
+                float w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v][j], k, -scale.c));
+                sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < VECS; ++v)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += scale.weight(x[v][j]);
         }
-    for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) best = fmaxf(best, countable(__builtin_bit_cast(float, value[i])));
-    best = wave_max(best);
-    if (!(best > NEG_INF)) return ChoicePart{best, 0.0f};
-    float sum = 0.0f;
+        for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) sum += scale.weight(countable(__builtin_bit_cast(float, value[i])));
+        return wave_sum(sum);
+    };
+    float sum = sums();
+    if (sum != sum || best != best) {                                         // a NaN among the logits: out with it, and again
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) {
-        float w[8];
+        for (int v = 0; v < VECS; ++v)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = weight(x[v][j], best, k);
-        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            for (int j = 0; j < 8; ++j) x[v][j] = countable(x[v][j]);
+        sum = sums();
     }
-    for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) sum += weight(countable(__builtin_bit_cast(float, value[i])), best, k);
-    return ChoicePart{best, wave_sum(sum)};
+    return ChoicePart{best, sum};
 }
 
 // Joins a row's segments: all lanes of one wave.  Tables: Chunk where the row's own window stands in LDS (`distinct` of it), OneSegment
@@ -537,7 +584,8 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         return;
     }
     const float k = weight_scale(t);
-    auto share = [&](uint32_t c) { return c < segments && p[c].best > NEG_INF ? (double)p[c].sum * (double)weight(p[c].best, best, k) : 0.0; };
+    const Scale scale(best, k);
+    auto share = [&](uint32_t c) { return c < segments ? (double)p[c].sum * scale.of(p[c].best) : 0.0; };
     double sum = 0.0;
     for (uint32_t c = lane; c < segments; c += 64) sum += share(c);
     sum = wave_sum(sum);
@@ -558,8 +606,8 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         }
         carry = __shfl(incl, 63, 64);
     }
-    const float segment_best = p[segment].best;
-    target = (target - before) / (double)weight(segment_best, best, k);
+    const Scale within(p[segment].best, k);
+    target = (target - before) / scale.of(within.best);
     const uint32_t w0 = segment * SEGMENT, n = a.vocab - w0, l0 = HERE ? w0 : 0;             // l0: the segment's start within the tables
     const auto from = logit_row<T>(a, row) + w0;
     Held<T> h;
@@ -597,7 +645,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
             double mine = 0.0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                w[j] = weight(countable(x[j]), segment_best, k);
+                w[j] = within.weight(countable(x[j]));
                 mine += (double)w[j];
             }
             const double incl = run + wave_scan(mine);
@@ -624,7 +672,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     }
     if (lane == 0) {
         tokens[row] = (int32_t)(w0 + at);
-        if (logprob) logprob[row] = log_probability(x_at, best, t, sum);
+        if (logprob) logprob[row] = scale.log_share(x_at, sum);
     }
 }
 
@@ -830,9 +878,10 @@ struct Step {
     }
     // the segments' sums of the weights against `best`, into LDS
     static __device__ void segment_sums(const float (&x)[EACH], float best, float k, Lds& s) {
+        const Scale scale(best, k);
 #pragma unroll
         for (int v = 0; v < EACH; ++v) {
-            const float w = wave_sum(best > NEG_INF ? weight(x[v], best, k) : 0.0f);
+            const float w = wave_sum(best > NEG_INF ? scale.weight(x[v]) : 0.0f);
             if ((threadIdx.x & 63) == 0) s.sum[v * WAVES + (threadIdx.x >> 6)] = w;
         }
         block_sync<THREADS>();
@@ -861,7 +910,7 @@ struct Step {
             for (int v = 0; v < EACH; ++v) pb = fmaxf(pb, x[v]);
             pb = read_lane(block_max(pb, s), 0);
             if (pb > best) {
-                sum = best > NEG_INF ? sum * (double)weight(best, pb, k) : 0.0;
+                sum = best > NEG_INF ? sum * Scale(pb, k).of(best) : 0.0;
                 best = pb;
             }
             segment_sums(x, best, k, s);
@@ -877,6 +926,7 @@ struct Step {
         }
         // Greedy: the first entry of the largest x.  Sampled: the first whose cumulative weight exceeds the target; where there is none (rounding, or
         // a `uniform` of 1 or more) the last of a weight above 0.
+        const Scale scale(best, k);
         const double target = t > 0.0f ? (double)uniform[row] * sum : 0.0;
         double carry = 0.0;
         bool found = false, mine = false;
@@ -918,7 +968,7 @@ struct Step {
                 uint2 es = make_uint2(0, 0);
 #pragma unroll
                 for (int v = 0; v < EACH; ++v) if (v == at / WAVES) { xs = x[v]; es = en[v]; }
-                const float w = weight(xs, best, k);
+                const float w = scale.weight(xs);
                 const double incl = before + wave_scan((double)w);
                 const uint64_t live = __ballot(w > 0.0f), over = __ballot(w > 0.0f && incl > target);
                 const int to = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(live);
@@ -929,7 +979,7 @@ struct Step {
         }
         if (mine) {
             tokens[row] = (int32_t)entry.x;
-            if (logprob) logprob[row] = log_probability(x_at, best, t, sum);
+            if (logprob) logprob[row] = scale.log_share(x_at, sum);
             take_entry(a, row, entry, states, append);
         }
     }
@@ -975,47 +1025,145 @@ __device__ inline Written written(const int32_t* begin, const int32_t* len, uint
     return Written{begin ? clamp_len(begin[row], width) : 0u, len ? clamp_len(len[row], width) : width};
 }
 
-// a wave per row: the bytes of its text
-__global__ __launch_bounds__(256) void k_line_sizes(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0, uint64_t rows, uint32_t* sizes) {
-    const uint64_t row = (block0 + blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const Written w = written(begin, len, width, row);
+// Sixteen rows a block, a wave each: first the bytes of every row's text and of the block's, then, each block adding the blocks before
+// it up, where a row begins, and its text.  (Rows beyond LINES_DIRECT are added up by the scan of the caption offsets instead.)
+constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64;
+constexpr uint64_t LINES_DIRECT = 65536;
+
+__global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0,
+                                                             uint64_t rows, uint32_t* sizes, unsigned long long* sums) {
+    __shared__ uint32_t of_row[LINE_ROWS];
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint64_t row = (block0 + blockIdx.x) * LINE_ROWS + wave;
     uint32_t n = 0;
-    for (uint64_t k = w.first + (threadIdx.x & 63); k < w.last; k += 64) {
-        const uint32_t t = (uint32_t)tokens[row * stride + k];
-        if (t < g.n_tokens) n += g.span[t].y;
+    if (row < rows) {
+        const Written w = written(begin, len, width, row);
+        const auto t = glob(tokens) + row * stride;
+        const auto span = (Glob<unsigned long long>)glob((const unsigned long long*)g.span);
+        for (uint32_t k = w.first + lane; k < w.last; k += 64) {
+            const uint32_t id = (uint32_t)t[k];
+            if (id < g.n_tokens) n += (uint32_t)(span[id] >> 32);
+        }
+        n = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+        if (lane == 0) sizes[row] = n;
     }
-    for (int d = 32; d; d >>= 1) n += (uint32_t)__shfl_xor((int)n, d, 64);
-    if ((threadIdx.x & 63) == 0) sizes[row] = n;
+    if (!sums) return;
+    if (lane == 0) of_row[wave] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned long long sum = 0;
+        for (uint32_t w = 0; w < LINE_ROWS; ++w) sum += of_row[w];
+        sums[block0 + blockIdx.x] = sum;
+    }
 }
 
-// a wave per row: a lane copies one token's bytes
-__global__ __launch_bounds__(256) void k_line_text(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0, uint64_t rows,
-                                                   const uint64_t* offsets, uint8_t* arena, uint64_t capacity) {
-    const uint64_t row = (block0 + blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const uint32_t lane = threadIdx.x & 63;
+// A wave's text on its way out: collected in LDS at the place it has within its 16-byte pieces of memory, and stored by whole pieces.
+constexpr uint32_t LINE_STAGE = 1024;
+typedef unsigned long long Bytes8 __attribute__((aligned(1)));
+struct Staged {
+    uint8_t* buf;                 // LINE_STAGE + 16 bytes
+    uint8_t __attribute__((address_space(1)))* piece;        // memory of buf[0], a multiple of 16
+    uint8_t __attribute__((address_space(1)))* end;          // the arena's end: nothing is stored at or behind it
+    uint32_t from, n;             // bytes [from, n) of buf are to be stored; from is 0 but in a row's first piece
+
+    __device__ void start(uint8_t __attribute__((address_space(1)))* at) {
+        from = n = (uint32_t)((uintptr_t)at & 15);
+        piece = at - from;
+    }
+    // the pieces that are full
+    __device__ void flush(uint32_t lane) {
+        const uint32_t full = n / 16;
+        if (!full) return;
+        block_sync<64>();
+        if (lane < 16 && lane >= from && piece + lane < end) piece[lane] = buf[lane];
+        for (uint32_t c = 1 + lane; c < full; c += 64) {
+            auto* to = piece + c * 16;
+            const Words4 d = *(const Words4*)(buf + c * 16);
+            if (to + 16 <= end) *(Words4 __attribute__((address_space(1)))*)to = d;
+            else for (uint32_t j = 0; j < 16; ++j) if (to + j < end) to[j] = buf[c * 16 + j];
+        }
+        const uint8_t rest = lane < (n & 15) ? buf[full * 16 + lane] : (uint8_t)0;
+        block_sync<64>();
+        if (lane < 16) buf[lane] = rest;
+        piece += full * 16;
+        n &= 15;
+        from = 0;
+    }
+    __device__ void finish(uint32_t lane) {
+        flush(lane);
+        block_sync<64>();
+        if (lane >= from && lane < n && piece + lane < end) piece[lane] = buf[lane];
+    }
+};
+
+__global__ __launch_bounds__(LINE_THREADS) void k_line_text(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0,
+                                                            uint64_t rows, const uint32_t* sizes, const unsigned long long* sums, uint64_t* offsets, uint8_t* arena, uint64_t capacity) {
+    __shared__ alignas(16) uint8_t stage[LINE_ROWS][LINE_STAGE + 16];
+    __shared__ unsigned long long before[LINE_ROWS];
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const uint64_t b = block0 + blockIdx.x, row = b * LINE_ROWS + wave;
+    uint64_t at;
+    if (sums) {
+        unsigned long long sum = 0;
+        for (uint64_t i = threadIdx.x; i < b; i += LINE_THREADS) sum += sums[i];
+        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        if (lane == 0) before[wave] = sum;
+        __syncthreads();
+        at = 0;
+        for (uint32_t w = 0; w < LINE_ROWS; ++w) at += before[w];
+        const uint32_t mine = lane < LINE_ROWS && b * LINE_ROWS + lane < rows ? sizes[b * LINE_ROWS + lane] : 0u;
+        for (uint32_t w = 0; w < wave; ++w) at += (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)w);
+        if (row >= rows) return;
+        if (lane == 0) {
+            offsets[row] = at;
+            if (row == rows - 1) offsets[rows] = at + sizes[row];
+        }
+    } else {
+        if (row >= rows) return;
+        at = offsets[row];
+    }
     const Written w = written(begin, len, width, row);
-    uint64_t at = offsets[row];
-    for (uint64_t k0 = w.first; k0 < w.last; k0 += 64) {
-        uint2 span = make_uint2(0, 0);
+    const auto t = glob(tokens) + row * stride;
+    const auto span = (Glob<unsigned long long>)glob((const unsigned long long*)g.span);
+    const auto text = glob(g.text);
+    auto* const out = (uint8_t __attribute__((address_space(1)))*)arena;
+    Staged s;
+    s.buf = stage[wave];
+    s.end = out + capacity;
+    s.start(out + at);
+    for (uint32_t k0 = w.first; k0 < w.last; k0 += 64) {
+        uint32_t n = 0;
+        uint32_t from = 0;
         if (k0 + lane < w.last) {
-            const uint32_t t = (uint32_t)tokens[row * stride + k0 + lane];
-            if (t < g.n_tokens) span = g.span[t];
+            const uint32_t id = (uint32_t)t[k0 + lane];
+            if (id < g.n_tokens) { const unsigned long long e = span[id]; from = (uint32_t)e; n = (uint32_t)(e >> 32); }
         }
-        uint32_t incl = span.y;
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = (uint32_t)__shfl_up((int)incl, d, 64);
-            if ((int)lane >= d) incl += o;
+        const uint32_t incl = wave_scan(n), all = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63), to = incl - n;
+        if (all <= LINE_STAGE - 16) {
+            s.flush(lane);
+            uint8_t* d = s.buf + s.n + to;                                   // a flush leaves at most 15 bytes
+            // the texts are followed by 8 bytes of room, so that eight bytes can be read at once
+            for (uint32_t j = 0; j < n; j += 8) {
+                const unsigned long long c = *(const Bytes8 __attribute__((address_space(1)))*)(text + from + j);
+#pragma unroll
+                for (uint32_t i = 0; i < 8; ++i) if (j + i < n) d[j + i] = (uint8_t)(c >> (8 * i));
+            }
+            s.n += all;
+        } else {                                                              // texts longer than the stage: a lane stores its token's
+            s.finish(lane);
+            auto* d = s.piece + s.n;
+            for (uint32_t j = 0; j < n; ++j) if (d + to + j < s.end) d[to + j] = text[from + j];
+            s.start(d + all);
         }
-        const uint64_t to = at + incl - span.y;
-        for (uint32_t j = 0; j < span.y; ++j) if (to + j < capacity) arena[to + j] = g.text[span.x + j];
-        at += (uint32_t)__shfl((int)incl, 63, 64);
     }
-    if (row == rows - 1 && lane < 16 && at + lane < capacity) arena[at + lane] = 0;
+    s.finish(lane);
+    if (row == rows - 1) {
+        auto* d = s.piece + s.n;
+        if (lane < 16 && d + lane < s.end) d[lane] = 0;
+    }
 }
 
-constexpr uint64_t MAX_BLOCKS = (uint64_t)1 << 22;   // of one launch: its threads stay below 2^32
+constexpr uint64_t MAX_BLOCKS = (uint64_t)1 << 21;   // of one launch: its threads stay below 2^32
 
 template <class F>
 hipError_t in_ranges(uint64_t blocks, F&& launch) {
@@ -1061,16 +1209,16 @@ hipError_t launch_shape(const tp_logits& io, void* out, uint64_t out_stride) {
     });
 }
 
-// Segments a wave of the choice takes, one after another.  More of them let fewer blocks read the row's history, and a row that
-// is one block's needs no second launch; fewer let a small call use more compute units: as many as still give every compute unit
-// its two blocks.  A window must also keep its repeated tokens in 64 KB of LDS.
+// Segments a wave of the choice takes, one after another.  Where a window holds the row (131072 tokens) its history is read once and
+// no second launch joins it: taken for rows of up to 64 segments, and where there are rows for every compute unit.  A unit works on a segment for
+// about 0.15 us, though, and fewer long rows than units leave the others idle (one row of 131072: 22 us in one block, 7 + 7 in eight and the join): they are split.
+// A window must also keep its repeated tokens in 64 KB of LDS.
 static uint32_t window_segments(const tp_logits& io) {
-    for (uint32_t segs = MOST_SEGS; segs > 1; segs /= 2) {
-        const uint64_t tokens = (uint64_t)CHOICE_WAVES * segs * SEGMENT;
-        if (tokens > 16384 && io.history && io.history_cap > 4096) continue;
-        if (tokens / 2 < io.vocab && io.rows * ((io.vocab + tokens - 1) / tokens) >= 512) return segs;
-    }
-    return 1;
+    uint32_t segs = 1;
+    const bool whole = reply_segments(io.vocab) <= 64 || io.rows >= 256;
+    while (segs < MOST_SEGS && segs * CHOICE_WAVES * SEGMENT < io.vocab && (whole || io.rows * ((io.vocab + 2 * segs * CHOICE_WAVES * SEGMENT - 1) / (2 * segs * CHOICE_WAVES * SEGMENT)) >= 256)) segs *= 2;
+    while (segs > 1 && io.history && std::min(io.history_cap, segs * CHOICE_WAVES * SEGMENT) > 16384) segs /= 2;
+    return segs;
 }
 
 hipError_t launch_choose(const tp_logits& io, const float* temperature, const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
@@ -1112,15 +1260,17 @@ hipError_t launch_grammar_step(const DevGrammar& g, const tp_logits& io, const f
 hipError_t launch_grammar_lines(const DevGrammar& g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t rows,
                                 uint8_t* arena, uint64_t capacity, uint64_t* offsets, void* workspace, hipStream_t s) {
     uint32_t* sizes = (uint32_t*)workspace;
-    uint64_t* tiles = (uint64_t*)((uint8_t*)workspace + (rows + 4) / 4 * 16);
-    hipError_t e = in_ranges((rows + 3) / 4, [&](uint64_t b, unsigned n) {
-        hipLaunchKernelGGL(k_line_sizes, dim3(n), dim3(256), 0, s, g, tokens, stride, width, begin, len, b, rows, sizes);
+    unsigned long long* sums = (unsigned long long*)((uint8_t*)workspace + (rows + 4) / 4 * 16);
+    const uint64_t blocks = (rows + LINE_ROWS - 1) / LINE_ROWS;
+    const bool direct = rows <= LINES_DIRECT;
+    hipError_t e = in_ranges(blocks, [&](uint64_t b, unsigned n) {
+        hipLaunchKernelGGL(k_line_sizes, dim3(n), dim3(LINE_THREADS), 0, s, g, tokens, stride, width, begin, len, b, rows, sizes, direct ? sums : nullptr);
     });
     if (e != hipSuccess) return e;
-    e = launch_scan_u32(sizes, rows, offsets, tiles, nullptr, nullptr, s);
+    if (!direct) e = launch_scan_u32(sizes, rows, offsets, (uint64_t*)sums, nullptr, nullptr, s);
     if (e != hipSuccess) return e;
-    return in_ranges((rows + 3) / 4, [&](uint64_t b, unsigned n) {
-        hipLaunchKernelGGL(k_line_text, dim3(n), dim3(256), 0, s, g, tokens, stride, width, begin, len, b, rows, offsets, arena, capacity);
+    return in_ranges(blocks, [&](uint64_t b, unsigned n) {
+        hipLaunchKernelGGL(k_line_text, dim3(n), dim3(LINE_THREADS), 0, s, g, tokens, stride, width, begin, len, b, rows, sizes, direct ? sums : nullptr, offsets, arena, capacity);
     });
 }
 

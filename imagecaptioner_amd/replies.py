@@ -14,140 +14,143 @@ torch tensors of that device, on torch's current stream, without waiting for it,
 Nothing here has a gradient: the calls shape what a model answers while it answers.
 """
 import ctypes as C
+import struct
 
 import numpy as np
 
-from ._abi import TP_E_CAPACITY, VERDICT_DTYPE, tp_counters, tp_device_io, tp_grammar_config, tp_grammar_info, tp_logits
+from ._abi import TP_E_CAPACITY, VERDICT_DTYPE, tp_counters, tp_device_io, tp_grammar_config, tp_grammar_info
 from .tagpipe import BatchResult, TagPipeError, load_library
 
+# A decoding loop makes these calls once per token, and the host's part of a small call takes longer than the GPU's: arguments are
+# checked with as few tensor queries as will do, and tp_logits is packed in one go (the layout of _abi.tp_logits).
+_LOGITS = struct.Struct("@IiQIIPQPQPPPPPPQPPQPIIP")
+_torch_module = None
 _TYPES = None
 
 
 def _torch():
-    global _TYPES
-    import torch
-    if _TYPES is None:
+    global _torch_module, _TYPES
+    if _torch_module is None:
+        import torch
         _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    return torch
+        _torch_module = torch
+    return _torch_module
 
 
 def _stream(torch, device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def _tensor(name, t, device, dtype, shape):
-    """t's data pointer after the checks every argument gets; -1 in `shape` takes any size.  The last axis must be dense."""
-    if t.dtype is not dtype or t.get_device() != device:
-        raise ValueError("%s must be a %s tensor on cuda:%d, got %s on %s" % (name, dtype, device, t.dtype, t.device))
-    if t.dim() != len(shape) or any(want not in (-1, got) for want, got in zip(shape, t.shape)):
-        raise ValueError("%s must have the shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
-    if shape and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError("%s must be dense along its last axis" % name)
-    return t.data_ptr() or None
+def _refuse(name, t, device, dtype, shape):
+    raise ValueError("%s must be a %s tensor of the shape %s on cuda:%d, dense along its last axis, got %s %s with strides %s on %s" % (
+        name, dtype, shape, device, t.dtype, tuple(t.shape), t.stride(), t.device))
 
 
-def _row_stride(t):
-    """Elements between rows; where there is one row at most, its length."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _vec(name, t, device, dtype, rows):
+    """A dense vector's data pointer."""
+    if t.dtype is not dtype or t.get_device() != device or t.shape != (rows,) or not t.is_contiguous():
+        _refuse(name, t, device, dtype, "(%d,)" % rows)
+    return t.data_ptr()
 
 
-def logit_rules(device, rows, vocab, *, history=None, history_len=None, prompt_len=None, repetition=None, frequency=None, presence=None,
+def _table(name, t, device, dtype, rows, columns):
+    """A table's data pointer, rows, columns and elements between rows (its columns where there is one row at most); rows or columns -1: any."""
+    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2:
+        _refuse(name, t, device, dtype, "(%d, %d)" % (rows, columns))
+    r, c = t.shape
+    stride, dense = t.stride()
+    if (rows != -1 and r != rows) or (columns != -1 and c != columns) or (c > 1 and dense != 1):
+        _refuse(name, t, device, dtype, "(%d, %d)" % (rows, columns))
+    return t.data_ptr(), r, c, stride if r > 1 else c
+
+
+def logit_rules(device, type_, rows, vocab, logits, stride, *, history=None, history_len=None, prompt_len=None, repetition=None, frequency=None, presence=None,
                 bias=None, bias_row=None, mask=None, mask_row=None):
-    """A tp_logits without its logits.
+    """A packed tp_logits.
 
     history int32 [rows, n] with history_len int32 [rows] (every row is full without it); entries before prompt_len int32 [rows] count as
     repeated but not for frequency and presence.  repetition, frequency, presence: float32 [rows].
     bias float32 [n, vocab] (or [vocab]) with bias_row int32 [rows]: which one a row takes, -1 none; row 0 for all without it.
     mask int32 [n, (vocab + 31) // 32] (or one row) with mask_row likewise: token t is allowed when bit t % 32 of word t // 32 is set."""
     torch = _torch()
-    io = tp_logits()
-    io.struct_size = C.sizeof(tp_logits)
-    io.rows, io.vocab = rows, vocab
     i32, f32 = torch.int32, torch.float32
+    h = h_cap = h_stride = h_len = prompt = b = b_stride = b_row = n_bias = m = m_stride = m_row = n_masks = 0
     if history is not None:
-        io.history = _tensor("history", history, device, i32, (rows, -1))
-        io.history_stride, io.history_cap = _row_stride(history), history.shape[1]
+        h, _, h_cap, h_stride = _table("history", history, device, i32, rows, -1)
         if history_len is not None:
-            io.history_len = _tensor("history_len", history_len, device, i32, (rows,))
+            h_len = _vec("history_len", history_len, device, i32, rows)
         if prompt_len is not None:
-            io.prompt_len = _tensor("prompt_len", prompt_len, device, i32, (rows,))
-        if io.history is None:                                # no rows, or rows of no room: there is no history, whatever the lengths say
-            io.history_len = io.prompt_len = None
+            prompt = _vec("prompt_len", prompt_len, device, i32, rows)
+        if not h:                                            # no rows, or rows of no room: there is no history, whatever the lengths say
+            h_len = prompt = 0
     elif history_len is not None or prompt_len is not None:
         raise ValueError("history_len or prompt_len without a history")
-    if repetition is not None:
-        io.repetition = _tensor("repetition", repetition, device, f32, (rows,))
-    if frequency is not None:
-        io.frequency = _tensor("frequency", frequency, device, f32, (rows,))
-    if presence is not None:
-        io.presence = _tensor("presence", presence, device, f32, (rows,))
     if bias is not None:
-        bias = bias if bias.dim() == 2 else bias[None]
-        io.bias = _tensor("bias", bias, device, f32, (-1, vocab))
-        io.bias_stride, io.n_bias = _row_stride(bias), bias.shape[0]
+        b, n_bias, _, b_stride = _table("bias", bias if bias.dim() == 2 else bias[None], device, f32, -1, vocab)
         if bias_row is not None:
-            io.bias_row = _tensor("bias_row", bias_row, device, i32, (rows,))
-        if bias.shape[0] == 0:
+            b_row = _vec("bias_row", bias_row, device, i32, rows)
+        if not n_bias:
             raise ValueError("bias has no rows")
     elif bias_row is not None:
         raise ValueError("bias_row without a bias")
     if mask is not None:
-        mask = mask if mask.dim() == 2 else mask[None]
-        io.mask = _tensor("mask", mask, device, i32, (-1, (vocab + 31) // 32))
-        io.mask_stride, io.n_masks = _row_stride(mask), mask.shape[0]
+        m, n_masks, _, m_stride = _table("mask", mask if mask.dim() == 2 else mask[None], device, i32, -1, (vocab + 31) // 32)
         if mask_row is not None:
-            io.mask_row = _tensor("mask_row", mask_row, device, i32, (rows,))
-        if mask.shape[0] == 0:
+            m_row = _vec("mask_row", mask_row, device, i32, rows)
+        if not n_masks:
             raise ValueError("mask has no rows")
     elif mask_row is not None:
         raise ValueError("mask_row without a mask")
-    io.stream = _stream(torch, device)
-    return io
+    return _LOGITS.pack(_LOGITS.size, type_, rows, vocab, h_cap, logits, stride, h, h_stride, h_len, prompt,
+                        0 if repetition is None else _vec("repetition", repetition, device, f32, rows),
+                        0 if frequency is None else _vec("frequency", frequency, device, f32, rows),
+                        0 if presence is None else _vec("presence", presence, device, f32, rows),
+                        b, b_stride, b_row, m, m_stride, m_row, n_bias, n_masks, _stream(torch, device))
 
 
 def _with_logits(device, logits, rules):
+    """(packed tp_logits, rows, vocab)"""
     torch = _torch()
-    if logits.dim() != 2 or logits.dtype not in _TYPES:
-        raise ValueError("logits must be a float32, float16 or bfloat16 tensor [rows, vocab], got %s %s" % (logits.dtype, tuple(logits.shape)))
+    dtype = logits.dtype
+    if dtype not in _TYPES:
+        raise ValueError("logits must be a float32, float16 or bfloat16 tensor [rows, vocab], got %s" % dtype)
     if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("logits require a gradient, which this call does not have: detach them")
-    io = logit_rules(device, logits.shape[0], logits.shape[1], **rules)
-    io.logits = _tensor("logits", logits, device, logits.dtype, (-1, -1))
-    io.type, io.stride = _TYPES[logits.dtype], _row_stride(logits)
-    return io
+    p, rows, vocab, stride = _table("logits", logits, device, dtype, -1, -1)
+    return logit_rules(device, _TYPES[dtype], rows, vocab, p, stride, **rules), rows, vocab
 
 
 def _choice_inputs(device, rows, temperature, uniform):
     torch = _torch()
-    t = None if temperature is None else _tensor("temperature", temperature, device, torch.float32, (rows,))
-    u = None if uniform is None else _tensor("uniform", uniform, device, torch.float32, (rows,))
-    if t is not None and u is None and rows:
+    t = None if temperature is None else _vec("temperature", temperature, device, torch.float32, rows)
+    u = None if uniform is None else _vec("uniform", uniform, device, torch.float32, rows)
+    if t and not u:
         raise ValueError("a temperature needs `uniform`, the random numbers of the choice")
     return t, u
 
 
 def shape_logits(pipe, logits, out, rules):
-    torch = _torch()
-    device = pipe._cfg.struct.device
-    io = _with_logits(device, logits, rules)
+    device = pipe._device
+    io, rows, vocab = _with_logits(device, logits, rules)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    to = _tensor("out", out, device, logits.dtype, tuple(logits.shape))
-    pipe._check(pipe._L.tp_shape_logits(pipe._h, C.byref(io), to, _row_stride(out)))
+        out = logits.new_empty((rows, vocab))
+        to, stride = out.data_ptr(), vocab
+    else:
+        to, _, _, stride = _table("out", out, device, logits.dtype, rows, vocab)
+    pipe._check(pipe._L.tp_shape_logits(pipe._h, io, to, stride))
     return out
 
 
 def choose_tokens(pipe, logits, temperature, uniform, rules):
     torch = _torch()
-    device = pipe._cfg.struct.device
-    io = _with_logits(device, logits, rules)
-    rows = logits.shape[0]
+    device = pipe._device
+    io, rows, vocab = _with_logits(device, logits, rules)
     t, u = _choice_inputs(device, rows, temperature, uniform)
-    need = pipe._L.tp_choose_workspace(rows, logits.shape[1])
-    workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)       # torch's own pool keeps it apart per stream and per graph
-    tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    pipe._check(pipe._L.tp_choose_tokens(pipe._h, C.byref(io), t, u, tokens.data_ptr(), logprob.data_ptr(), workspace.data_ptr(), need))
+    need = pipe._L.tp_choose_workspace(rows, vocab)
+    workspace = logits.new_empty((need,), dtype=torch.uint8) if need else None   # torch's own pool keeps it apart per stream and per graph
+    tokens = logits.new_empty((rows,), dtype=torch.int32)
+    logprob = logits.new_empty((rows,), dtype=torch.float32)
+    pipe._check(pipe._L.tp_choose_tokens(pipe._h, io, t, u, tokens.data_ptr(), logprob.data_ptr(), workspace.data_ptr() if need else None, need))
     return tokens, logprob
 
 
@@ -181,8 +184,9 @@ class TagGrammar:
             raise TagPipeError(-2, self._L.tp_last_error().decode("utf-8", "replace"))
         self.info = tp_grammar_info()
         self._check(self._L.tp_grammar_get_info(self._h, C.byref(self.info)))
-        self.device = pipe._cfg.struct.device
+        self.device = pipe._device
         self.end_place = self.info.n_prefixes + 1
+        self._words = (self.info.n_tokens + 31) // 32
 
     def _check(self, rc):
         if rc != 0:
@@ -205,65 +209,64 @@ class TagGrammar:
         return torch.zeros(rows, 2, dtype=torch.int32, device="cuda:%d" % self.device)
 
     def _states(self, states):
-        torch = _torch()
-        p = _tensor("states", states, self.device, torch.int32, (-1, 2))
-        if states.shape[0] > 1 and states.stride(0) != 2:
+        p, rows, _, stride = _table("states", states, self.device, _torch().int32, -1, 2)
+        if stride != 2:
             raise ValueError("states must be dense")
-        return p
+        return p, rows
 
     def mask(self, states, out=None):
         """tp_grammar_mask: the allowed-token masks of rows of states, int32 [rows, (n_tokens + 31) // 32]."""
-        torch = _torch()
-        p, rows, words = self._states(states), states.shape[0], (self.info.n_tokens + 31) // 32
+        p, rows = self._states(states)
+        words = self._words
         if out is None:
-            out = torch.empty(rows, words, dtype=torch.int32, device=states.device)
-        to = _tensor("out", out, self.device, torch.int32, (rows, words))
-        self._check(self._L.tp_grammar_mask(self._h, p, rows, to, _row_stride(out), _stream(torch, self.device)))
+            out = states.new_empty((rows, words))
+            to, stride = out.data_ptr(), words
+        else:
+            to, _, _, stride = _table("out", out, self.device, states.dtype, rows, words)
+        self._check(self._L.tp_grammar_mask(self._h, p, rows, to, stride, _stream(_torch(), self.device)))
         return out
 
     def step(self, states, logits, *, temperature=None, uniform=None, append=False, **rules):
         """tp_grammar_step: (tokens int32 [rows], log-probabilities float32 [rows]); `states` move on in place, and with append=True the
         tokens go to the end of `history` and `history_len` rises.  -1: the row's line is at its end, or nothing is left to choose."""
-        torch = _torch()
-        p, rows = self._states(states), states.shape[0]
-        io = _with_logits(self.device, logits, rules)
-        if logits.shape[0] != rows:
+        p, rows = self._states(states)
+        io, of_logits, _ = _with_logits(self.device, logits, rules)
+        if of_logits != rows:
             raise ValueError("one state per row of logits")
         t, u = _choice_inputs(self.device, rows, temperature, uniform)
-        tokens = torch.empty(rows, dtype=torch.int32, device=states.device)
-        logprob = torch.empty(rows, dtype=torch.float32, device=states.device)
-        self._check(self._L.tp_grammar_step(self._h, C.byref(io), t, u, p, tokens.data_ptr(), logprob.data_ptr(), int(append)))
+        tokens = states.new_empty((rows,))
+        logprob = states.new_empty((rows,), dtype=_torch().float32)
+        self._check(self._L.tp_grammar_step(self._h, io, t, u, p, tokens.data_ptr(), logprob.data_ptr(), bool(append)))
         return tokens, logprob
 
     def advance(self, states, tokens, *, history=None, history_len=None, append=False):
         """tp_grammar_step by the caller's own tokens (int32 [rows]): `states` move on in place; to place -1 where a token is not allowed."""
-        torch = _torch()
-        p, rows = self._states(states), states.shape[0]
-        io = logit_rules(self.device, rows, self.info.n_tokens, history=history, history_len=history_len)
-        given = _tensor("tokens", tokens, self.device, torch.int32, (rows,))
-        self._check(self._L.tp_grammar_step(self._h, C.byref(io), None, None, p, given, None, int(append)))
+        p, rows = self._states(states)
+        io = logit_rules(self.device, 0, rows, self.info.n_tokens, 0, 0, history=history, history_len=history_len)
+        self._check(self._L.tp_grammar_step(self._h, io, None, None, p, _vec("tokens", tokens, self.device, states.dtype, rows), None, bool(append)))
 
     def lines(self, tokens, lengths=None, begin=None, arena=None):
         """tp_grammar_lines: (arena uint8, offsets int64 [rows + 1]) of rows of tokens int32 [rows, n], from begin to below lengths (int32
         [rows]).  A given arena bounds what is written: compare offsets[rows] with its size."""
         torch = _torch()
-        p, (rows, n) = _tensor("tokens", tokens, self.device, torch.int32, (-1, -1)), tokens.shape
-        le = None if lengths is None else _tensor("lengths", lengths, self.device, torch.int32, (rows,))
-        be = None if begin is None else _tensor("begin", begin, self.device, torch.int32, (rows,))
+        i32 = torch.int32
+        p, rows, n, stride = _table("tokens", tokens, self.device, i32, -1, -1)
+        le = None if lengths is None else _vec("lengths", lengths, self.device, i32, rows)
+        be = None if begin is None else _vec("begin", begin, self.device, i32, rows)
         if arena is None:
-            arena = torch.empty(rows * n * self.info.longest_token + 16, dtype=torch.uint8, device=tokens.device)
-        to = _tensor("arena", arena, self.device, torch.uint8, (-1,))
-        offsets = torch.zeros(1, dtype=torch.int64, device=tokens.device) if rows == 0 else torch.empty(rows + 1, dtype=torch.int64, device=tokens.device)
+            arena = tokens.new_empty((rows * n * self.info.longest_token + 16,), dtype=torch.uint8)
+        to = _vec("arena", arena, self.device, torch.uint8, arena.numel())
+        offsets = tokens.new_empty((rows + 1,), dtype=torch.int64) if rows else tokens.new_zeros((1,), dtype=torch.int64)
         need = self._L.tp_lines_workspace(rows)
-        workspace = torch.empty(need, dtype=torch.uint8, device=tokens.device)
-        self._check(self._L.tp_grammar_lines(self._h, p, _row_stride(tokens), n, be, le, rows, to, arena.shape[0], offsets.data_ptr(), workspace.data_ptr(), need,
+        workspace = tokens.new_empty((need,), dtype=torch.uint8)
+        self._check(self._L.tp_grammar_lines(self._h, p, stride, n, be, le, rows, to, arena.numel(), offsets.data_ptr(), workspace.data_ptr(), need,
                                              _stream(torch, self.device)))
         return arena, offsets
 
 
 def run_tokens(pipe, grammar, tokens, lengths, begin):
     torch = _torch()
-    if grammar.device != pipe._cfg.struct.device:
+    if grammar.device != pipe._device:
         raise ValueError("the grammar is on another device than the context")
     arena, offsets = grammar.lines(tokens, lengths, begin)
     rows, info, device = tokens.shape[0], pipe.info, tokens.device

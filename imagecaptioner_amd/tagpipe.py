@@ -10,7 +10,7 @@ import os
 import numpy as np
 
 from ._abi import (tp_replies, TP_E_CAPACITY, TP_OK, VERDICT_DTYPE, Config, tp_audit, tp_config, tp_counters, tp_device_io, tp_grammar_config,
-                   tp_grammar_info, tp_logits, tp_result, tp_table_info, tp_timing)
+                   tp_grammar_info, tp_result, tp_table_info, tp_timing)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtagpipe_hip.so")
@@ -90,17 +90,17 @@ def load_library():
                                         C.c_void_p, C.c_uint64, C.c_void_p, C.POINTER(C.c_uint64)]
     L.tp_fallback_caption.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.POINTER(C.c_uint64)]
     L.tp_error_needtag_text.restype = C.c_char_p
-    L.tp_shape_logits.argtypes = [C.c_void_p, C.POINTER(tp_logits), C.c_void_p, C.c_uint64]
+    L.tp_shape_logits.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64]                # tp_logits as a struct or as packed bytes
     L.tp_choose_workspace.argtypes = [C.c_uint64, C.c_uint32]
     L.tp_choose_workspace.restype = C.c_uint64
-    L.tp_choose_tokens.argtypes = [C.c_void_p, C.POINTER(tp_logits), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64]
+    L.tp_choose_tokens.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64]
     L.tp_grammar_create.argtypes = [C.c_void_p, C.POINTER(tp_grammar_config)]
     L.tp_grammar_create.restype = C.c_void_p
     L.tp_grammar_destroy.argtypes = [C.c_void_p]
     L.tp_grammar_destroy.restype = None
     L.tp_grammar_get_info.argtypes = [C.c_void_p, C.POINTER(tp_grammar_info)]
     L.tp_grammar_mask.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]
-    L.tp_grammar_step.argtypes = [C.c_void_p, C.POINTER(tp_logits), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]
+    L.tp_grammar_step.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]
     L.tp_lines_workspace.argtypes = [C.c_uint64]
     L.tp_lines_workspace.restype = C.c_uint64
     L.tp_grammar_lines.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p,
@@ -141,6 +141,7 @@ class TagPipe:
     def __init__(self, config: Config):
         self._L = load_library()
         self._cfg = config
+        self._device = config.struct.device
         self._h = self._L.tp_create(C.byref(config.struct))
         if not self._h:
             raise TagPipeError(-2, self._L.tp_last_error().decode("utf-8", "replace"))

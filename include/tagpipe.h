@@ -555,7 +555,7 @@ int tp_shape_logits(tp_ctx* ctx, const tp_logits* io, void* out, uint64_t out_st
  * The token of every row.  z = x / temperature[r] where temperature[r] > 0, else z = x.  Without a temperature (NULL
  * array, 0, negative, NaN) the token is the largest x, ties to the lowest token.  With one it is the lowest token whose
  * cumulative weight exceeds uniform[r] * (the sum of all weights), weights exp(z - max z) in token order, summed in 64
- * bits; uniform[r] in [0, 1), NULL: as temperature NULL.  Values of uniform outside [0, 1) give the first or last token of a weight above 0.
+ * bits (a thousand neighbours at a time in 32); uniform[r] in [0, 1), NULL: as temperature NULL.  Values of uniform outside [0, 1) give the first or last token of a weight above 0.
  * A z of NaN counts as -infinity.  Where +infinity stands, the tokens that have it share the weight.
  * logprob[r] = z - max z - ln(sum of weights) of the chosen token.  A row without a z above -infinity gets token -1 and
  * log-probability -infinity.  logprob may be NULL.  workspace: tp_choose_workspace bytes (host function), aligned to 16.

@@ -252,6 +252,14 @@ def test_null_handles_are_refused_by_the_library():
     L.tp_grammar_destroy(None)
 
 
+def test_packed_logits_have_the_structs_layout():
+    from imagecaptioner_amd.replies import _LOGITS
+    n = len(tp_logits._fields_)
+    assert _LOGITS.size == C.sizeof(tp_logits)
+    io = tp_logits.from_buffer_copy(_LOGITS.pack(*range(1, n + 1)))
+    assert [getattr(io, f) for f, _ in tp_logits._fields_] == list(range(1, n + 1))
+
+
 def test_struct_layouts_match_the_header(tmp_path):
     from imagecaptioner_amd import _abi
     names = ("tp_logits", "tp_grammar_config", "tp_grammar_info")

@@ -478,7 +478,7 @@ def lines_of(plain, rows, first, last):
     return [plain.text(row[a:b]) for row, a, b in zip(rows, first, last)]
 
 
-@pytest.mark.parametrize("rows,width", [(1, 1), (1, 300), (5, 64), (4, 65), (70, 131), (4100, 9)])
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 300), (5, 64), (4, 65), (70, 131), (4100, 9), (70001, 2)])
 def test_lines(pipe, rows, width):
     g, plain, tokens = small_grammar(pipe)
     rng = np.random.default_rng(rows * width)
@@ -503,6 +503,29 @@ def test_lines(pipe, rows, width):
     wide[:, 1:1 + width] = dev(t)
     arena, offsets = g.lines(wide[:, 1:1 + width])
     assert bytes(arena[:int(offsets[-1])].cpu().numpy()) == b"".join(lines_of(plain, t, [0] * rows, [width] * rows))
+
+
+def test_lines_of_long_tokens(pipe):
+    """Texts around and beyond the 1008 bytes that 64 tokens are collected in, at every offset within 16 bytes."""
+    rng = random.Random(3)
+    texts = [bytes(rng.choice(b"abcdef") for _ in range(n)) for n in (1, 7, 8, 9, 15, 16, 17, 31, 63, 250, 1000, 1007, 1008, 1009, 1024, 5000)]
+    tokens = [bytes([b]) for b in range(256)] + texts + [b""]
+    g = pipe.tag_grammar(tokens, len(tokens) - 1)
+    plain = PlainGrammar(["ab"], tokens, len(tokens) - 1)
+    rows = []
+    for r in range(64):
+        row = [ord("x")] * (r % 17) + [256 + rng.randrange(len(texts)) for _ in range(r % 5)] + [256] * (70 if r % 3 else 0) + [256 + (r % len(texts))]
+        rows.append(row + [-1] * (100 - len(row)))
+    t = np.array(rows, np.int32)
+    arena, offsets = g.lines(dev(t))
+    want = [plain.text(row) for row in rows]
+    assert offsets.tolist() == np.cumsum([0] + [len(x) for x in want]).tolist()
+    assert bytes(arena[:int(offsets[-1])].cpu().numpy()) == b"".join(want)
+    for first in range(1, 16):                                             # an arena of any alignment
+        room = torch.full((int(offsets[-1]) + 64,), 0x55, device="cuda", dtype=torch.uint8)
+        g.lines(dev(t), arena=room[first:first + int(offsets[-1])])
+        got = bytes(room.cpu().numpy())
+        assert got[first:first + int(offsets[-1])] == b"".join(want) and set(got[:first] + got[first + int(offsets[-1]):]) == {0x55}
 
 
 def test_nothing_to_do(pipe):
