@@ -1873,9 +1873,22 @@ tp_grammar* tp_grammar_create(tp_ctx* ctx, const tp_grammar_config* cfg) {
         std::vector<uint2> pairs(h.token.size());
         for (size_t e = 0; e < pairs.size(); ++e) { pairs[e].x = (uint32_t)h.token[e]; pairs[e].y = h.move[e]; }
         g->dev.entry = upload(g->owned, pairs);
-        pairs.resize(h.info.n_tokens);
-        for (size_t t = 0; t < pairs.size(); ++t) { pairs[t].x = h.text_begin[t]; pairs[t].y = h.text_begin[t + 1] - h.text_begin[t]; }
-        g->dev.span = upload(g->owned, pairs);
+        std::vector<uint8_t> bytes(h.info.n_tokens);
+        std::vector<uint4> records(h.info.n_tokens);
+        for (size_t t = 0; t < records.size(); ++t) {
+            const uint32_t begin = h.text_begin[t], n = h.text_begin[t + 1] - begin;
+            uint8_t rec[16] = {};
+            if (n < 16) {
+                std::memcpy(rec, h.text.data() + begin, n);
+            } else {
+                std::memcpy(rec, &begin, 4);
+                std::memcpy(rec + 4, &n, 4);
+            }
+            bytes[t] = rec[15] = (uint8_t)(n < 16 ? n : LONG_TOKEN);
+            std::memcpy(&records[t], rec, 16);
+        }
+        g->dev.bytes = upload(g->owned, bytes);
+        g->dev.record = upload(g->owned, records);
         h.text.resize(h.text.size() + 8);                                  // k_line_text reads eight bytes at a time
         g->dev.text = upload(g->owned, h.text);
         g->dev.n_tokens = h.info.n_tokens;

@@ -9,12 +9,16 @@
 
 namespace tp {
 
+constexpr uint32_t LONG_TOKEN = 255;
+
 // A compiled grammar in device memory.
 struct DevGrammar {
     const uint32_t* begin;        // HostGrammar::begin
     const uint2* entry;           // per entry: token, move
-    const uint8_t* text;          // the tokens' bytes
-    const uint2* span;            // per token: first byte, bytes
+    const uint8_t* bytes;         // per token: its bytes, or LONG_TOKEN
+    const uint4* record;          // per token: up to 15 bytes of text and their number in the last byte; of a longer one where it starts in
+                                  //   `text`, its bytes, and LONG_TOKEN in the last byte
+    const uint8_t* text;          // the tokens' bytes, and eight behind them
     uint32_t n_tokens, n_places;  // places 0 .. n_places - 1 (the end among them)
     uint32_t min_tags, max_tags;
 };

@@ -730,10 +730,10 @@ __device__ inline bool may(uint32_t move, uint32_t tags, const DevGrammar& g) {
 
 struct List { uint32_t lo, hi, tags; };
 __device__ inline List list_of(const DevGrammar& g, const int32_t* states, uint64_t row) {
-    const uint32_t place = (uint32_t)states[2 * row];
-    const int32_t tags = states[2 * row + 1];
+    const uint32_t place = (uint32_t)glob(states)[2 * row];
+    const int32_t tags = glob(states)[2 * row + 1];
     List q{0, 0, tags < 0 ? 0u : tags > 65535 ? 65535u : (uint32_t)tags};
-    if (place < g.n_places) { q.lo = g.begin[place]; q.hi = g.begin[place + 1]; }
+    if (place < g.n_places) { q.lo = glob(g.begin)[place]; q.hi = glob(g.begin)[place + 1]; }
     return q;
 }
 
@@ -760,21 +760,27 @@ __device__ inline uint32_t lower_entry_wave(const uint2* entry, uint32_t lo, uin
 
 // A block writes MASK_PIECE words of one row: cleared in LDS, the list's entries that fall into the piece set there, stored
 // in 16-byte pieces.  Of a list longer than a few rounds of the block only the piece's own part is read.
-constexpr uint32_t MASK_PIECE = 1024;
-__global__ __launch_bounds__(256) void k_grammar_mask(DevGrammar g, const int32_t* states, uint64_t block0, uint32_t pieces, uint32_t* mask, uint64_t mask_stride) {
+constexpr uint32_t MASK_PIECE = 1024, MASK_AHEAD = 4;
+__global__ __launch_bounds__(256) void k_grammar_mask(DevGrammar g, const int32_t* states, uint64_t row0, uint32_t* mask, uint64_t mask_stride) {
     __shared__ alignas(16) uint32_t bits[MASK_PIECE];
-    const uint64_t b = block0 + blockIdx.x, row = b / pieces;
-    const uint32_t w0 = (uint32_t)(b % pieces) * MASK_PIECE, words = (g.n_tokens + 31) / 32;
+    const uint64_t row = row0 + blockIdx.y;
+    const uint32_t w0 = blockIdx.x * MASK_PIECE, words = (g.n_tokens + 31) / 32;
     List q = list_of(g, states, row);
     *(uint4*)(bits + threadIdx.x * 4) = make_uint4(0, 0, 0, 0);
     const uint32_t t0 = w0 * 32;
-    if (t0 && q.hi - q.lo > 1024) q.lo = lower_entry_wave(g.entry, q.lo, q.hi, t0);
+    if (t0 && q.hi - q.lo > 256 * MASK_AHEAD) q.lo = lower_entry_wave(g.entry, q.lo, q.hi, t0);
     __syncthreads();
-    for (uint32_t e = q.lo + threadIdx.x; e < q.hi; e += 256) {
-        const uint2 en = g.entry[e];
-        const uint32_t t = en.x - t0;
-        if (en.x >= t0 + MASK_PIECE * 32) break;
-        if (en.x >= t0 && may(en.y, q.tags, g)) atomicOr(&bits[t >> 5], 1u << (t & 31));
+    const auto entries = (Glob<unsigned long long>)glob((const unsigned long long*)g.entry);
+    for (uint32_t e0 = q.lo + threadIdx.x; e0 < q.hi; e0 += 256 * MASK_AHEAD) {
+        unsigned long long en[MASK_AHEAD];
+#pragma unroll
+        for (uint32_t i = 0; i < MASK_AHEAD; ++i) en[i] = e0 + i * 256 < q.hi ? entries[e0 + i * 256] : 0xFFFFFFFFull;
+#pragma unroll
+        for (uint32_t i = 0; i < MASK_AHEAD; ++i) {
+            const uint32_t t = (uint32_t)en[i] - t0;                          // beyond the piece where the entry is one of another piece, or none
+            if (t < MASK_PIECE * 32 && may((uint32_t)(en[i] >> 32), q.tags, g)) atomicOr(&bits[t >> 5], 1u << (t & 31));
+        }
+        if ((uint32_t)en[MASK_AHEAD - 1] >= t0 + MASK_PIECE * 32) break;       // ascending: so is whatever follows
     }
     __syncthreads();
     uint32_t* out = mask + row * mask_stride + w0;
@@ -1027,7 +1033,8 @@ __device__ inline Written written(const int32_t* begin, const int32_t* len, uint
 
 // Sixteen rows a block, a wave each: first the bytes of every row's text and of the block's, then, each block adding the blocks before
 // it up, where a row begins, and its text.  (Rows beyond LINES_DIRECT are added up by the scan of the caption offsets instead.)
-constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64;
+// A wave holds LINE_AHEAD times 64 tokens at once, so that 256 tokens cost three rounds of memory latency: the tokens, where their texts stand, the texts.
+constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, LINE_AHEAD = 4;
 constexpr uint64_t LINES_DIRECT = 65536;
 
 __global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0,
@@ -1039,10 +1046,15 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const
     if (row < rows) {
         const Written w = written(begin, len, width, row);
         const auto t = glob(tokens) + row * stride;
-        const auto span = (Glob<unsigned long long>)glob((const unsigned long long*)g.span);
-        for (uint32_t k = w.first + lane; k < w.last; k += 64) {
-            const uint32_t id = (uint32_t)t[k];
-            if (id < g.n_tokens) n += (uint32_t)(span[id] >> 32);
+        const auto bytes = glob(g.bytes);
+        for (uint32_t k0 = w.first; k0 < w.last; k0 += LINE_AHEAD * 64) {
+            uint32_t id[LINE_AHEAD], of[LINE_AHEAD];
+#pragma unroll
+            for (uint32_t q = 0; q < LINE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
+#pragma unroll
+            for (uint32_t q = 0; q < LINE_AHEAD; ++q) of[q] = id[q] < g.n_tokens ? (uint32_t)bytes[id[q]] : 0u;
+#pragma unroll
+            for (uint32_t q = 0; q < LINE_AHEAD; ++q) n += of[q] == LONG_TOKEN ? glob((const uint32_t*)g.record)[id[q] * 4ull + 1] : of[q];
         }
         n = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
         if (lane == 0) sizes[row] = n;
@@ -1057,34 +1069,54 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const
     }
 }
 
-// A wave's text on its way out: collected in LDS at the place it has within its 16-byte pieces of memory, and stored by whole pieces.
+// A wave's text on its way out: collected in LDS at the place it has within its 16-byte pieces of memory, and stored by whole pieces.  Texts are put there
+// eight bytes at a time by two OR operations on aligned words of eight bytes (a byte at a time takes four times as many LDS operations), so the words are 0
+// where nothing has been put yet.
 constexpr uint32_t LINE_STAGE = 1024;
 typedef unsigned long long Bytes8 __attribute__((aligned(1)));
+typedef uint8_t __attribute__((address_space(1)))* OutBytes;
 struct Staged {
-    uint8_t* buf;                 // LINE_STAGE + 16 bytes
-    uint8_t __attribute__((address_space(1)))* piece;        // memory of buf[0], a multiple of 16
-    uint8_t __attribute__((address_space(1)))* end;          // the arena's end: nothing is stored at or behind it
-    uint32_t from, n;             // bytes [from, n) of buf are to be stored; from is 0 but in a row's first piece
+    unsigned long long* word;     // LINE_STAGE bytes and two words
+    OutBytes piece;               // memory of the first word, a multiple of 16
+    OutBytes end;                 // the arena's end: nothing is stored at or behind it
+    uint32_t from, n;             // bytes [from, n) are to be stored; from is 0 but in a row's first piece
 
-    __device__ void start(uint8_t __attribute__((address_space(1)))* at) {
+    __device__ uint8_t byte(uint32_t i) const { return ((const uint8_t*)word)[i]; }
+    __device__ void clear(uint32_t lane) {
+        block_sync<64>();
+        *(uint4*)(word + lane * 2) = make_uint4(0, 0, 0, 0);
+        if (lane < 2) word[LINE_STAGE / 8 + lane] = 0;
+        block_sync<64>();
+    }
+    __device__ void start(OutBytes at, uint32_t lane) {
         from = n = (uint32_t)((uintptr_t)at & 15);
         piece = at - from;
+        clear(lane);
+    }
+    // the low `count` (up to 8) bytes of `text` to byte i
+    __device__ void put(uint32_t i, unsigned long long text, uint32_t count) {
+        if (!count) return;
+        const uint32_t shift = (i & 7) * 8;
+        text &= ~0ull >> (64 - 8 * count);
+        atomicOr(word + (i >> 3), text << shift);
+        if ((i & 7) + count > 8) atomicOr(word + (i >> 3) + 1, text >> (64 - shift));
     }
     // the pieces that are full
     __device__ void flush(uint32_t lane) {
         const uint32_t full = n / 16;
         if (!full) return;
         block_sync<64>();
-        if (lane < 16 && lane >= from && piece + lane < end) piece[lane] = buf[lane];
+        if (lane < 16 && lane >= from && piece + lane < end) piece[lane] = byte(lane);
         for (uint32_t c = 1 + lane; c < full; c += 64) {
-            auto* to = piece + c * 16;
-            const Words4 d = *(const Words4*)(buf + c * 16);
+            const OutBytes to = piece + c * 16;
+            const Words4 d = *(const Words4*)(word + c * 2);
             if (to + 16 <= end) *(Words4 __attribute__((address_space(1)))*)to = d;
-            else for (uint32_t j = 0; j < 16; ++j) if (to + j < end) to[j] = buf[c * 16 + j];
+            else for (uint32_t j = 0; j < 16; ++j) if (to + j < end) to[j] = byte(c * 16 + j);
         }
-        const uint8_t rest = lane < (n & 15) ? buf[full * 16 + lane] : (uint8_t)0;
+        const unsigned long long rest = lane < 2 ? word[full * 2 + lane] : 0ull;    // the last piece's bytes, 0 from n on
+        clear(lane);
+        if (lane < 2) word[lane] = rest;
         block_sync<64>();
-        if (lane < 16) buf[lane] = rest;
         piece += full * 16;
         n &= 15;
         from = 0;
@@ -1092,13 +1124,13 @@ struct Staged {
     __device__ void finish(uint32_t lane) {
         flush(lane);
         block_sync<64>();
-        if (lane >= from && lane < n && piece + lane < end) piece[lane] = buf[lane];
+        if (lane >= from && lane < n && piece + lane < end) piece[lane] = byte(lane);
     }
 };
 
 __global__ __launch_bounds__(LINE_THREADS) void k_line_text(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0,
                                                             uint64_t rows, const uint32_t* sizes, const unsigned long long* sums, uint64_t* offsets, uint8_t* arena, uint64_t capacity) {
-    __shared__ alignas(16) uint8_t stage[LINE_ROWS][LINE_STAGE + 16];
+    __shared__ alignas(16) unsigned long long stage[LINE_ROWS][LINE_STAGE / 8 + 2];
     __shared__ unsigned long long before[LINE_ROWS];
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const uint64_t b = block0 + blockIdx.x, row = b * LINE_ROWS + wave;
@@ -1124,41 +1156,48 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_text(DevGrammar g, const 
     }
     const Written w = written(begin, len, width, row);
     const auto t = glob(tokens) + row * stride;
-    const auto span = (Glob<unsigned long long>)glob((const unsigned long long*)g.span);
+    const auto record = (Glob<Words4>)glob((const Words4*)g.record);
     const auto text = glob(g.text);
-    auto* const out = (uint8_t __attribute__((address_space(1)))*)arena;
+    const OutBytes out = (OutBytes)arena;
     Staged s;
-    s.buf = stage[wave];
+    s.word = stage[wave];
     s.end = out + capacity;
-    s.start(out + at);
-    for (uint32_t k0 = w.first; k0 < w.last; k0 += 64) {
-        uint32_t n = 0;
-        uint32_t from = 0;
-        if (k0 + lane < w.last) {
-            const uint32_t id = (uint32_t)t[k0 + lane];
-            if (id < g.n_tokens) { const unsigned long long e = span[id]; from = (uint32_t)e; n = (uint32_t)(e >> 32); }
-        }
-        const uint32_t incl = wave_scan(n), all = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63), to = incl - n;
-        if (all <= LINE_STAGE - 16) {
-            s.flush(lane);
-            uint8_t* d = s.buf + s.n + to;                                   // a flush leaves at most 15 bytes
-            // the texts are followed by 8 bytes of room, so that eight bytes can be read at once
-            for (uint32_t j = 0; j < n; j += 8) {
-                const unsigned long long c = *(const Bytes8 __attribute__((address_space(1)))*)(text + from + j);
+    s.start(out + at, lane);
+    for (uint32_t k0 = w.first; k0 < w.last; k0 += LINE_AHEAD * 64) {
+        uint32_t id[LINE_AHEAD];
+        Words4 rec[LINE_AHEAD];
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) if (j + i < n) d[j + i] = (uint8_t)(c >> (8 * i));
+        for (uint32_t q = 0; q < LINE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
+#pragma unroll
+        for (uint32_t q = 0; q < LINE_AHEAD; ++q) rec[q] = id[q] < g.n_tokens ? record[id[q]] : Words4{0, 0, 0, 0};
+#pragma unroll
+        for (uint32_t q = 0; q < LINE_AHEAD; ++q) {
+            if (k0 + q * 64 >= w.last) break;
+            const uint32_t kind = rec[q][3] >> 24, n = kind == LONG_TOKEN ? rec[q][1] : kind;
+            const uint32_t incl = wave_scan(n), all = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63), to = incl - n;
+            if (all <= LINE_STAGE - 16) {
+                s.flush(lane);
+                const uint32_t d = s.n + to;                                  // a flush leaves at most 15 bytes
+                if (kind != LONG_TOKEN) {
+                    s.put(d, (unsigned long long)rec[q][1] << 32 | rec[q][0], n < 8 ? n : 8);
+                    if (n > 8) s.put(d + 8, (unsigned long long)rec[q][3] << 32 | rec[q][2], n - 8);
+                } else {
+                    for (uint32_t j = 0; j < n; j += 8)                       // the texts are followed by eight bytes of room
+                        s.put(d + j, *(const Bytes8 __attribute__((address_space(1)))*)(text + rec[q][0] + j), n - j < 8 ? n - j : 8);
+                }
+                s.n += all;
+            } else {                                                          // texts longer than the stage: a lane stores its token's
+                s.finish(lane);
+                const OutBytes d = s.piece + s.n + to;
+                for (uint32_t j = 0; j < n; ++j)
+                    if (d + j < s.end) d[j] = kind == LONG_TOKEN ? text[rec[q][0] + j] : (uint8_t)((j < 8 ? j < 4 ? rec[q][0] : rec[q][1] : j < 12 ? rec[q][2] : rec[q][3]) >> (8 * (j & 3)));
+                s.start(s.piece + s.n + all, lane);
             }
-            s.n += all;
-        } else {                                                              // texts longer than the stage: a lane stores its token's
-            s.finish(lane);
-            auto* d = s.piece + s.n;
-            for (uint32_t j = 0; j < n; ++j) if (d + to + j < s.end) d[to + j] = text[from + j];
-            s.start(d + all);
         }
     }
     s.finish(lane);
     if (row == rows - 1) {
-        auto* d = s.piece + s.n;
+        const OutBytes d = s.piece + s.n;
         if (lane < 16 && d + lane < s.end) d[lane] = 0;
     }
 }
@@ -1237,9 +1276,9 @@ hipError_t launch_choose(const tp_logits& io, const float* temperature, const fl
 }
 
 hipError_t launch_grammar_mask(const DevGrammar& g, const int32_t* states, uint64_t rows, uint32_t* mask, uint64_t mask_stride, hipStream_t s) {
-    const uint32_t pieces = ((g.n_tokens + 31) / 32 + MASK_PIECE - 1) / MASK_PIECE;
-    return in_ranges(rows * pieces, [&](uint64_t b, unsigned n) {
-        hipLaunchKernelGGL(k_grammar_mask, dim3(n), dim3(256), 0, s, g, states, b, pieces, mask, mask_stride);
+    const uint32_t columns = ((g.n_tokens + 31) / 32 + MASK_PIECE - 1) / MASK_PIECE;
+    return in_row_ranges(rows, columns, [&](uint64_t r, unsigned n) {
+        hipLaunchKernelGGL(k_grammar_mask, dim3(columns, n), dim3(256), 0, s, g, states, r, mask, mask_stride);
     });
 }
 
