@@ -148,10 +148,6 @@ __device__ inline float wave_sum(float v) {
     v += dpp<0x143, 0xC>(0.0f, v);
     return read_lane(v, 63);
 }
-__device__ inline double wave_sum(double v) {
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d, 64);
-    return v;
-}
 // sum of the lanes up to and including this one
 __device__ inline uint32_t wave_scan(uint32_t v) {
     v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
@@ -162,14 +158,28 @@ __device__ inline uint32_t wave_scan(uint32_t v) {
     v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
     return v;
 }
+template <int CTRL, int ROWS>
+__device__ inline double dpp(double v) {                                      // 0 where no lane is the source
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ inline double read_lane(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ inline double wave_scan(double v) {
-    const int lane = (int)(threadIdx.x & 63);
-    for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(v, d, 64);
-        if (lane >= d) v += o;
-    }
+    v += dpp<0x111, 0xF>(v);
+    v += dpp<0x112, 0xF>(v);
+    v += dpp<0x114, 0xF>(v);
+    v += dpp<0x118, 0xF>(v);
+    v += dpp<0x142, 0xA>(v);
+    v += dpp<0x143, 0xC>(v);
     return v;
 }
+__device__ inline double wave_sum(double v) { return read_lane(wave_scan(v), 63); }
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------
 // A token's weight is 2^(x * k - c), k = log2(e) / T rounded once for the row and c = best * k rounded once for the tokens that are summed
@@ -602,9 +612,9 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
             found = over != 0;
             const int to = found ? __builtin_ctzll(over) : 63 - __builtin_clzll(live);
             segment = c0 + (uint32_t)to;
-            before = __shfl(incl - w, to, 64);
+            before = read_lane(incl - w, to);
         }
-        carry = __shfl(incl, 63, 64);
+        carry = read_lane(incl, 63);
     }
     const Scale within(p[segment].best, k);
     target = (target - before) / scale.of(within.best);
@@ -658,7 +668,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
                     if (first == 8 && cum > target) { first = (uint32_t)j; x_first = x[j]; }
                 }
             }
-            run = __shfl(incl, 63, 64);
+            run = read_lane(incl, 63);
         } else {
 #pragma unroll
             for (int j = 7; j >= 0; --j) if (x[j] == best) first = (uint32_t)j;
@@ -667,8 +677,8 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         if (!over && !live) continue;
         done = over != 0;
         const int to = done ? __builtin_ctzll(over) : 63 - __builtin_clzll(live);
-        at = (uint32_t)v * 512 + (uint32_t)to * 8 + (uint32_t)__shfl((int)((done ? first : last) - cut), to, 64);
-        x_at = __shfl(done ? x_first : x_last, to, 64);
+        at = (uint32_t)v * 512 + (uint32_t)to * 8 + (uint32_t)__builtin_amdgcn_readlane((int)((done ? first : last) - cut), to);
+        x_at = read_lane(done ? x_first : x_last, to);
     }
     if (lane == 0) {
         tokens[row] = (int32_t)(w0 + at);
@@ -900,9 +910,8 @@ struct Step {
     }
 
     template <class T>
-    static __device__ void run(const DevGrammar& g, const tp_logits& a, uint64_t row, const List& q, const float* temperature, const float* uniform, int32_t* states,
+    static __device__ void run(const DevGrammar& g, const tp_logits& a, const RowRules& r, uint64_t row, const List& q, const float* temperature, const float* uniform, int32_t* states,
                                int32_t* tokens, float* logprob, int append, Lds& s) {
-        const RowRules r = row_rules(a, row);
         const float t = temperature_of(temperature, uniform, row), k = weight_scale(t);
         const bool one = q.hi - q.lo <= PIECE, room = has_room(a, row, append);
         const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
@@ -964,9 +973,9 @@ struct Step {
                     found = over != 0;
                     const int to = found ? __builtin_ctzll(over) : 63 - __builtin_clzll(live);
                     at = (int)i0 + to;
-                    before = __shfl(incl - w, to, 64);
+                    before = read_lane(incl - w, to);
                 }
-                in_piece = __shfl(incl, 63, 64) - carry;
+                in_piece = read_lane(incl, 63) - carry;
             }
             if (at >= 0) mine = false;                                       // a later place than any before
             if (at >= 0 && at % WAVES == wave) {
@@ -1002,12 +1011,13 @@ __global__ __launch_bounds__(STEP_THREADS) void k_grammar_step(DevGrammar g, tp_
                                                                int32_t* states, int32_t* tokens, float* logprob, int append) {
     __shared__ union { LongStep::Lds l; ShortStep::Lds s; } lds;
     const uint64_t row = row0 + blockIdx.x;
+    const RowRules r = row_rules(a, row);
     const List q = list_of(g, states, row);
     if (q.hi - q.lo > ShortStep::PIECE) {
         __syncthreads();                                                     // every wave has read the state before one moves it
-        LongStep::run<T>(g, a, row, q, temperature, uniform, states, tokens, logprob, append, lds.l);
+        LongStep::run<T>(g, a, r, row, q, temperature, uniform, states, tokens, logprob, append, lds.l);
     } else if (threadIdx.x < 64) {
-        ShortStep::run<T>(g, a, row, q, temperature, uniform, states, tokens, logprob, append, lds.s);
+        ShortStep::run<T>(g, a, r, row, q, temperature, uniform, states, tokens, logprob, append, lds.s);
     }
 }
 
@@ -1034,7 +1044,7 @@ __device__ inline Written written(const int32_t* begin, const int32_t* len, uint
 // Sixteen rows a block, a wave each: first the bytes of every row's text and of the block's, then, each block adding the blocks before
 // it up, where a row begins, and its text.  (Rows beyond LINES_DIRECT are added up by the scan of the caption offsets instead.)
 // A wave holds LINE_AHEAD times 64 tokens at once, so that 256 tokens cost three rounds of memory latency: the tokens, where their texts stand, the texts.
-constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, LINE_AHEAD = 4;
+constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, LINE_AHEAD = 4, SIZE_AHEAD = 8;
 constexpr uint64_t LINES_DIRECT = 65536;
 
 __global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0,
@@ -1047,14 +1057,14 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const
         const Written w = written(begin, len, width, row);
         const auto t = glob(tokens) + row * stride;
         const auto bytes = glob(g.bytes);
-        for (uint32_t k0 = w.first; k0 < w.last; k0 += LINE_AHEAD * 64) {
-            uint32_t id[LINE_AHEAD], of[LINE_AHEAD];
+        for (uint32_t k0 = w.first; k0 < w.last; k0 += SIZE_AHEAD * 64) {
+            uint32_t id[SIZE_AHEAD], of[SIZE_AHEAD];
 #pragma unroll
-            for (uint32_t q = 0; q < LINE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
+            for (uint32_t q = 0; q < SIZE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
 #pragma unroll
-            for (uint32_t q = 0; q < LINE_AHEAD; ++q) of[q] = id[q] < g.n_tokens ? (uint32_t)bytes[id[q]] : 0u;
+            for (uint32_t q = 0; q < SIZE_AHEAD; ++q) of[q] = id[q] < g.n_tokens ? (uint32_t)bytes[id[q]] : 0u;
 #pragma unroll
-            for (uint32_t q = 0; q < LINE_AHEAD; ++q) n += of[q] == LONG_TOKEN ? glob((const uint32_t*)g.record)[id[q] * 4ull + 1] : of[q];
+            for (uint32_t q = 0; q < SIZE_AHEAD; ++q) n += of[q] == LONG_TOKEN ? glob((const uint32_t*)g.record)[id[q] * 4ull + 1] : of[q];
         }
         n = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
         if (lane == 0) sizes[row] = n;
