@@ -38,7 +38,8 @@ def _torch():
 
 
 def _stream(torch, device):
-    return torch.cuda.current_stream(device).cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)                 # the same number without a Stream object around it
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _refuse(name, t, device, dtype, shape):
@@ -283,7 +284,7 @@ def run_tokens(pipe, grammar, tokens, lengths, begin):
         io.arena, io.offsets, io.n_files = arena.data_ptr(), offsets.data_ptr(), rows
         io.captions, io.caption_capacity, io.caption_offsets = captions.data_ptr(), capacity, caption_offsets.data_ptr()
         io.verdicts, io.histogram, io.counters = verdicts.data_ptr(), histogram.data_ptr(), counters.data_ptr()
-        io.fired, io.facet_choice, io.stream = fired.data_ptr(), facets.data_ptr(), _stream(torch, device)
+        io.fired, io.facet_choice, io.stream = fired.data_ptr(), facets.data_ptr(), _stream(torch, pipe._device)
         try:
             total = pipe.run_lines_device(io)
             break
