@@ -130,13 +130,15 @@ __device__ inline float dpp(float old, float v) {
 }
 __device__ inline float read_lane(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
 
+// One instruction a step (the waits are for the step before, whose result another lane reads); a NaN is passed over.
 __device__ inline float wave_max(float v) {
-    v = fmaxf(v, dpp<0x111, 0xF>(v, v));   // row_shr:1, 2, 4, 8
-    v = fmaxf(v, dpp<0x112, 0xF>(v, v));
-    v = fmaxf(v, dpp<0x114, 0xF>(v, v));
-    v = fmaxf(v, dpp<0x118, 0xF>(v, v));
-    v = fmaxf(v, dpp<0x142, 0xA>(v, v));   // row_bcast:15 into rows 1 and 3
-    v = fmaxf(v, dpp<0x143, 0xC>(v, v));   // row_bcast:31 into rows 2 and 3
+    asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:1 row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:2 row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:4 row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_shr:8 row_mask:0xf bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_bcast:15 row_mask:0xa bank_mask:0xf\n\t"
+        "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_bcast:31 row_mask:0xc bank_mask:0xf\n\t"
+        "s_nop 1" : "+v"(v));
     return read_lane(v, 63);
 }
 __device__ inline float wave_sum(float v) {
@@ -330,7 +332,10 @@ __device__ inline void finish_segment(const RowRules& r, uint32_t w0, uint32_t n
     for (int v = 0; v < VECS; ++v)
         if (take[v] != 0xFFu) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[v][j] = take[v] >> j & 1 ? x[v][j] : NEG_INF;
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe((int)take[v], j, 1);   // all ones or none
+                x[v][j] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x[v][j]) & keep) | (0xFF800000u & ~keep));
+            }
         }
 }
 
@@ -509,7 +514,7 @@ struct Window {
 };
 
 // ---- the choice -------------------------------------------------------------------------------------------------------------
-// The first launch reads the logits once and leaves of every segment the largest x and the sum of the weights against it; a wave does
+// The first launch reads the logits once and leaves of every segment the sum of its weights and the x that they are relative to; a wave does
 // that by itself.  The second joins a row with one wave: the token's segment by a scan of the segments' shares, and the token in that segment, which
 // the wave shapes again (1024 tokens of the row).  A row of one window does both in the first launch.  A segment's sum is a 32-bit sum of 1024
 // weights in a tree of 10 levels; everything above is summed in 64.
@@ -517,9 +522,13 @@ using OneSegment = Window<1, 1>;
 constexpr int CHOICE_WAVES = 16, MOST_SEGS = 8;                               // waves of a block, segments of a wave at the most
 using Chunk = Window<CHOICE_WAVES, MOST_SEGS>;
 
+// Its weights are taken against `ref`, what the wave's segment before was taken against, and only where they outgrow it, or there is none, against
+// the segment's own largest x, which is `ref` from then on: the shares that the join works with do not mind what they are
+// relative to, and the largest need not be found.  With `greedy` it is the segment's largest in any case.
 template <class T, bool TINY>
-__device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32_t n, uint32_t g, const Held<T>& h, float k, uint32_t distinct, const Chunk::Lds& l, const uint32_t* value) {
-    float x[VECS][8], best = NEG_INF;
+__device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32_t n, uint32_t g, const Held<T>& h, float k, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
+                                          const uint32_t* value) {
+    float x[VECS][8];
     uint32_t take[VECS], i0 = 0, i1 = 0;
 #pragma unroll
     for (int v = 0; v < VECS; ++v) take[v] = h.take[v];
@@ -537,17 +546,17 @@ __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32
 #pragma unroll
     for (int v = 0; v < VECS; ++v) T::up8(h.d[v], x[v]);
     finish_segment<TINY>(r, w0, n, g, take, x);
-    auto sums = [&]() {
-        best = NEG_INF;
+    auto largest = [&]() {
+        float best = NEG_INF;
 #pragma unroll
         for (int v = 0; v < VECS; ++v)
 #pragma unroll
             for (int j = 0; j < 8; j += 2) best = max3(best, x[v][j], x[v][j + 1]);
         for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) best = fmaxf(best, countable(__builtin_bit_cast(float, value[i])));
-        best = wave_max(best);
-        const Scale scale(best, k);
+        return wave_max(best);
+    };
+    auto weights = [&](const Scale& scale) {
         float sum = 0.0f;
-        if (best == NEG_INF) return sum;
         if (!scale.equal) {
 #pragma unroll
             for (int v = 0; v < VECS; ++v) {
@@ -565,15 +574,17 @@ __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32
         for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) sum += scale.weight(countable(__builtin_bit_cast(float, value[i])));
         return wave_sum(sum);
     };
-    float sum = sums();
-    if (sum != sum || best != best) {                                         // a NaN among the logits: out with it, and again
+    if (greedy || ref == NEG_INF) ref = largest();
+    float sum = weights(Scale(ref, k));
+    if (!(sum < 1e30f) || Scale(ref, k).equal) {                              // outgrown, or a NaN among the logits, or no scale to go by
 #pragma unroll
         for (int v = 0; v < VECS; ++v)
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[v][j] = countable(x[v][j]);
-        sum = sums();
+        ref = largest();
+        sum = ref == NEG_INF ? 0.0f : weights(Scale(ref, k));
     }
-    return ChoicePart{best, sum};
+    return ChoicePart{ref, sum};
 }
 
 // Joins a row's segments: all lanes of one wave.  Tables: Chunk where the row's own window stands in LDS (`distinct` of it), OneSegment
@@ -697,15 +708,16 @@ __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_
     const RowRules r = row_rules(a, row);
     const auto from = logit_row<T>(a, row) + w0;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * CHOICE_WAVES, reply_segments(n));
-    History<CHOICE_WAVES * 64, 2> history;
+    History<CHOICE_WAVES * 64, 1> history;
     history.load(r, w0);
     // two segments in turn: one's loads are in flight while the other is worked on (and stay in the registers they were sent to)
     Held<T> even, odd;
     if (wave < last) load_segment<T, TINY>(r, from, w0, n, wave, even);
     const uint32_t distinct = Chunk::repeated<T>(r, history, from, w0, std::min(n, window), l, dynamic_lds);
     ChoicePart* out = parts + row * segments + w0 / SEGMENT;
+    float ref = NEG_INF;
     auto part = [&](uint32_t g, const Held<T>& h) {
-        const ChoicePart p = segment_part<T, TINY>(r, w0, n, g, h, k, distinct, l, dynamic_lds);
+        const ChoicePart p = segment_part<T, TINY>(r, w0, n, g, h, k, t == 0.0f, ref, distinct, l, dynamic_lds);
         if ((threadIdx.x & 63) == 0) {
             if (chunks > 1) out[g] = p; else here[g] = p;
         }
@@ -817,19 +829,64 @@ __device__ inline bool has_room(const tp_logits& a, uint64_t row, int append) { 
 
 // The choice among a row's list.  THREADS threads hold EACH entries apiece: entry, logit and bias of all of them are loaded before any is used,
 // so that a list costs two rounds of memory latency (entries, then what they point to) whatever its length up to
-// THREADS * EACH.  Only the listed tokens' logits are read.  History tokens are looked up among the list's ascending tokens in LDS.  A
-// longer list is worked on in pieces, twice: for the largest x and the sum, and for the place.
-template <int THREADS, int EACH>
+// THREADS * EACH.  Only the listed tokens' logits are read.  The history goes through a hash table in LDS, a part of THREADS * RECALL entries at a time,
+// in which every entry of the list looks its token up.  (Looking every history token up in the sorted list takes a binary search of
+// dependent LDS reads: 3.4 of the 8.5 us that a list of 4781 took.)  A list longer than THREADS * EACH is worked on in pieces,
+// twice: for the largest x and the sum, and for the place.
+template <int THREADS, int EACH, int RECALL>
 struct Step {
     static constexpr uint32_t PIECE = THREADS * EACH;
     static constexpr int WAVES = THREADS / 64, SEGMENTS = WAVES * EACH;      // a wave's 64 entries of one round are a segment, in token order
+    static constexpr uint32_t SLOTS = 2 * THREADS * RECALL, EMPTY = 0xFFFFFFFFu;   // at most half of the slots are taken: a search ends
+    static_assert((SLOTS & (SLOTS - 1)) == 0, "a power of two");
     struct Lds {
-        uint32_t token[PIECE];
-        uint32_t cnt[PIECE];
+        alignas(16) uint32_t key[SLOTS];
+        alignas(16) uint32_t cnt[SLOTS];
         float sum[SEGMENTS];
         float max[WAVES];
         uint32_t first;
     };
+    static __device__ uint32_t slot_of(uint32_t token) { return (token * 0x9E3779B1u) >> (32 - __builtin_ctz(SLOTS)); }
+
+    // count words of the thread's entries
+    static __device__ void recall(const DevGrammar& g, const RowRules& r, const uint2 (&en)[EACH], Lds& s, uint32_t (&c)[EACH]) {
+        const uint32_t tid = threadIdx.x;
+        for (uint32_t k0 = 0; k0 < r.len; k0 += THREADS * RECALL) {
+            uint32_t token[RECALL];
+#pragma unroll
+            for (int i = 0; i < RECALL; ++i) { const uint32_t k = k0 + i * THREADS + tid; token[i] = k < r.len ? (uint32_t)r.history[k] : EMPTY; }
+            block_sync<THREADS>();                                           // the part before has been looked up
+#pragma unroll
+            for (uint32_t i = tid * 4; i < SLOTS; i += THREADS * 4) {
+                *(uint4*)(s.key + i) = make_uint4(EMPTY, EMPTY, EMPTY, EMPTY);
+                *(uint4*)(s.cnt + i) = make_uint4(0, 0, 0, 0);
+            }
+            block_sync<THREADS>();
+#pragma unroll
+            for (int i = 0; i < RECALL; ++i) {
+                if (token[i] >= g.n_tokens) continue;                           // none: EMPTY among them
+                uint32_t h = slot_of(token[i]);
+                for (;; h = (h + 1) & (SLOTS - 1)) {
+                    const uint32_t was = atomicCAS(&s.key[h], EMPTY, token[i]);
+                    if (was == EMPTY || was == token[i]) break;
+                }
+                if (k0 + i * THREADS + tid >= r.prompt) atomicAdd(&s.cnt[h], 1u); else atomicOr(&s.cnt[h], SEEN);
+            }
+            block_sync<THREADS>();
+            uint32_t found[EACH];
+#pragma unroll
+            for (int v = 0; v < EACH; ++v) found[v] = s.key[slot_of(en[v].x)];
+#pragma unroll
+            for (int v = 0; v < EACH; ++v) {
+                uint32_t h = slot_of(en[v].x);
+                while (found[v] != EMPTY && found[v] != en[v].x) { h = (h + 1) & (SLOTS - 1); found[v] = s.key[h]; }
+                if (found[v] != EMPTY) {
+                    const uint32_t n = s.cnt[h];
+                    c[v] = (c[v] + (n & ~SEEN)) | (n & SEEN);
+                }
+            }
+        }
+    }
 
     // x of the m entries from e0: entry i of the piece is thread i % THREADS's number i / THREADS; -infinity where it may not be taken
     template <class T>
@@ -842,37 +899,17 @@ struct Step {
         float b[EACH];
 #pragma unroll
         for (int v = 0; v < EACH; ++v) {
-            const unsigned long long e = (uint32_t)v * THREADS + tid < m ? entries[v * THREADS + tid] : 0xFFFFFFFFull;
+            const unsigned long long e = (uint32_t)v * THREADS + tid < m ? entries[v * THREADS + tid] : (unsigned long long)EMPTY;
             en[v] = make_uint2((uint32_t)e, (uint32_t)(e >> 32));
         }
 #pragma unroll
         for (int v = 0; v < EACH; ++v) {
-            ok[v] = en[v].x != 0xFFFFFFFFu && may(en[v].y, tags, g);
+            ok[v] = en[v].x != EMPTY && may(en[v].y, tags, g);
             raw[v] = ok[v] ? l[en[v].x] : (typename T::S)0;
             b[v] = ok[v] && r.bias ? r.bias[en[v].x] : 0.0f;
         }
         uint32_t c[EACH] = {};
-        if (r.len) {
-            block_sync<THREADS>();                                           // the piece before is done with the tables
-#pragma unroll
-            for (int v = 0; v < EACH; ++v)
-                if ((uint32_t)v * THREADS + tid < m) { s.token[v * THREADS + tid] = en[v].x; s.cnt[v * THREADS + tid] = 0; }
-            block_sync<THREADS>();
-            for (uint32_t k = tid; k < r.len; k += THREADS) {
-                const uint32_t h = (uint32_t)r.history[k];
-                uint32_t lo = 0, hi = m;
-                while (lo < hi) {
-                    const uint32_t mid = (lo + hi) / 2;
-                    if (s.token[mid] < h) lo = mid + 1; else hi = mid;
-                }
-                if (lo < m && s.token[lo] == h) {
-                    if (k >= r.prompt) atomicAdd(&s.cnt[lo], 1u); else atomicOr(&s.cnt[lo], SEEN);
-                }
-            }
-            block_sync<THREADS>();
-#pragma unroll
-            for (int v = 0; v < EACH; ++v) if ((uint32_t)v * THREADS + tid < m) c[v] = s.cnt[v * THREADS + tid];
-        }
+        recall(g, r, en, s, c);
 #pragma unroll
         for (int v = 0; v < EACH; ++v) {
             float y = penalised(T::up(raw[v]), c[v], r);
@@ -1003,8 +1040,8 @@ struct Step {
 // A block per row.  Most places of a tag line have a handful of tokens, and the places where a tag begins thousands: a list of up to 64
 // is the work of one wave, which needs no barrier, and the block's other waves are done at once.
 constexpr int STEP_THREADS = 1024;
-using LongStep = Step<STEP_THREADS, 8>;
-using ShortStep = Step<64, 1>;
+using LongStep = Step<STEP_THREADS, 8, 1>;
+using ShortStep = Step<64, 1, 4>;
 
 template <class T>
 __global__ __launch_bounds__(STEP_THREADS) void k_grammar_step(DevGrammar g, tp_logits a, uint64_t row0, const float* temperature, const float* uniform,
