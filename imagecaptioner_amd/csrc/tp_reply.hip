@@ -250,7 +250,7 @@ extern __shared__ uint32_t dynamic_lds[];
 // are left out by their bits of `take`.  (TINY: a vocabulary of fewer than eight tokens, loaded one by one.)
 template <class T>
 struct Held {
-    Words4 d[VECS][T::VEC];
+    Words4 d[VECS][T::VEC], b[VECS][2];                                       // logits, biases
     uint32_t take[VECS];                                                      // tokens that are this lane's, inside the row and allowed by the mask
 };
 __device__ inline uint32_t lane_at(uint32_t segment) { return segment * SEGMENT + (threadIdx.x & 63) * 8; }
@@ -261,10 +261,20 @@ template <class E>
 using Vec = const typename At<E>::W __attribute__((address_space(1)));
 
 // `n`: tokens from the window's start to the row's end
-template <class T, bool TINY>
+// ONCE: the loads do not ask the caches to keep the logits, which nobody reads again, so that a shared bias keeps its place there (choosing for 512 rows
+// of 131072 with one: 47 -> 45 us).  Shaping, which writes what it reads, is slower that way (256 rows of 131071 in 32 bits: 51 -> 57 us).
+template <class T, bool TINY, bool ONCE>
 __device__ inline void load_segment(const RowRules& r, Glob<typename T::S> row, uint32_t w0, uint32_t n, uint32_t segment, Held<T>& h) {
     using S = typename T::S;
     const uint32_t at = lane_at(segment);
+    if (r.bias && !TINY) {
+#pragma unroll
+        for (int v = 0; v < VECS; ++v) {
+            auto* from = (Vec<uint32_t>*)(r.bias + w0 + (int32_t)std::min((int32_t)(at + v * 512), (int32_t)n - 8));
+            h.b[v][0] = from[0];
+            h.b[v][1] = from[1];
+        }
+    }
     if constexpr (TINY) {
 #pragma unroll
         for (int v = 0; v < VECS; ++v) {
@@ -292,7 +302,11 @@ __device__ inline void load_segment(const RowRules& r, Glob<typename T::S> row, 
             h.take[v] = bits[v] << cut_of(t, n) & 0xFFu;
             if (h.take[v])
 #pragma unroll
-                for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((Vec<S>*)(row + (int32_t)std::min((int32_t)t, (int32_t)n - 8)))[g];
+                for (int g = 0; g < T::VEC; ++g) {
+                    auto* from = (Vec<S>*)(row + (int32_t)std::min((int32_t)t, (int32_t)n - 8)) + g;
+                    if constexpr (ONCE) h.d[v][g] = __builtin_nontemporal_load(from);
+                    else h.d[v][g] = *from;
+                }
         }
     } else {
 #pragma unroll
@@ -300,13 +314,17 @@ __device__ inline void load_segment(const RowRules& r, Glob<typename T::S> row, 
             const uint32_t t = at + v * 512;
             h.take[v] = 0xFFu << cut_of(t, n) & 0xFFu;
 #pragma unroll
-            for (int g = 0; g < T::VEC; ++g) h.d[v][g] = ((Vec<S>*)(row + (int32_t)std::min((int32_t)t, (int32_t)n - 8)))[g];
+            for (int g = 0; g < T::VEC; ++g) {
+                auto* from = (Vec<S>*)(row + (int32_t)std::min((int32_t)t, (int32_t)n - 8)) + g;
+                if constexpr (ONCE) h.d[v][g] = __builtin_nontemporal_load(from);
+                else h.d[v][g] = *from;
+            }
         }
     }
 }
 // the bias, and -infinity where `take` has no bit
-template <bool TINY>
-__device__ inline void finish_segment(const RowRules& r, uint32_t w0, uint32_t n, uint32_t segment, const uint32_t (&take)[VECS], float (&x)[VECS][8]) {
+template <class T, bool TINY>
+__device__ inline void finish_segment(const RowRules& r, uint32_t n, uint32_t segment, const Held<T>& h, const uint32_t (&take)[VECS], float (&x)[VECS][8]) {
     const uint32_t at = lane_at(segment);
     if (r.bias) {
         if constexpr (TINY) {
@@ -315,17 +333,10 @@ __device__ inline void finish_segment(const RowRules& r, uint32_t w0, uint32_t n
 #pragma unroll
                 for (int j = 0; j < 8; ++j) if (take[v] >> j & 1) x[v][j] = x[v][j] + r.bias[j - cut_of(at + v * 512, n)];
         } else {
-            Words4 b[VECS][2];
-#pragma unroll
-            for (int v = 0; v < VECS; ++v) {
-                auto* from = (Vec<uint32_t>*)(r.bias + w0 + (int32_t)std::min((int32_t)(at + v * 512), (int32_t)n - 8));
-                b[v][0] = from[0];
-                b[v][1] = from[1];
-            }
 #pragma unroll
             for (int v = 0; v < VECS; ++v)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[v][j] = x[v][j] + __builtin_bit_cast(float, (uint32_t)b[v][j >> 2][j & 3]);
+                for (int j = 0; j < 8; ++j) x[v][j] = x[v][j] + __builtin_bit_cast(float, (uint32_t)h.b[v][j >> 2][j & 3]);
         }
     }
 #pragma unroll
@@ -388,7 +399,7 @@ __global__ __launch_bounds__(SHAPE_WAVES * 64) __attribute__((amdgpu_waves_per_e
     History<THREADS, 4> history;
     history.load(r, w0);
     Held<T> h;
-    load_segment<T, TINY>(r, logit_row<T>(a, row) + w0, w0, n, g, h);
+    load_segment<T, TINY, false>(r, logit_row<T>(a, row) + w0, w0, n, g, h);
     if (r.len) {
         for (uint32_t k = threadIdx.x * 4; k < SHAPE_TOKENS; k += THREADS * 4) *(uint4*)(cnt + k) = make_uint4(0, 0, 0, 0);
         __syncthreads();
@@ -415,7 +426,7 @@ __global__ __launch_bounds__(SHAPE_WAVES * 64) __attribute__((amdgpu_waves_per_e
             }
         }
     }
-    finish_segment<TINY>(r, w0, n, g, h.take, x);
+    finish_segment<T, TINY>(r, n, g, h, h.take, x);
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
         const uint32_t t = at + v * 512, cut = cut_of(t, n);
@@ -525,9 +536,9 @@ using Chunk = Window<CHOICE_WAVES, MOST_SEGS>;
 // Its weights are taken against `ref`, what the wave's segment before was taken against, and only where they outgrow it, or there is none, against
 // the segment's own largest x, which is `ref` from then on: the shares that the join works with do not mind what they are
 // relative to, and the largest need not be found.  With `greedy` it is the segment's largest in any case.
-template <class T, bool TINY>
-__device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32_t n, uint32_t g, const Held<T>& h, float k, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
-                                          const uint32_t* value) {
+template <class T, bool TINY, class Next>
+__device__ inline ChoicePart segment_part(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, float k, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
+                                          const uint32_t* value, Next&& next) {
     float x[VECS][8];
     uint32_t take[VECS], i0 = 0, i1 = 0;
 #pragma unroll
@@ -545,7 +556,8 @@ __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t w0, uint32
     }
 #pragma unroll
     for (int v = 0; v < VECS; ++v) T::up8(h.d[v], x[v]);
-    finish_segment<TINY>(r, w0, n, g, take, x);
+    finish_segment<T, TINY>(r, n, g, h, take, x);
+    next();                                                                   // `h` is free for the loads of the wave's next segment
     auto largest = [&]() {
         float best = NEG_INF;
 #pragma unroll
@@ -633,11 +645,11 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     const auto from = logit_row<T>(a, row) + w0;
     Held<T> h;
     if constexpr (HERE) {
-        load_segment<T, TINY>(r, from, w0, n, 0, h);
+        load_segment<T, TINY, false>(r, from, w0, n, 0, h);
     } else {
         History<64, 8> history;
         history.load(r, w0);
-        load_segment<T, TINY>(r, from, w0, n, 0, h);
+        load_segment<T, TINY, false>(r, from, w0, n, 0, h);
         distinct = OneSegment::repeated<T>(r, history, from, w0, std::min(n, SEGMENT), l, value);
     }
     uint32_t at = 0;
@@ -647,7 +659,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     float xs[VECS][8];
 #pragma unroll
     for (int v = 0; v < VECS; ++v) T::up8(h.d[v], xs[v]);
-    finish_segment<TINY>(r, w0, n, 0, h.take, xs);
+    finish_segment<T, TINY>(r, n, 0, h, h.take, xs);
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
         if (done) continue;
@@ -710,23 +722,18 @@ __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * CHOICE_WAVES, reply_segments(n));
     History<CHOICE_WAVES * 64, 1> history;
     history.load(r, w0);
-    // two segments in turn: one's loads are in flight while the other is worked on (and stay in the registers they were sent to)
-    Held<T> even, odd;
-    if (wave < last) load_segment<T, TINY>(r, from, w0, n, wave, even);
+    Held<T> h;
+    if (wave < last) load_segment<T, TINY, true>(r, from, w0, n, wave, h);
     const uint32_t distinct = Chunk::repeated<T>(r, history, from, w0, std::min(n, window), l, dynamic_lds);
     ChoicePart* out = parts + row * segments + w0 / SEGMENT;
     float ref = NEG_INF;
-    auto part = [&](uint32_t g, const Held<T>& h) {
-        const ChoicePart p = segment_part<T, TINY>(r, w0, n, g, h, k, t == 0.0f, ref, distinct, l, dynamic_lds);
+    for (uint32_t g = wave; g < last; g += CHOICE_WAVES) {
+        const ChoicePart p = segment_part<T, TINY>(r, n, g, h, k, t == 0.0f, ref, distinct, l, dynamic_lds, [&] {
+            if (g + CHOICE_WAVES < last) load_segment<T, TINY, true>(r, from, w0, n, g + CHOICE_WAVES, h);
+        });
         if ((threadIdx.x & 63) == 0) {
             if (chunks > 1) out[g] = p; else here[g] = p;
         }
-    };
-    for (uint32_t g = wave; g < last; g += 2 * CHOICE_WAVES) {
-        if (g + CHOICE_WAVES < last) load_segment<T, TINY>(r, from, w0, n, g + CHOICE_WAVES, odd);
-        part(g, even);
-        if (g + 2 * CHOICE_WAVES < last) load_segment<T, TINY>(r, from, w0, n, g + 2 * CHOICE_WAVES, even);
-        if (g + CHOICE_WAVES < last) part(g + CHOICE_WAVES, odd);
     }
     if (chunks > 1) return;
     __syncthreads();
