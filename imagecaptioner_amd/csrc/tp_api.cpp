@@ -1218,6 +1218,7 @@ tp_ctx* tp_create(const tp_config* cfg) {
         own_config(c.get(), *cfg);
         load_tables(c.get(), nullptr);
         c->public_strings = c->ht.strings;
+        HIP_OK(load_reply_kernels());
         // Tags in no table are kept when no strict vocabulary drops them; the lean stage notes the ones it meets so that
         // later calls find them interned (TAGPIPE_NO_LEARN=1: off)
         c->learning = c->use_lean && !c->dt.drop_unknown;

@@ -23,6 +23,8 @@ struct DevGrammar {
     uint32_t min_tags, max_tags;
 };
 
+// Loads the kernels' code on the current device, so that the first call of one may already be a captured one.
+hipError_t load_reply_kernels();
 hipError_t launch_shape(const tp_logits& io, void* out, uint64_t out_stride);
 hipError_t launch_choose(const tp_logits& io, const float* temperature, const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts);
 hipError_t launch_grammar_mask(const DevGrammar& g, const int32_t* states, uint64_t rows, uint32_t* mask, uint64_t mask_stride, hipStream_t s);

@@ -1188,29 +1188,40 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_text(DevGrammar g, const 
     __shared__ unsigned long long before[LINE_ROWS];
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const uint64_t b = block0 + blockIdx.x, row = b * LINE_ROWS + wave;
-    uint64_t at;
+    const bool mine = row < rows;
+    const Written w = mine ? written(begin, len, width, row) : Written{0, 0};
+    const auto t = glob(tokens) + row * stride;
+    const auto record = glob((const Words4*)g.record);
+    Words4 rec[LINE_AHEAD];
+    auto load = [&](uint32_t k0) {                                               // 256 tokens of the row, 64 apart in a lane
+        uint32_t id[LINE_AHEAD];
+#pragma unroll
+        for (uint32_t q = 0; q < LINE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
+#pragma unroll
+        for (uint32_t q = 0; q < LINE_AHEAD; ++q) rec[q] = id[q] < g.n_tokens ? record[id[q]] : Words4{0, 0, 0, 0};
+    };
+    load(w.first);                                                              // in flight while the row's place is found
+    uint64_t at = 0;
     if (sums) {
         unsigned long long sum = 0;
         for (uint64_t i = threadIdx.x; i < b; i += LINE_THREADS) sum += sums[i];
+        const uint32_t size = lane < LINE_ROWS && b * LINE_ROWS + lane < rows ? sizes[b * LINE_ROWS + lane] : 0u;
         for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
         if (lane == 0) before[wave] = sum;
         __syncthreads();
-        at = 0;
-        for (uint32_t w = 0; w < LINE_ROWS; ++w) at += before[w];
-        const uint32_t mine = lane < LINE_ROWS && b * LINE_ROWS + lane < rows ? sizes[b * LINE_ROWS + lane] : 0u;
-        for (uint32_t w = 0; w < wave; ++w) at += (uint32_t)__builtin_amdgcn_readlane((int)mine, (int)w);
-        if (row >= rows) return;
-        if (lane == 0) {
+        sum = lane < LINE_ROWS ? before[lane] : 0ull;                             // the blocks before, a wave's share a lane
+        sum += lane < wave ? size : 0u;                                           // and the block's rows before this one
+        for (int d = 8; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        at = sum;                                                                 // of the first sixteen lanes
+        at = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at);
+        if (mine && lane == 0) {
             offsets[row] = at;
             if (row == rows - 1) offsets[rows] = at + sizes[row];
         }
-    } else {
-        if (row >= rows) return;
+    } else if (mine) {
         at = offsets[row];
     }
-    const Written w = written(begin, len, width, row);
-    const auto t = glob(tokens) + row * stride;
-    const auto record = (Glob<Words4>)glob((const Words4*)g.record);
+    if (!mine) return;
     const auto text = glob(g.text);
     const OutBytes out = (OutBytes)arena;
     Staged s;
@@ -1218,12 +1229,7 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_text(DevGrammar g, const 
     s.end = out + capacity;
     s.start(out + at, lane);
     for (uint32_t k0 = w.first; k0 < w.last; k0 += LINE_AHEAD * 64) {
-        uint32_t id[LINE_AHEAD];
-        Words4 rec[LINE_AHEAD];
-#pragma unroll
-        for (uint32_t q = 0; q < LINE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
-#pragma unroll
-        for (uint32_t q = 0; q < LINE_AHEAD; ++q) rec[q] = id[q] < g.n_tokens ? record[id[q]] : Words4{0, 0, 0, 0};
+        if (k0 != w.first) load(k0);
 #pragma unroll
         for (uint32_t q = 0; q < LINE_AHEAD; ++q) {
             if (k0 + q * 64 >= w.last) break;
@@ -1291,6 +1297,11 @@ hipError_t by_type_and_size(const tp_logits& io, F&& f) {
 }
 
 }  // namespace
+
+hipError_t load_reply_kernels() {
+    hipFuncAttributes attr;                                                    // of one of them: they are one code object
+    return hipFuncGetAttributes(&attr, (const void*)k_grammar_mask);
+}
 
 hipError_t launch_shape(const tp_logits& io, void* out, uint64_t out_stride) {
     const uint32_t chunks = (io.vocab + SHAPE_TOKENS - 1) / SHAPE_TOKENS;
