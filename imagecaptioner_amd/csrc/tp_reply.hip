@@ -662,7 +662,6 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     finish_segment<T, TINY>(r, n, 0, h, h.take, xs);
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
-        if (done) continue;
         float (&x)[8] = xs[v];
         const uint32_t t0 = l0 + lane_at(0) + v * 512, cut = cut_of(lane_at(0) + v * 512, n);
         const uint32_t hit = distinct && cut < 8 ? (uint32_t)((const uint8_t*)l.seen)[t0 >> 3] << cut & 0xFFu : 0u;
@@ -671,17 +670,19 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
 #pragma unroll
             for (int j = 0; j < 8; ++j) if (hit >> j & 1) x[j] = __builtin_bit_cast(float, value[i++]);
         }
+        float w[8];
+        double mine = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w[j] = within.weight(countable(x[j]));
+            mine += (double)w[j];
+        }
+        const double incl = run + wave_scan(mine);
+        run = read_lane(incl, 63);
+        if (done) continue;
         uint32_t first = 8, last = 8;
         float x_first = best, x_last = best;
         if (t > 0.0f) {
-            float w[8];
-            double mine = 0.0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                w[j] = within.weight(countable(x[j]));
-                mine += (double)w[j];
-            }
-            const double incl = run + wave_scan(mine);
             double cum = incl - mine;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -691,7 +692,6 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
                     if (first == 8 && cum > target) { first = (uint32_t)j; x_first = x[j]; }
                 }
             }
-            run = read_lane(incl, 63);
         } else {
 #pragma unroll
             for (int j = 7; j >= 0; --j) if (x[j] == best) first = (uint32_t)j;
@@ -703,6 +703,9 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         at = (uint32_t)v * 512 + (uint32_t)to * 8 + (uint32_t)__builtin_amdgcn_readlane((int)((done ? first : last) - cut), to);
         x_at = read_lane(done ? x_first : x_last, to);
     }
+    // The token's own segment is now known to 64 bits: where the token has nearly all the weight, its logarithm is that of a number next to 1, and the
+    // segment's sum in 32 bits would have rounded the rest away.
+    sum += (run - (double)p[segment].sum) * scale.of(within.best);
     if (lane == 0) {
         tokens[row] = (int32_t)(w0 + at);
         if (logprob) logprob[row] = scale.log_share(x_at, sum);
@@ -849,7 +852,7 @@ struct Step {
     struct Lds {
         alignas(16) uint32_t key[SLOTS];
         alignas(16) uint32_t cnt[SLOTS];
-        float sum[SEGMENTS];
+        double sum[SEGMENTS];
         float max[WAVES];
         uint32_t first;
     };
@@ -941,15 +944,15 @@ struct Step {
         const Scale scale(best, k);
 #pragma unroll
         for (int v = 0; v < EACH; ++v) {
-            const float w = wave_sum(best > NEG_INF ? scale.weight(x[v]) : 0.0f);
+            const double w = wave_sum(best > NEG_INF ? (double)scale.weight(x[v]) : 0.0);
             if ((threadIdx.x & 63) == 0) s.sum[v * WAVES + (threadIdx.x >> 6)] = w;
         }
         block_sync<THREADS>();
     }
-    static __device__ double segment(const Lds& s, uint32_t i) { return i < (uint32_t)SEGMENTS ? (double)s.sum[i] : 0.0; }
+    static __device__ double segment(const Lds& s, uint32_t i) { return i < (uint32_t)SEGMENTS ? s.sum[i] : 0.0; }
     static __device__ double piece_sum(const Lds& s) {
         double w = 0.0;
-        for (uint32_t i = threadIdx.x & 63; i < (uint32_t)SEGMENTS; i += 64) w += (double)s.sum[i];
+        for (uint32_t i = threadIdx.x & 63; i < (uint32_t)SEGMENTS; i += 64) w += s.sum[i];
         return wave_sum(w);
     }
 
