@@ -528,7 +528,12 @@ struct Window {
 // The first launch reads the logits once and leaves of every segment the sum of its weights and the x that they are relative to; a wave does
 // that by itself.  The second joins a row with one wave: the token's segment by a scan of the segments' shares, and the token in that segment, which
 // the wave shapes again (1024 tokens of the row).  A row of one window does both in the first launch.  A segment's sum is a 32-bit sum of 1024
-// weights in a tree of 10 levels; everything above is summed in 64.
+// weights in a tree of 10 levels (and one rounding more for a lane with repeated tokens), off by 11 half steps at most; the segments are
+// summed in 64 bits, and so is the chosen token's own segment when the join works on it.
+//
+// What bounds it: 512 rows of 131072 bfloat16 (134 MB, 26 us at a copy's rate) with 256 tokens of history and a bias take 40 us: the vector units
+// spend some 250 instructions a segment, most of them in the powers and the sums; the block's start (rules, history and repeated tokens: 6 us) and the join of the
+// row (4 us) are chains of latency that only other blocks hide.  Without rules the launch reads at 5.8 TB/s.
 using OneSegment = Window<1, 1>;
 constexpr int CHOICE_WAVES = 16, MOST_SEGS = 8;                               // waves of a block, segments of a wave at the most
 using Chunk = Window<CHOICE_WAVES, MOST_SEGS>;
@@ -583,8 +588,9 @@ __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t n, uint32_
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum += scale.weight(x[v][j]);
         }
-        for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) sum += scale.weight(countable(__builtin_bit_cast(float, value[i])));
-        return wave_sum(sum);
+        double more = 0.0;                                                    // up to sixteen, one after another
+        for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) more += (double)scale.weight(countable(__builtin_bit_cast(float, value[i])));
+        return wave_sum(i1 > i0 ? (float)((double)sum + more) : sum);
     };
     if (greedy || ref == NEG_INF) ref = largest();
     float sum = weights(Scale(ref, k));
@@ -791,7 +797,8 @@ __device__ inline uint32_t lower_entry_wave(const uint2* entry, uint32_t lo, uin
 }
 
 // A block writes MASK_PIECE words of one row: cleared in LDS, the list's entries that fall into the piece set there, stored
-// in 16-byte pieces.  Of a list longer than a few rounds of the block only the piece's own part is read.
+// in 16-byte pieces.  Of a list longer than a few rounds of the block only the piece's own part is read.  Bound by the blocks of the long
+// lists: 1024 rows over 131072 tokens (17 MB of mask, 4 us at a copy's rate) take 7.2 us.
 constexpr uint32_t MASK_PIECE = 1024, MASK_AHEAD = 4;
 __global__ __launch_bounds__(256) void k_grammar_mask(DevGrammar g, const int32_t* states, uint64_t row0, uint32_t* mask, uint64_t mask_stride) {
     __shared__ alignas(16) uint32_t bits[MASK_PIECE];
@@ -1048,7 +1055,9 @@ struct Step {
 };
 
 // A block per row.  Most places of a tag line have a handful of tokens, and the places where a tag begins thousands: a list of up to 64
-// is the work of one wave, which needs no barrier, and the block's other waves are done at once.
+// is the work of one wave, which needs no barrier, and the block's other waves are done at once.  Bound by latency: 256 rows over
+// 131072 tokens and lists of up to 4781 take 16 us, one row 14, of which the bytes (1.3 MB, 0.3 us) are next to nothing; rules and list, entries, their
+// logits, the history's table, the sums and the choice each wait for what comes before.
 constexpr int STEP_THREADS = 1024;
 using LongStep = Step<STEP_THREADS, 8, 1>;
 using ShortStep = Step<64, 1, 4>;
@@ -1060,8 +1069,9 @@ __global__ __launch_bounds__(STEP_THREADS) void k_grammar_step(DevGrammar g, tp_
     const uint64_t row = row0 + blockIdx.x;
     const RowRules r = row_rules(a, row);
     const List q = list_of(g, states, row);
-    if (q.hi - q.lo > ShortStep::PIECE) {
-        __syncthreads();                                                     // every wave has read the state before one moves it
+    const bool many = q.hi - q.lo > ShortStep::PIECE;
+    __syncthreads();                                                         // every wave has read the state before one moves it
+    if (many) {
         LongStep::run<T>(g, a, r, row, q, temperature, uniform, states, tokens, logprob, append, lds.l);
     } else if (threadIdx.x < 64) {
         ShortStep::run<T>(g, a, r, row, q, temperature, uniform, states, tokens, logprob, append, lds.s);
@@ -1090,7 +1100,9 @@ __device__ inline Written written(const int32_t* begin, const int32_t* len, uint
 
 // Sixteen rows a block, a wave each: first the bytes of every row's text and of the block's, then, each block adding the blocks before
 // it up, where a row begins, and its text.  (Rows beyond LINES_DIRECT are added up by the scan of the caption offsets instead.)
-// A wave holds LINE_AHEAD times 64 tokens at once, so that 256 tokens cost three rounds of memory latency: the tokens, where their texts stand, the texts.
+// A wave holds LINE_AHEAD times 64 tokens at once, so that 256 tokens cost two rounds of memory latency: the tokens, and their texts, which stand beside
+// their sizes in 16 bytes up to a length of 15.  Bound by the gathers (64 cache lines a wave's load) and by LDS: 8192 rows of up to 300 tokens (7 MB of
+// tokens, 13 of text: 4.5 us at a copy's rate) take 10 us for the sizes and 17 for the texts.
 constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, LINE_AHEAD = 4, SIZE_AHEAD = 8;
 constexpr uint64_t LINES_DIRECT = 65536;
 

@@ -43,20 +43,22 @@ def _stream(torch, device):
 
 
 def _refuse(name, t, device, dtype, shape):
+    if t.requires_grad and _torch_module.is_grad_enabled():
+        raise ValueError("%s requires a gradient, which this call does not have: detach it" % name)
     raise ValueError("%s must be a %s tensor of the shape %s on cuda:%d, dense along its last axis, got %s %s with strides %s on %s" % (
         name, dtype, shape, device, t.dtype, tuple(t.shape), t.stride(), t.device))
 
 
 def _vec(name, t, device, dtype, rows):
     """A dense vector's data pointer."""
-    if t.dtype is not dtype or t.get_device() != device or t.shape != (rows,) or not t.is_contiguous():
+    if t.dtype is not dtype or t.get_device() != device or t.shape != (rows,) or not t.is_contiguous() or (t.requires_grad and _torch_module.is_grad_enabled()):
         _refuse(name, t, device, dtype, "(%d,)" % rows)
     return t.data_ptr()
 
 
 def _table(name, t, device, dtype, rows, columns):
     """A table's data pointer, rows, columns and elements between rows (its columns where there is one row at most); rows or columns -1: any."""
-    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2:
+    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2 or (t.requires_grad and _torch_module.is_grad_enabled()):
         _refuse(name, t, device, dtype, "(%d, %d)" % (rows, columns))
     r, c = t.shape
     stride, dense = t.stride()
@@ -111,12 +113,10 @@ def logit_rules(device, type_, rows, vocab, logits, stride, *, history=None, his
 
 def _with_logits(device, logits, rules):
     """(packed tp_logits, rows, vocab)"""
-    torch = _torch()
+    _torch()
     dtype = logits.dtype
     if dtype not in _TYPES:
         raise ValueError("logits must be a float32, float16 or bfloat16 tensor [rows, vocab], got %s" % dtype)
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise ValueError("logits require a gradient, which this call does not have: detach them")
     p, rows, vocab, stride = _table("logits", logits, device, dtype, -1, -1)
     return logit_rules(device, _TYPES[dtype], rows, vocab, p, stride, **rules), rows, vocab
 
@@ -138,6 +138,7 @@ def shape_logits(pipe, logits, out, rules):
         to, stride = out.data_ptr(), vocab
     else:
         to, _, _, stride = _table("out", out, device, logits.dtype, rows, vocab)
+        _torch().autograd.graph.increment_version(out)           # a backward pass that has kept what `out` held finds it changed
     pipe._check(pipe._L.tp_shape_logits(pipe._h, io, to, stride))
     return out
 
@@ -265,11 +266,20 @@ class TagGrammar:
         return arena, offsets
 
 
+# An arena for rows of nothing but the longest token is made up to this many bytes; beyond it (a token list may hold a token of a hundred
+# spaces) the texts' sizes are found first, at the price of doing the work twice.
+MOST_ARENA = 1 << 30
+
+
 def run_tokens(pipe, grammar, tokens, lengths, begin):
     torch = _torch()
     if grammar.device != pipe._device:
         raise ValueError("the grammar is on another device than the context")
-    arena, offsets = grammar.lines(tokens, lengths, begin)
+    arena = None
+    if tokens.numel() * grammar.info.longest_token > MOST_ARENA:
+        _, offsets = grammar.lines(tokens, lengths, begin, arena=tokens.new_empty((0,), dtype=torch.uint8))
+        arena = tokens.new_empty((int(offsets[-1]) + 16,), dtype=torch.uint8)
+    arena, offsets = grammar.lines(tokens, lengths, begin, arena)
     rows, info, device = tokens.shape[0], pipe.info, tokens.device
 
     def zeros(n, dtype):

@@ -503,8 +503,8 @@ int tp_format_review_rows(const tp_ctx* ctx, const tp_result* res, int format, c
  *
  * Conventions.  Every pointer in these structs and argument lists is a device pointer on the context's device unless
  * it is said to be host memory.  Work is enqueued on `stream` (a hipStream_t, NULL = default stream); no call
- * allocates, copies to the host or waits, so all but tp_grammar_create may be captured into a HIP graph.  The caller's current
- * device is left as it was.  A workspace holds nothing between calls and needs no initial contents, but calls that may
+ * allocates, copies to the host or waits, so all but tp_grammar_create may be captured into a HIP graph.  The caller's
+ * current device is left as it was.  Equal arguments give equal bits, call after call.  A workspace holds nothing between calls and needs no initial contents, but calls that may
  * overlap (two streams, two graphs replayed at once) need one each.  Outputs must not overlap inputs except where a
  * call says so.  Zero rows: nothing is done.  A grammar does not refer to the context it was made from.
  */
@@ -554,9 +554,9 @@ int tp_shape_logits(tp_ctx* ctx, const tp_logits* io, void* out, uint64_t out_st
 /*
  * The token of every row.  z = x / temperature[r] where temperature[r] > 0, else z = x.  Without a temperature (NULL
  * array, 0, negative, NaN) the token is the largest x, ties to the lowest token.  With one it is the lowest token whose
- * cumulative weight exceeds uniform[r] * (the sum of all weights), weights exp(z - max z) in token order, summed in 64
- * bits (a thousand neighbours at a time in 32); uniform[r] in [0, 1), NULL: as temperature NULL.  Values of uniform outside [0, 1) give the first or last token of a weight above 0.
- * A z of NaN counts as -infinity.  Where +infinity stands, the tokens that have it share the weight.
+ * cumulative weight exceeds uniform[r] * (the sum of all weights), weights exp(z - max z) in token order; uniform[r] in
+ * [0, 1), NULL: as temperature NULL.  Values of uniform outside [0, 1) give the first or last token of a weight above 0.
+ * Weights are 32-bit numbers, summed 1024 neighbours at a time in 32 bits and in 64 from there on.  A z of NaN counts as -infinity.  Where +infinity stands, the tokens that have it share the weight.
  * logprob[r] = z - max z - ln(sum of weights) of the chosen token.  A row without a z above -infinity gets token -1 and
  * log-probability -infinity.  logprob may be NULL.  workspace: tp_choose_workspace bytes (host function), aligned to 16.
  */
@@ -568,12 +568,13 @@ int tp_choose_tokens(tp_ctx* ctx, const tp_logits* io, const float* temperature,
  * The grammar of a tag line over a model's token list:  tag ", " tag ", " ... tag <end>,  between min_tags and max_tags
  * tags.  A tag is one the pipeline keeps: with a vocabulary file a member of it that ShouldDropTag lets pass
  * (Program.cs:1121-1133), without one any such string of the context's tables; or one of the caller's own `tags`.
- * Tags may repeat (tp_logits' penalties are there for that).  A token may be any piece of text; one that holds two commas is never allowed.
+ * Tags may repeat (tp_logits' penalties are there for that).  A token may be any piece of text; one that holds two
+ * commas is never allowed.
  * Refused (TP_E_CONFIG): no tags; a token list without a token of its own for every single byte that the lines use,
  * because a line could then come to a place with no way on.  All pointers are host memory and are not kept.
  *
- * A row's state is two int32: the place its text has come to, and how many tags it has finished (commas written).  Places: k = the
- * k-th of the sorted distinct prefixes of the tags (bytes, ascending; 0 = the empty one, where a line and every tag
+ * A row's state is two int32: the place its text has come to, and how many tags it has finished (commas written).
+ * Places: k = the k-th of the sorted distinct prefixes of the tags (bytes, ascending; 0 = the empty one, where a line and every tag
  * begins); n_prefixes = behind a tag's comma; n_prefixes + 1 = the end is written.  {0, 0} starts a line.  Nothing is
  * allowed behind the end or in a place outside [0, n_prefixes + 1].
  */
@@ -606,21 +607,22 @@ int tp_grammar_get_info(const tp_grammar* g, tp_grammar_info* out);
 int tp_grammar_mask(const tp_grammar* g, const int32_t* states, uint64_t rows, uint32_t* mask, uint64_t mask_stride, void* stream);
 
 /*
- * tp_choose_tokens with the grammar's tokens of every row's state as the mask (io's mask must be NULL; io->vocab must be n_tokens), then the
- * state moves on and, with append = 1, the token goes to the end of the row's history and history_len is raised (both must then be
- * given; a row whose history is full gets no token).  A row without a token (-1: its line is at the end, or no allowed token has an
- * x above -infinity) keeps its state and its history.  io->logits NULL: `tokens` is an input, the caller's own choice; a token that the
- * grammar does not allow there moves the row to place -1, token -1 does nothing; logprob is not written.
+ * tp_choose_tokens with the grammar's tokens of every row's state as the mask (io's mask must be NULL; io->vocab must be
+ * n_tokens), all sums in 64 bits, then the state moves on and, with append = 1, the token goes to the end of the row's
+ * history and history_len is raised (both must then be given; a row whose history is full gets no token).  A row without
+ * a token (-1: its line is at the end, or no allowed token has an x above -infinity) keeps its state and its history.
+ * io->logits NULL: `tokens` is an input, the caller's own choice; a token that the grammar does not allow there moves the
+ * row to place -1, token -1 does nothing; logprob is not written.
  */
 int tp_grammar_step(const tp_grammar* g, const tp_logits* io, const float* temperature, const float* uniform, int32_t* states,
                     int32_t* tokens, float* logprob, int append);
 
 /*
  * The texts of rows of tokens, back to back: row r's is arena[offsets[r] .. offsets[r + 1]).  Row r's tokens are
- * tokens[r * stride + k], from begin[r] (NULL: 0) to below len[r] (NULL: width; both taken as 0 below 0 and as width above it); one outside
- * [0, n_tokens) has no text.  A row's text must stay below 4 GiB.  Nothing is written at or behind `capacity`: offsets[rows] is the size needed, and a caller that
- * cannot bound it compares the two.  16 zero bytes behind the last text are written where they fit, so that the arena can go to
- * tp_run_lines_device as it is.  workspace: tp_lines_workspace bytes (host function), aligned to 16.
+ * tokens[r * stride + k], from begin[r] (NULL: 0) to below len[r] (NULL: width; both taken as 0 below 0 and as width
+ * above it); one outside [0, n_tokens) has no text.  A row's text must stay below 4 GiB.  Nothing is written at or behind
+ * `capacity`: offsets[rows] is the size needed, and a caller that cannot bound it compares the two.  16 zero bytes behind
+ * the last text are written where they fit, so that the arena can go to tp_run_lines_device as it is.  workspace: tp_lines_workspace bytes (host function), aligned to 16.
  */
 uint64_t tp_lines_workspace(uint64_t rows);
 int tp_grammar_lines(const tp_grammar* g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t rows,

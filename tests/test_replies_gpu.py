@@ -170,9 +170,9 @@ def test_masked_places_may_hold_anything(pipe, name):
 
 
 def check_choice(token, logprob, xs, sizes, temperature, uniform):
-    """The token against the 64-bit distribution.  z = x / T is off by e = (5 + 1) half steps of the largest intermediate over T.  A weight is 2^((x - m) * k): the
-    difference, the product and k (log2 e and its quotient by T: two) are off by four half steps relative, which moves the weight by 4 half steps times |ln w|;
-    the power itself is off by one step (two half steps), and a sum of 1024 weights in 32 bits by its ten levels.  u * sum may fall on the other side of
+    """The token against the 64-bit distribution.  z = x / T is off by e = (5 + 1) half steps of the largest intermediate over T.  A weight is 2^(x * k - c): the
+    fused product and k (log2 e and its quotient by T: two) are off by three half steps relative, which moves the weight by 3 half steps times |ln w|, taken as 4;
+    the power itself is off by one step (two half steps), and a sum of 1024 weights in 32 bits by its ten levels (repeated tokens' eleventh is within the fourth).  u * sum may fall on the other side of
     a border by that share of the sum."""
     for r, x in enumerate(xs):
         t = float(temperature[r]) if temperature is not None and uniform is not None and temperature[r] > 0 else 0.0
@@ -274,6 +274,66 @@ def test_choose_ties_and_specials(pipe, vocab):
     flat = torch.zeros(4, vocab, device="cuda")
     token, _ = pipe.choose_tokens(flat, temperature=torch.ones(4, device="cuda"), uniform=u)
     assert token.tolist() == [0, 0, int(0.5 * vocab), vocab - 1]        # cumulative weights k + 1 > u * vocab: exact in 64 bits
+
+
+@pytest.mark.parametrize("name", sorted(TYPES))
+def test_signalling_nans(pipe, name):
+    """NaNs of either kind among the logits, in every position of a lane's eight, hide no larger number beside them."""
+    bits = {"f32": (torch.int32, [0x7F800001, -0x7FFFFF, 0x7FC00000]), "f16": (torch.int16, [0x7C01, -0x3FF, 0x7E00]), "bf16": (torch.int16, [0x7F81, -0x7F, 0x7FC0])}[name]
+    rows, vocab = 64, 3001
+    rng = np.random.default_rng(77)
+    logits, l = make_logits(rng, rows, vocab, TYPES[name])
+    at = rng.random((rows, vocab)) < 0.4
+    raw = logits.view(bits[0])
+    raw[dev(at)] = dev(rng.choice(bits[1], size=int(at.sum())), bits[0])
+    l[at] = np.nan
+    token, logprob = pipe.choose_tokens(logits)
+    assert token.tolist() == np.nanargmax(l, axis=1).tolist()
+    temperature, uniform = choice_numbers(rng, rows)
+    token, logprob = pipe.choose_tokens(logits, temperature=dev(temperature), uniform=dev(uniform))
+    check_choice(token.cpu().numpy(), logprob.cpu().numpy(), [np.where(at[r], -np.inf, l[r]) for r in range(rows)], [np.abs(np.nan_to_num(l[r])) for r in range(rows)], temperature, uniform)
+    shaped = pipe.shape_logits(logits).double().cpu().numpy()
+    assert np.array_equal(np.isnan(shaped), at) and np.array_equal(shaped[~at], l[~at])
+
+
+@pytest.mark.parametrize("rows,vocab,history", [(65537, 12, 3), (2 ** 21 + 3, 1, 1), (70001, 40, 0)])
+def test_more_rows_than_a_launch_takes(pipe, rows, vocab, history):
+    """Integers a 16-bit float holds: every value and every choice of the largest is exact."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    logits = torch.randint(-60, 60, (rows, vocab), generator=gen, device="cuda").to(torch.float16)
+    rules, want = {}, logits.double()
+    if history:
+        h = torch.randint(0, vocab, (rows, history), generator=gen, device="cuda", dtype=torch.int32)
+        rules = dict(history=h, presence=torch.full((rows,), 2.0, device="cuda"), frequency=torch.full((rows,), 3.0, device="cuda"))
+        count = torch.zeros(rows, vocab, device="cuda", dtype=torch.float64).scatter_add_(1, h.long(), torch.ones(rows, history, device="cuda", dtype=torch.float64))
+        want = want - 3 * count - 2 * (count > 0)
+    bits = torch.randint(-2 ** 31, 2 ** 31 - 1, (5, (vocab + 31) // 32), generator=gen, device="cuda").to(torch.int32)
+    pick = torch.arange(rows, device="cuda", dtype=torch.int32) % 5
+    rules.update(mask=bits, mask_row=pick)
+    allowed = (bits[pick.long()][:, torch.arange(vocab, device="cuda") // 32] >> (torch.arange(vocab, device="cuda", dtype=torch.int32) % 32)) & 1
+    want = torch.where(allowed > 0, want, -math.inf)
+    assert torch.equal(pipe.shape_logits(logits, **rules).double(), want)
+    token, _ = pipe.choose_tokens(logits, **rules)
+    best = want.max(1).values
+    first = torch.where(want == best[:, None], torch.arange(vocab, device="cuda"), vocab).min(1).values
+    assert torch.equal(token.long(), torch.where(best > -math.inf, first, -1))
+
+
+def test_the_largest_vocabulary(pipe):
+    """2^24 tokens, and an odd million: windows, segments and history tables of a row's last tokens."""
+    rng = np.random.default_rng(78)
+    for vocab in (2 ** 24, 1200003):
+        logits, l = make_logits(rng, 2, vocab, torch.bfloat16, scale=1.0)
+        rules = Rules(rng, 2, vocab, history=300, bias=1, mask=2)
+        rules.history[:, :3] = [vocab - 1, vocab - 2, vocab - 1025]
+        rules.mask[:, -40:], rules.mask_row[:] = -1, 0
+        rules.args.update(history=dev(rules.history), mask=dev(rules.mask), mask_row=dev(rules.mask_row))
+        check_shaped(pipe.shape_logits(logits, **rules.args), l, rules, torch.bfloat16)
+        xs, sizes, _ = zip(*(rules.plain(l[r], r) for r in range(2)))
+        temperature, uniform = np.float32([1, 0.8]), np.float32([0.9999999, 0.3])
+        for tu in (dict(temperature=dev(temperature), uniform=dev(uniform)), dict()):
+            token, logprob = pipe.choose_tokens(logits, **tu, **rules.args)
+            check_choice(token.cpu().numpy(), logprob.cpu().numpy(), xs, sizes, temperature if tu else None, uniform if tu else None)
 
 
 def test_rows_beyond_32_bit_offsets(pipe):
@@ -440,6 +500,34 @@ def test_step_is_choose_under_the_grammars_mask(pipe, wide_grammar):
         other, logprob2 = pipe.choose_tokens(logits, temperature=tu[0], uniform=tu[1], mask=mask, mask_row=torch.arange(rows, device="cuda", dtype=torch.int32), **rules.args)
         assert torch.equal(token, other)
         assert torch.allclose(logprob[token >= 0], logprob2[token >= 0], rtol=1e-6, atol=1e-6) and torch.equal(logprob[token < 0], logprob2[token < 0])
+
+
+def test_grammar_on_more_rows_than_a_launch_takes(pipe):
+    tokens = [b"a", b"b", b",", b" ", b"ab", b"", b"b, "]
+    g, plain = pipe.tag_grammar(tokens, 5, tags=["ab", "aba"], min_tags=2), PlainGrammar(["ab", "aba"], tokens, 5, min_tags=2)
+    rows = 2 ** 21 + 70003
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    kinds = every_state(plain)
+    which = torch.randint(0, len(kinds), (rows,), generator=gen, device="cuda")
+    states = dev(kinds)[which]
+    logits = torch.randn(rows, 7, generator=gen, device="cuda")
+    mask = g.mask(states)
+    want = dev(np.array([np.packbits(plain.allowed((int(a), int(b))), bitorder="little")[0] for a, b in kinds], np.int32))[which]
+    assert torch.equal(mask[:, 0], want)
+    allowed = (want[:, None] >> torch.arange(7, device="cuda", dtype=torch.int32)) & 1
+    x = torch.where(allowed > 0, logits, -math.inf)
+    token, _ = g.step(states, logits)
+    best = x.max(1)
+    assert torch.equal(token.long(), torch.where(best.values > -math.inf, best.indices, -1))
+    to = {(k, t): plain.go((int(s[0]), int(s[1])), t) for k, s in enumerate(kinds) for t in range(7) if plain.allowed((int(s[0]), int(s[1])))[t]}
+    table = np.repeat(kinds[:, None, :], 8, axis=1)                        # [.., 7]: no token, the state stays
+    for (k, t), s in to.items():
+        table[k, t] = s
+    went = dev(table)[which, torch.where(token < 0, 7, token.long())]
+    assert torch.equal(states, went)
+    again = dev(kinds)[which]
+    g.advance(again, token)
+    assert torch.equal(again, went)
 
 
 def test_grammar_advance(pipe):
@@ -632,6 +720,36 @@ def test_a_captured_loop_replays(pipe):
             assert torch.equal(a, b)
         n = int(want[-1][-1])
         assert torch.equal(held_arena[:n], arena[:n])
+
+
+def test_run_tokens_finds_the_sizes_first_where_the_bound_is_large(pipe, monkeypatch):
+    from imagecaptioner_amd import replies
+    g, plain, tokens = small_grammar(pipe, max_tags=12)
+    history, length, prompt, _ = write_replies(pipe, g, plain, np.random.default_rng(36), 40, 60)
+    want = pipe.run_tokens(g, history, length, begin=prompt)
+    monkeypatch.setattr(replies, "MOST_ARENA", 100)
+    got = pipe.run_tokens(g, history, length, begin=prompt)
+    assert np.array_equal(want.captions, got.captions) and np.array_equal(want.caption_offsets, got.caption_offsets)
+    assert pipe.run_tokens(g, history[:0], length[:0]).n_files == 0
+
+
+def test_gradients_are_refused_or_reported(pipe):
+    """What is given requires no gradient, and a backward pass whose kept values are shaped in place says so."""
+    x = torch.randn(2, 50, device="cuda")
+    one = torch.ones(2, device="cuda")
+    for rules in (dict(bias=torch.zeros(50, device="cuda", requires_grad=True)), dict(repetition=one.clone().requires_grad_(), history=torch.zeros(2, 3, device="cuda", dtype=torch.int32)),
+                  dict(out=torch.zeros(2, 50, device="cuda", requires_grad=True))):
+        with pytest.raises(ValueError, match="gradient"):
+            pipe.shape_logits(x, **rules)
+        with torch.no_grad():
+            pipe.shape_logits(x, **rules)
+    with pytest.raises(ValueError, match="gradient"):
+        pipe.choose_tokens(x, temperature=one.clone().requires_grad_(), uniform=one)
+    leaf = x.clone().requires_grad_()
+    kept = leaf.exp()                                                      # its backward pass multiplies by what it holds
+    pipe.shape_logits(kept.detach(), out=kept.detach(), bias=torch.ones(50, device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.sum().backward()
 
 
 def test_two_streams_at_once(pipe):
