@@ -184,26 +184,24 @@ __device__ inline double wave_scan(double v) {
 __device__ inline double wave_sum(double v) { return read_lane(wave_scan(v), 63); }
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------
-// A token's weight is 2^(x * k - c), k = log2(e) / T rounded once for the row and c = best * k rounded once for the tokens that are summed
-// together: one fused multiply-add and one power.  c is no more than a common scale, known exactly to whoever joins sums of
-// different c, so that a weight is off by the rounding of k and of the fma's one result, each half a step relative in the exponent.
-// k stays a normal number, so that neither 0 * k nor -infinity * k is a NaN.  Where c overflows, neighbouring numbers already lie so far apart that only
-// the largest x weighs anything.
-__device__ inline float weight_scale(float t) {
-    return t > 0.0f ? fminf(fmaxf(1.44269504088896341f / t, 1.17549435e-38f), 3.40282347e38f) : 1.44269504088896341f;
-}
+// z = x / T is rounded to 32 bits, as the formula says, by the quotient's own rounding: with 131072 tokens a border between two of them lies in every
+// hundred-thousandth of the weight, and unrounded quotients chose another token than the rounded ones in one row of 700.
+// A token's weight is 2^(z * LOG2E - c), c = best * LOG2E rounded once for the tokens that are summed together: one fused multiply-add and one power.  c is no
+// more than a common scale, known exactly to whoever joins sums of different c, so that a weight is off by LOG2E's rounding and the fma's, each half a step
+// relative in the exponent, and by the power's own step.  Where c overflows, neighbouring numbers already lie so far apart that only the largest z weighs anything.
+constexpr float LOG2E = 1.44269504088896341f;
 struct Scale {
-    float k, c, best;
+    float c, best;
     bool equal;                   // weigh by equality with the largest
-    __device__ Scale(float best_, float k_) : k(k_), c(best_ * k_), best(best_), equal(!(fabsf(best_ * k_) < __builtin_inff())) {}
-    __device__ float weight(float x) const { return equal ? (x == best ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(__builtin_fmaf(x, k, -c)); }
-    // what a sum of the weights of another scale (of the same k) counts for in this one's
-    __device__ double of(float other_best) const { return equal || !(other_best > NEG_INF) ? (other_best == best ? 1.0 : 0.0) : (double)__builtin_amdgcn_exp2f(other_best * k - c); }
+    __device__ Scale(float best_) : c(best_ * LOG2E), best(best_), equal(!(fabsf(best_ * LOG2E) < __builtin_inff())) {}
+    __device__ float weight(float z) const { return equal ? (z == best ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(__builtin_fmaf(z, LOG2E, -c)); }
+    // what a sum of the weights of another scale counts for in this one's
+    __device__ double of(float other_best) const { return equal || !(other_best > NEG_INF) ? (other_best == best ? 1.0 : 0.0) : (double)__builtin_amdgcn_exp2f(other_best * LOG2E - c); }
     // ln of the weight's share of `sum`: of the weight as it was summed, so that a token that is alone has 0 exactly; of its exponent where that is
     // next to nothing
-    __device__ float log_share(float x, double sum) const {
-        const float w = weight(x);
-        return (float)(w > 1e-30f ? log((double)w / sum) : ((double)x * (double)k - (double)c) * 0.69314718055994531 - log(sum));
+    __device__ float log_share(float z, double sum) const {
+        const float w = weight(z);
+        return (float)(w > 1e-30f ? log((double)w / sum) : ((double)z * (double)LOG2E - (double)c) * 0.69314718055994531 - log(sum));
     }
 };
 __device__ inline float temperature_of(const float* temperature, const float* uniform, uint64_t row) {
@@ -212,6 +210,14 @@ __device__ inline float temperature_of(const float* temperature, const float* un
 }
 // a NaN counts as -infinity in a choice
 __device__ inline float countable(float x) { return x == x ? x : NEG_INF; }
+// the z of the weights, never a NaN; temper: the temperature, 1 where the largest is chosen
+__device__ inline float z_of(float x, float temper) { return countable(x / temper); }
+// x of at least `low`; the builtins would first make an ordinary number of every operand
+__device__ inline float at_least(float x, float low) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(low));
+    return r;
+}
 __device__ inline float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -445,7 +451,7 @@ __global__ __launch_bounds__(SHAPE_WAVES * 64) __attribute__((amdgpu_waves_per_e
 // ---- repeated tokens of a window ------------------------------------------------------------------------------------------------
 // For the choice, which the vector units bound: the tokens of the history inside a window of a row are marked in a bitmap, a prefix sum over
 // its words ranks them, and the distinct ones' counts are taken in an array as long as the history has room for.  One
-// thread per distinct token then works its x out, with a load of the token's own logit, and puts it in the count's place.  The
+// thread per distinct token then works its z out, with a load of the token's own logit, and puts it in the count's place.  The
 // vectors leave these tokens out: the penalties' arithmetic, a division among it, is done once per repeated token instead
 // of once per token of the row.  The first segment's loads are in flight meanwhile.
 template <int WAVES, int SEGS>
@@ -459,14 +465,14 @@ struct Window {
         uint32_t rank[WORDS + 1];                                             // distinct tokens before the word
         uint32_t wave[WAVES];
     };
-    // `value`, in dynamic LDS: the distinct tokens' x, in token order; as many words as the history has entries, or the window tokens
+    // `value`, in dynamic LDS: the distinct tokens' z, in token order; as many words as the history has entries, or the window tokens
 
     static __device__ uint32_t tid() { return threadIdx.x % THREADS; }
     static __device__ uint32_t rank_of(const Lds& l, uint32_t t) { return l.rank[t >> 5] + (uint32_t)__popc(l.seen[t >> 5] & ((1u << (t & 31)) - 1)); }
 
-    // How many distinct tokens of the window of `inside` tokens from w0 the history has; their x stand in `value`.
+    // How many distinct tokens of the window of `inside` tokens from w0 the history has; their z stand in `value`.
     template <class T, class H>
-    static __device__ uint32_t repeated(const RowRules& r, const H& history, Glob<typename T::S> row, uint32_t w0, uint32_t inside, Lds& l, uint32_t* value) {
+    static __device__ uint32_t repeated(const RowRules& r, float temper, const H& history, Glob<typename T::S> row, uint32_t w0, uint32_t inside, Lds& l, uint32_t* value) {
         if (!r.len) return 0;
         const uint32_t words = (inside + SEGMENT - 1) / SEGMENT * (SEGMENT / 32);      // the bitmap's, in whole segments
         for (uint32_t k = tid(); k < words; k += THREADS) l.seen[k] = l.claimed[k] = 0;
@@ -517,7 +523,7 @@ struct Window {
             float x = penalised(T::up(logit), value[i], r);
             if (r.bias) x = x + b;
             if (r.mask && !(r.mask[(w0 + t) >> 3] >> (t & 7) & 1)) x = NEG_INF;
-            value[i] = __builtin_bit_cast(uint32_t, x);
+            value[i] = __builtin_bit_cast(uint32_t, z_of(x, temper));
         });
         block_sync<THREADS>();
         return distinct;
@@ -538,14 +544,11 @@ using OneSegment = Window<1, 1>;
 constexpr int CHOICE_WAVES = 16, MOST_SEGS = 8;                               // waves of a block, segments of a wave at the most
 using Chunk = Window<CHOICE_WAVES, MOST_SEGS>;
 
-// Its weights are taken against `ref`, what the wave's segment before was taken against, and only where they outgrow it, or there is none, against
-// the segment's own largest x, which is `ref` from then on: the shares that the join works with do not mind what they are
-// relative to, and the largest need not be found.  With `greedy` it is the segment's largest in any case.
-template <class T, bool TINY, class Next>
-__device__ inline ChoicePart segment_part(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, float k, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
-                                          const uint32_t* value, Next&& next) {
-    float x[VECS][8];
-    uint32_t take[VECS], i0 = 0, i1 = 0;
+// x of a segment without its repeated tokens, which are value[i0 .. i1)
+template <class T, bool TINY>
+__device__ inline void segment_x(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, uint32_t distinct, const Chunk::Lds& l, float (&x)[VECS][8], uint32_t& i0, uint32_t& i1) {
+    uint32_t take[VECS];
+    i0 = i1 = 0;
 #pragma unroll
     for (int v = 0; v < VECS; ++v) take[v] = h.take[v];
     if (distinct) {
@@ -562,45 +565,64 @@ __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t n, uint32_
 #pragma unroll
     for (int v = 0; v < VECS; ++v) T::up8(h.d[v], x[v]);
     finish_segment<T, TINY>(r, n, g, h, take, x);
+}
+// the largest z; a NaN among the x may hide others, or be passed over
+__device__ inline float segment_largest(const float (&x)[VECS][8], float temper, const uint32_t* value, uint32_t i0, uint32_t i1) {
+    float best = NEG_INF;
+#pragma unroll
+    for (int v = 0; v < VECS; ++v)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) best = max3(best, x[v][j], x[v][j + 1]);
+    best = z_of(best, temper);                                                      // the quotients are in the order of the x
+    for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) best = fmaxf(best, __builtin_bit_cast(float, value[i]));
+    return wave_max(best);
+}
+
+// The sum of a segment's weights.  They are taken against `ref`, and only where they outgrow it, or there is none, against
+// the segment's own largest z, which is the wave's `ref` from then on: the shares that the join works with do not mind what they are
+// relative to, and the largest need not be found.  With `greedy` it is the segment's largest in any case.
+// A quotient x / T of the vectors is x * (1 / T), corrected by its exact remainder; what that cannot do (infinities, temperatures whose inverse is none) becomes
+// a NaN, and the segment is done again by divisions.  The x far below `ref`, -infinity among them, are lifted to where a weight is still 0.
+template <class T, bool TINY, class Next>
+__device__ inline ChoicePart segment_part(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, float temper, float inverse, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
+                                          const uint32_t* value, Next&& next) {
+    float x[VECS][8];
+    uint32_t i0, i1;
+    segment_x<T, TINY>(r, n, g, h, distinct, l, x, i0, i1);
     next();                                                                   // `h` is free for the loads of the wave's next segment
-    auto largest = [&]() {
-        float best = NEG_INF;
-#pragma unroll
-        for (int v = 0; v < VECS; ++v)
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) best = max3(best, x[v][j], x[v][j + 1]);
-        for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) best = fmaxf(best, countable(__builtin_bit_cast(float, value[i])));
-        return wave_max(best);
-    };
-    auto weights = [&](const Scale& scale) {
-        float sum = 0.0f;
-        if (!scale.equal) {
-#pragma unroll
-            for (int v = 0; v < VECS; ++v) {
-                float w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[v][j], k, -scale.c));
-                sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-            }
-        } else {
-#pragma unroll
-            for (int v = 0; v < VECS; ++v)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum += scale.weight(x[v][j]);
-        }
+    auto repeated = [&](const Scale& scale) {
         double more = 0.0;                                                    // up to sixteen, one after another
-        for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) more += (double)scale.weight(countable(__builtin_bit_cast(float, value[i])));
-        return wave_sum(i1 > i0 ? (float)((double)sum + more) : sum);
+        for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) more += (double)scale.weight(__builtin_bit_cast(float, value[i]));
+        return more;
     };
-    if (greedy || ref == NEG_INF) ref = largest();
-    float sum = weights(Scale(ref, k));
-    if (!(sum < 1e30f) || Scale(ref, k).equal) {                              // outgrown, or a NaN among the logits, or no scale to go by
+    if (greedy || ref == NEG_INF) ref = segment_largest(x, temper, value, i0, i1);
+    Scale scale(ref);
+    float sum = 0.0f;
+    const float low = (ref - 200.0f - fabsf(ref) * 0x1p-10f) * temper;
+#pragma unroll
+    for (int v = 0; v < VECS; ++v) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float y = at_least(x[v][j], low), q = y * inverse;
+            w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(-q, temper, y), inverse, q), LOG2E, -scale.c));
+        }
+        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    }
+    sum = wave_sum(i1 > i0 ? (float)((double)sum + repeated(scale)) : sum);
+    if (!(sum < 1e30f) || scale.equal) {                                      // outgrown, or a NaN, or no scale to go by
 #pragma unroll
         for (int v = 0; v < VECS; ++v)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[v][j] = countable(x[v][j]);
-        ref = largest();
-        sum = ref == NEG_INF ? 0.0f : weights(Scale(ref, k));
+            for (int j = 0; j < 8; ++j) x[v][j] = z_of(x[v][j], temper);
+        ref = segment_largest(x, 1.0f, value, i0, i1);
+        scale = Scale(ref);
+        sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < VECS; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += scale.weight(x[v][j]);
+        sum = ref == NEG_INF ? 0.0f : wave_sum((float)((double)sum + repeated(scale)));
     }
     return ChoicePart{ref, sum};
 }
@@ -622,13 +644,13 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         }
         return;
     }
-    const float k = weight_scale(t);
-    const Scale scale(best, k);
+    const float temper = t > 0.0f ? t : 1.0f;
+    const Scale scale(best);
     auto share = [&](uint32_t c) { return c < segments ? (double)p[c].sum * scale.of(p[c].best) : 0.0; };
     double sum = 0.0;
     for (uint32_t c = lane; c < segments; c += 64) sum += share(c);
     sum = wave_sum(sum);
-    // Greedy: the first segment that has the largest x.  Sampled: the first whose cumulative share exceeds the target; where there is none (rounding,
+    // Greedy: the first segment that has the largest z.  Sampled: the first whose cumulative share exceeds the target; where there is none (rounding,
     // or a `uniform` of 1 or more) the last of a share above 0, and so within the segment.
     double target = t > 0.0f ? (double)uniform[row] * sum : 0.0, carry = 0.0, before = 0.0;
     uint32_t segment = 0;
@@ -645,7 +667,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         }
         carry = read_lane(incl, 63);
     }
-    const Scale within(p[segment].best, k);
+    const Scale within(p[segment].best);
     target = (target - before) / scale.of(within.best);
     const uint32_t w0 = segment * SEGMENT, n = a.vocab - w0, l0 = HERE ? w0 : 0;             // l0: the segment's start within the tables
     const auto from = logit_row<T>(a, row) + w0;
@@ -656,7 +678,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         History<64, 8> history;
         history.load(r, w0);
         load_segment<T, TINY, false>(r, from, w0, n, 0, h);
-        distinct = OneSegment::repeated<T>(r, history, from, w0, std::min(n, SEGMENT), l, value);
+        distinct = OneSegment::repeated<T>(r, temper, history, from, w0, std::min(n, SEGMENT), l, value);
     }
     uint32_t at = 0;
     float x_at = best;
@@ -671,6 +693,8 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         float (&x)[8] = xs[v];
         const uint32_t t0 = l0 + lane_at(0) + v * 512, cut = cut_of(lane_at(0) + v * 512, n);
         const uint32_t hit = distinct && cut < 8 ? (uint32_t)((const uint8_t*)l.seen)[t0 >> 3] << cut & 0xFFu : 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = z_of(x[j], temper);
         if (hit) {
             uint32_t i = Tables::rank_of(l, t0);
 #pragma unroll
@@ -680,7 +704,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
         double mine = 0.0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            w[j] = within.weight(countable(x[j]));
+            w[j] = within.weight(x[j]);
             mine += (double)w[j];
         }
         const double incl = run + wave_scan(mine);
@@ -723,9 +747,10 @@ __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_
                                                                                                      const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
     __shared__ Chunk::Lds l;
     __shared__ ChoicePart here[CHOICE_WAVES * MOST_SEGS];
+    __shared__ float largest[CHOICE_WAVES];
     const uint64_t row = row0 + blockIdx.y;
     const uint32_t chunks = gridDim.x, window = segs * CHOICE_WAVES * SEGMENT, w0 = blockIdx.x * window, n = a.vocab - w0, segments = reply_segments(a.vocab);
-    const float t = temperature_of(temperature, uniform, row), k = weight_scale(t);
+    const float t = temperature_of(temperature, uniform, row), temper = t > 0.0f ? t : 1.0f, inverse = 1.0f / temper;
     const RowRules r = row_rules(a, row);
     const auto from = logit_row<T>(a, row) + w0;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * CHOICE_WAVES, reply_segments(n));
@@ -733,11 +758,22 @@ __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_
     history.load(r, w0);
     Held<T> h;
     if (wave < last) load_segment<T, TINY, true>(r, from, w0, n, wave, h);
-    const uint32_t distinct = Chunk::repeated<T>(r, history, from, w0, std::min(n, window), l, dynamic_lds);
+    const uint32_t distinct = Chunk::repeated<T>(r, temper, history, from, w0, std::min(n, window), l, dynamic_lds);
     ChoicePart* out = parts + row * segments + w0 / SEGMENT;
     float ref = NEG_INF;
+    if (t > 0.0f) {                                                           // the largest of the waves' first segments, a number near the row's largest: small exponents round less
+        if (wave < last) {
+            float x[VECS][8];
+            uint32_t i0, i1;
+            segment_x<T, TINY>(r, n, wave, h, distinct, l, x, i0, i1);
+            ref = segment_largest(x, temper, dynamic_lds, i0, i1);
+        }
+        if ((threadIdx.x & 63) == 0) largest[wave] = ref;
+        __syncthreads();
+        ref = wave_max(largest[threadIdx.x % CHOICE_WAVES]);
+    }
     for (uint32_t g = wave; g < last; g += CHOICE_WAVES) {
-        const ChoicePart p = segment_part<T, TINY>(r, n, g, h, k, t == 0.0f, ref, distinct, l, dynamic_lds, [&] {
+        const ChoicePart p = segment_part<T, TINY>(r, n, g, h, temper, inverse, t == 0.0f, ref, distinct, l, dynamic_lds, [&] {
             if (g + CHOICE_WAVES < last) load_segment<T, TINY, true>(r, from, w0, n, g + CHOICE_WAVES, h);
         });
         if ((threadIdx.x & 63) == 0) {
@@ -905,9 +941,9 @@ struct Step {
         }
     }
 
-    // x of the m entries from e0: entry i of the piece is thread i % THREADS's number i / THREADS; -infinity where it may not be taken
+    // z of the m entries from e0: entry i of the piece is thread i % THREADS's number i / THREADS; -infinity where it may not be taken
     template <class T>
-    static __device__ void shaped(const DevGrammar& g, const tp_logits& a, const RowRules& r, uint64_t row, uint32_t tags, uint32_t e0, uint32_t m, Lds& s, uint2 (&en)[EACH], float (&x)[EACH]) {
+    static __device__ void shaped(const DevGrammar& g, const tp_logits& a, const RowRules& r, float temper, uint64_t row, uint32_t tags, uint32_t e0, uint32_t m, Lds& s, uint2 (&en)[EACH], float (&x)[EACH]) {
         const auto l = logit_row<T>(a, row);
         const auto entries = (Glob<unsigned long long>)(glob((const unsigned long long*)g.entry) + e0);
         const uint32_t tid = threadIdx.x;
@@ -931,7 +967,7 @@ struct Step {
         for (int v = 0; v < EACH; ++v) {
             float y = penalised(T::up(raw[v]), c[v], r);
             if (r.bias) y = y + b[v];
-            x[v] = ok[v] ? countable(y) : NEG_INF;
+            x[v] = ok[v] ? z_of(y, temper) : NEG_INF;
         }
     }
 
@@ -947,8 +983,8 @@ struct Step {
         return v;
     }
     // the segments' sums of the weights against `best`, into LDS
-    static __device__ void segment_sums(const float (&x)[EACH], float best, float k, Lds& s) {
-        const Scale scale(best, k);
+    static __device__ void segment_sums(const float (&x)[EACH], float best, Lds& s) {
+        const Scale scale(best);
 #pragma unroll
         for (int v = 0; v < EACH; ++v) {
             const double w = wave_sum(best > NEG_INF ? (double)scale.weight(x[v]) : 0.0);
@@ -966,23 +1002,23 @@ struct Step {
     template <class T>
     static __device__ void run(const DevGrammar& g, const tp_logits& a, const RowRules& r, uint64_t row, const List& q, const float* temperature, const float* uniform, int32_t* states,
                                int32_t* tokens, float* logprob, int append, Lds& s) {
-        const float t = temperature_of(temperature, uniform, row), k = weight_scale(t);
+        const float t = temperature_of(temperature, uniform, row), temper = t > 0.0f ? t : 1.0f;
         const bool one = q.hi - q.lo <= PIECE, room = has_room(a, row, append);
         const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
         uint2 en[EACH];
         float x[EACH], best = NEG_INF;
         double sum = 0.0;
         for (uint32_t p = q.lo; p < q.hi; p += PIECE) {
-            shaped<T>(g, a, r, row, q.tags, p, q.hi - p < PIECE ? q.hi - p : PIECE, s, en, x);
+            shaped<T>(g, a, r, temper, row, q.tags, p, q.hi - p < PIECE ? q.hi - p : PIECE, s, en, x);
             float pb = NEG_INF;
 #pragma unroll
             for (int v = 0; v < EACH; ++v) pb = fmaxf(pb, x[v]);
             pb = read_lane(block_max(pb, s), 0);
             if (pb > best) {
-                sum = best > NEG_INF ? sum * Scale(pb, k).of(best) : 0.0;
+                sum = best > NEG_INF ? sum * Scale(pb).of(best) : 0.0;
                 best = pb;
             }
-            segment_sums(x, best, k, s);
+            segment_sums(x, best, s);
             sum += piece_sum(s);
             if (!one) block_sync<THREADS>();                                 // before the next piece's sums
         }
@@ -995,14 +1031,14 @@ struct Step {
         }
         // Greedy: the first entry of the largest x.  Sampled: the first whose cumulative weight exceeds the target; where there is none (rounding, or
         // a `uniform` of 1 or more) the last of a weight above 0.
-        const Scale scale(best, k);
+        const Scale scale(best);
         const double target = t > 0.0f ? (double)uniform[row] * sum : 0.0;
         double carry = 0.0;
         bool found = false, mine = false;
         uint2 entry = make_uint2(0, 0);
         float x_at = best;
         for (uint32_t p = q.lo; p < q.hi && !found; p += PIECE) {
-            if (!one) shaped<T>(g, a, r, row, q.tags, p, q.hi - p < PIECE ? q.hi - p : PIECE, s, en, x);
+            if (!one) shaped<T>(g, a, r, temper, row, q.tags, p, q.hi - p < PIECE ? q.hi - p : PIECE, s, en, x);
             if (t == 0.0f) {
                 if (threadIdx.x == 0) s.first = 0xFFFFFFFFu;
                 block_sync<THREADS>();
@@ -1016,7 +1052,7 @@ struct Step {
                 if (!one) block_sync<THREADS>();
                 continue;
             }
-            if (!one) segment_sums(x, best, k, s);
+            if (!one) segment_sums(x, best, s);
             // the piece's segment: every wave finds it
             int at = -1;
             double before = 0.0, in_piece = 0.0;
