@@ -44,10 +44,10 @@ const char* check_lines(const int32_t* tokens, uint64_t stride, uint32_t width, 
                         const void* workspace, uint64_t workspace_bytes);
 
 constexpr uint64_t MAX_REPLY_ROWS = (uint64_t)1 << 31;
-// The choice of a token joins segments of a row: of each the sum of its weights, and the x that they are relative to.
+// The choice of a token joins segments of a row: of each the sum of its weights, and the z that they are relative to.
 constexpr uint32_t REPLY_SEGMENT = 1024;
 constexpr uint32_t reply_segments(uint32_t vocab) { return (vocab + REPLY_SEGMENT - 1) / REPLY_SEGMENT; }
-struct ChoicePart { float best, sum; };
+struct ChoicePart { double sum; float best; };
 uint64_t choose_workspace(uint64_t rows, uint32_t vocab);
 uint64_t lines_workspace(uint64_t rows);
 

@@ -461,7 +461,10 @@ struct Window {
     static constexpr int MINE = (int)((WORDS + THREADS - 1) / THREADS);    // bitmap words of a thread
     struct Lds {
         alignas(16) uint32_t seen[WORDS];
-        uint32_t claimed[WORDS];
+        union {
+            uint32_t claimed[WORDS];
+            alignas(16) float lane_sum[TOKENS / (8 * VECS)];                  // what the choice makes of every lane's tokens, when `claimed` is done with
+        };
         uint32_t rank[WORDS + 1];                                             // distinct tokens before the word
         uint32_t wave[WAVES];
     };
@@ -531,15 +534,15 @@ struct Window {
 };
 
 // ---- the choice -------------------------------------------------------------------------------------------------------------
-// The first launch reads the logits once and leaves of every segment the sum of its weights and the x that they are relative to; a wave does
-// that by itself.  The second joins a row with one wave: the token's segment by a scan of the segments' shares, and the token in that segment, which
-// the wave shapes again (1024 tokens of the row).  A row of one window does both in the first launch.  A segment's sum is a 32-bit sum of 1024
-// weights in a tree of 10 levels (and one rounding more for a lane with repeated tokens), off by 11 half steps at most; the segments are
-// summed in 64 bits, and so is the chosen token's own segment when the join works on it.
+// The first launch reads the logits once and leaves of every segment the sum of its weights and the z that they are relative to.  The second joins a
+// row with one wave: the token's segment by a scan of the segments' shares, and the token in that segment, which
+// the wave shapes again (1024 tokens of the row).  A row of one window does both in the first launch.  A lane's sixteen weights of a segment are summed in
+// 32 bits (five roundings, one more where repeated tokens are among them), everything above in 64.  Against the formula with 64-bit sums, 131072 tokens and temperatures
+// of 0.5 .. 1.2, one row of 5000 got another token, always the border's other side.
 //
-// What bounds it: 512 rows of 131072 bfloat16 (134 MB, 26 us at a copy's rate) with 256 tokens of history and a bias take 40 us: the vector units
-// spend some 250 instructions a segment, most of them in the powers and the sums; the block's start (rules, history and repeated tokens: 6 us) and the join of the
-// row (4 us) are chains of latency that only other blocks hide.  Without rules the launch reads at 5.8 TB/s.
+// What bounds it: 512 rows of 131072 bfloat16 (134 MB, 26 us at a copy's rate) with 256 tokens of history and a bias take 45 us: the vector units
+// spend some 300 instructions a segment, a third of them in the quotients and a quarter in the powers; the block's start (rules, history and repeated tokens: 6 us) and the join of
+// the row (4 us) are chains of latency that no other block hides, since all rows are at work at once.
 using OneSegment = Window<1, 1>;
 constexpr int CHOICE_WAVES = 16, MOST_SEGS = 8;                               // waves of a block, segments of a wave at the most
 using Chunk = Window<CHOICE_WAVES, MOST_SEGS>;
@@ -578,13 +581,13 @@ __device__ inline float segment_largest(const float (&x)[VECS][8], float temper,
     return wave_max(best);
 }
 
-// The sum of a segment's weights.  They are taken against `ref`, and only where they outgrow it, or there is none, against
+// The lane's sum of a segment's weights.  They are taken against `ref`, and only where they outgrow it, or there is none, against
 // the segment's own largest z, which is the wave's `ref` from then on: the shares that the join works with do not mind what they are
 // relative to, and the largest need not be found.  With `greedy` it is the segment's largest in any case.
 // A quotient x / T of the vectors is x * (1 / T), corrected by its exact remainder; what that cannot do (infinities, temperatures whose inverse is none) becomes
 // a NaN, and the segment is done again by divisions.  The x far below `ref`, -infinity among them, are lifted to where a weight is still 0.
 template <class T, bool TINY, class Next>
-__device__ inline ChoicePart segment_part(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, float temper, float inverse, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
+__device__ inline float segment_part(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, float temper, float inverse, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
                                           const uint32_t* value, Next&& next) {
     float x[VECS][8];
     uint32_t i0, i1;
@@ -609,8 +612,8 @@ __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t n, uint32_
         }
         sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     }
-    sum = wave_sum(i1 > i0 ? (float)((double)sum + repeated(scale)) : sum);
-    if (!(sum < 1e30f) || scale.equal) {                                      // outgrown, or a NaN, or no scale to go by
+    if (i1 > i0) sum = (float)((double)sum + repeated(scale));
+    if (__ballot(!(sum < 1e30f)) || scale.equal) {                                      // outgrown, or a NaN, or no scale to go by
 #pragma unroll
         for (int v = 0; v < VECS; ++v)
 #pragma unroll
@@ -622,9 +625,9 @@ __device__ inline ChoicePart segment_part(const RowRules& r, uint32_t n, uint32_
         for (int v = 0; v < VECS; ++v)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum += scale.weight(x[v][j]);
-        sum = ref == NEG_INF ? 0.0f : wave_sum((float)((double)sum + repeated(scale)));
+        sum = ref == NEG_INF ? 0.0f : (float)((double)sum + repeated(scale));
     }
-    return ChoicePart{ref, sum};
+    return sum;
 }
 
 // Joins a row's segments: all lanes of one wave.  Tables: Chunk where the row's own window stands in LDS (`distinct` of it), OneSegment
@@ -646,7 +649,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     }
     const float temper = t > 0.0f ? t : 1.0f;
     const Scale scale(best);
-    auto share = [&](uint32_t c) { return c < segments ? (double)p[c].sum * scale.of(p[c].best) : 0.0; };
+    auto share = [&](uint32_t c) { return c < segments ? p[c].sum * scale.of(p[c].best) : 0.0; };
     double sum = 0.0;
     for (uint32_t c = lane; c < segments; c += 64) sum += share(c);
     sum = wave_sum(sum);
@@ -735,7 +738,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     }
     // The token's own segment is now known to 64 bits: where the token has nearly all the weight, its logarithm is that of a number next to 1, and the
     // segment's sum in 32 bits would have rounded the rest away.
-    sum += (run - (double)p[segment].sum) * scale.of(within.best);
+    sum += (run - p[segment].sum) * scale.of(within.best);
     if (lane == 0) {
         tokens[row] = (int32_t)(w0 + at);
         if (logprob) logprob[row] = scale.log_share(x_at, sum);
@@ -773,11 +776,22 @@ __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_
         ref = wave_max(largest[threadIdx.x % CHOICE_WAVES]);
     }
     for (uint32_t g = wave; g < last; g += CHOICE_WAVES) {
-        const ChoicePart p = segment_part<T, TINY>(r, n, g, h, temper, inverse, t == 0.0f, ref, distinct, l, dynamic_lds, [&] {
+        const float sum = segment_part<T, TINY>(r, n, g, h, temper, inverse, t == 0.0f, ref, distinct, l, dynamic_lds, [&] {
             if (g + CHOICE_WAVES < last) load_segment<T, TINY, true>(r, from, w0, n, g + CHOICE_WAVES, h);
         });
-        if ((threadIdx.x & 63) == 0) {
-            if (chunks > 1) out[g] = p; else here[g] = p;
+        l.lane_sum[g * 64 + (threadIdx.x & 63)] = sum;
+        if ((threadIdx.x & 63) == 0) here[g].best = ref;
+    }
+    __syncthreads();
+    if (threadIdx.x < last * 8) {                                             // eight threads a segment
+        const float4 a0 = *(const float4*)(l.lane_sum + threadIdx.x * 8), a1 = *(const float4*)(l.lane_sum + threadIdx.x * 8 + 4);
+        double sum = (((double)a0.x + a0.y) + ((double)a0.z + a0.w)) + (((double)a1.x + a1.y) + ((double)a1.z + a1.w));
+        sum += dpp<0x111, 0xF>(sum);
+        sum += dpp<0x112, 0xF>(sum);
+        sum += dpp<0x114, 0xF>(sum);
+        if (threadIdx.x % 8 == 7) {
+            const uint32_t g = threadIdx.x / 8;
+            if (chunks > 1) out[g] = ChoicePart{sum, here[g].best}; else here[g].sum = sum;
         }
     }
     if (chunks > 1) return;

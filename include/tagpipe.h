@@ -556,7 +556,7 @@ int tp_shape_logits(tp_ctx* ctx, const tp_logits* io, void* out, uint64_t out_st
  * array, 0, negative, NaN) the token is the largest x, ties to the lowest token.  With one it is the lowest token whose
  * cumulative weight exceeds uniform[r] * (the sum of all weights), weights exp(z - max z) in token order; uniform[r] in
  * [0, 1), NULL: as temperature NULL.  Values of uniform outside [0, 1) give the first or last token of a weight above 0.
- * Weights are 32-bit numbers, summed 1024 neighbours at a time in 32 bits and in 64 from there on.  A z of NaN counts as -infinity.  Where +infinity stands, the tokens that have it share the weight.
+ * z and the weights are 32-bit numbers; the weights are summed 16 at a time in 32 bits and in 64 from there on.  A z of NaN counts as -infinity.  Where +infinity stands, the tokens that have it share the weight.
  * logprob[r] = z - max z - ln(sum of weights) of the chosen token.  A row without a z above -infinity gets token -1 and
  * log-probability -infinity.  logprob may be NULL.  workspace: tp_choose_workspace bytes (host function), aligned to 16.
  */

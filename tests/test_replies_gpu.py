@@ -170,9 +170,9 @@ def test_masked_places_may_hold_anything(pipe, name):
 
 
 def check_choice(token, logprob, xs, sizes, temperature, uniform):
-    """The token against the 64-bit distribution.  z = x / T is off by e = (5 + 1) half steps of the largest intermediate over T.  A weight is 2^(x * k - c): the
-    fused product and k (log2 e and its quotient by T: two) are off by three half steps relative, which moves the weight by 3 half steps times |ln w|, taken as 4;
-    the power itself is off by one step (two half steps), and a sum of 1024 weights in 32 bits by its ten levels (repeated tokens' eleventh is within the fourth).  u * sum may fall on the other side of
+    """The token against the 64-bit distribution.  z = x / T is off by e = (5 + 1) half steps of the largest intermediate over T.  A weight is 2^(z * log2 e - c): log2 e and
+    the fused product are off by two half steps relative, which moves the weight by 2 half steps times |ln w|, taken as 4;
+    the power itself is off by one step (two half steps), and a sum of 1024 weights by six roundings to 32 bits, taken as 10.  u * sum may fall on the other side of
     a border by that share of the sum."""
     for r, x in enumerate(xs):
         t = float(temperature[r]) if temperature is not None and uniform is not None and temperature[r] > 0 else 0.0
