@@ -1888,7 +1888,10 @@ tp_grammar* tp_grammar_create(tp_ctx* ctx, const tp_grammar_config* cfg) {
             bytes[t] = rec[15] = (uint8_t)(n < 16 ? n : LONG_TOKEN);
             std::memcpy(&records[t], rec, 16);
         }
+        std::vector<uint4> quarter((h.info.n_tokens + 31) / 32);
+        for (size_t t = 0; t < bytes.size(); ++t) ((uint8_t*)quarter.data())[t / 2] |= (uint8_t)(std::min<uint8_t>(bytes[t], 15) << (t % 2 * 4));
         g->dev.bytes = upload(g->owned, bytes);
+        g->dev.quarter = upload(g->owned, quarter);
         g->dev.record = upload(g->owned, records);
         h.text.resize(h.text.size() + 8);                                  // k_line_text reads eight bytes at a time
         g->dev.text = upload(g->owned, h.text);

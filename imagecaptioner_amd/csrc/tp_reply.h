@@ -16,6 +16,7 @@ struct DevGrammar {
     const uint32_t* begin;        // HostGrammar::begin
     const uint2* entry;           // per entry: token, move
     const uint8_t* bytes;         // per token: its bytes, or LONG_TOKEN
+    const uint4* quarter;         // per token four bits, 32 tokens an element: its bytes, or 15 for 15 and more
     const uint4* record;          // per token: up to 15 bytes of text and their number in the last byte; of a longer one where it starts in
                                   //   `text`, its bytes, and LONG_TOKEN in the last byte
     const uint8_t* text;          // the tokens' bytes, and eight behind them

@@ -915,47 +915,50 @@ struct Step {
     };
     static __device__ uint32_t slot_of(uint32_t token) { return (token * 0x9E3779B1u) >> (32 - __builtin_ctz(SLOTS)); }
 
-    // count words of the thread's entries
-    static __device__ void recall(const DevGrammar& g, const RowRules& r, const uint2 (&en)[EACH], Lds& s, uint32_t (&c)[EACH]) {
+    // The history's entries [k0, k0 + THREADS * RECALL) as the threads take them.
+    static __device__ void remember(const RowRules& r, uint32_t k0, uint32_t (&token)[RECALL]) {
+#pragma unroll
+        for (int i = 0; i < RECALL; ++i) { const uint32_t k = k0 + i * THREADS + threadIdx.x; token[i] = k < r.len ? (uint32_t)r.history[k] : EMPTY; }
+    }
+    // their table
+    static __device__ void put_down(const DevGrammar& g, const RowRules& r, uint32_t k0, const uint32_t (&token)[RECALL], Lds& s) {
         const uint32_t tid = threadIdx.x;
-        for (uint32_t k0 = 0; k0 < r.len; k0 += THREADS * RECALL) {
-            uint32_t token[RECALL];
 #pragma unroll
-            for (int i = 0; i < RECALL; ++i) { const uint32_t k = k0 + i * THREADS + tid; token[i] = k < r.len ? (uint32_t)r.history[k] : EMPTY; }
-            block_sync<THREADS>();                                           // the part before has been looked up
+        for (uint32_t i = tid * 4; i < SLOTS; i += THREADS * 4) {
+            *(uint4*)(s.key + i) = make_uint4(EMPTY, EMPTY, EMPTY, EMPTY);
+            *(uint4*)(s.cnt + i) = make_uint4(0, 0, 0, 0);
+        }
+        block_sync<THREADS>();
 #pragma unroll
-            for (uint32_t i = tid * 4; i < SLOTS; i += THREADS * 4) {
-                *(uint4*)(s.key + i) = make_uint4(EMPTY, EMPTY, EMPTY, EMPTY);
-                *(uint4*)(s.cnt + i) = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < RECALL; ++i) {
+            if (token[i] >= g.n_tokens) continue;                               // none: EMPTY among them
+            uint32_t h = slot_of(token[i]);
+            for (;; h = (h + 1) & (SLOTS - 1)) {
+                const uint32_t was = atomicCAS(&s.key[h], EMPTY, token[i]);
+                if (was == EMPTY || was == token[i]) break;
             }
-            block_sync<THREADS>();
+            if (k0 + i * THREADS + tid >= r.prompt) atomicAdd(&s.cnt[h], 1u); else atomicOr(&s.cnt[h], SEEN);
+        }
+        block_sync<THREADS>();
+    }
+    // what the table adds to the count words of the thread's entries
+    static __device__ void look_up(const uint2 (&en)[EACH], const Lds& s, uint32_t (&c)[EACH]) {
+        uint32_t found[EACH];
 #pragma unroll
-            for (int i = 0; i < RECALL; ++i) {
-                if (token[i] >= g.n_tokens) continue;                           // none: EMPTY among them
-                uint32_t h = slot_of(token[i]);
-                for (;; h = (h + 1) & (SLOTS - 1)) {
-                    const uint32_t was = atomicCAS(&s.key[h], EMPTY, token[i]);
-                    if (was == EMPTY || was == token[i]) break;
-                }
-                if (k0 + i * THREADS + tid >= r.prompt) atomicAdd(&s.cnt[h], 1u); else atomicOr(&s.cnt[h], SEEN);
-            }
-            block_sync<THREADS>();
-            uint32_t found[EACH];
+        for (int v = 0; v < EACH; ++v) found[v] = s.key[slot_of(en[v].x)];
 #pragma unroll
-            for (int v = 0; v < EACH; ++v) found[v] = s.key[slot_of(en[v].x)];
-#pragma unroll
-            for (int v = 0; v < EACH; ++v) {
-                uint32_t h = slot_of(en[v].x);
-                while (found[v] != EMPTY && found[v] != en[v].x) { h = (h + 1) & (SLOTS - 1); found[v] = s.key[h]; }
-                if (found[v] != EMPTY) {
-                    const uint32_t n = s.cnt[h];
-                    c[v] = (c[v] + (n & ~SEEN)) | (n & SEEN);
-                }
+        for (int v = 0; v < EACH; ++v) {
+            uint32_t h = slot_of(en[v].x);
+            while (found[v] != EMPTY && found[v] != en[v].x) { h = (h + 1) & (SLOTS - 1); found[v] = s.key[h]; }
+            if (found[v] != EMPTY) {
+                const uint32_t n = s.cnt[h];
+                c[v] = (c[v] + (n & ~SEEN)) | (n & SEEN);
             }
         }
     }
 
-    // z of the m entries from e0: entry i of the piece is thread i % THREADS's number i / THREADS; -infinity where it may not be taken
+    // z of the m entries from e0: entry i of the piece is thread i % THREADS's number i / THREADS; -infinity where it may not be taken.  The history's table is made
+    // while the entries are on their way, and asked while their logits are.
     template <class T>
     static __device__ void shaped(const DevGrammar& g, const tp_logits& a, const RowRules& r, float temper, uint64_t row, uint32_t tags, uint32_t e0, uint32_t m, Lds& s, uint2 (&en)[EACH], float (&x)[EACH]) {
         const auto l = logit_row<T>(a, row);
@@ -964,19 +967,30 @@ struct Step {
         bool ok[EACH];
         typename T::S raw[EACH];
         float b[EACH];
+        unsigned long long e[EACH];
+        uint32_t token[RECALL];
+        remember(r, 0, token);
 #pragma unroll
-        for (int v = 0; v < EACH; ++v) {
-            const unsigned long long e = (uint32_t)v * THREADS + tid < m ? entries[v * THREADS + tid] : (unsigned long long)EMPTY;
-            en[v] = make_uint2((uint32_t)e, (uint32_t)(e >> 32));
+        for (int v = 0; v < EACH; ++v) e[v] = (uint32_t)v * THREADS + tid < m ? entries[v * THREADS + tid] : (unsigned long long)EMPTY;
+        if (r.len) {
+            block_sync<THREADS>();                                               // the piece before has asked its table
+            put_down(g, r, 0, token, s);
         }
 #pragma unroll
         for (int v = 0; v < EACH; ++v) {
+            en[v] = make_uint2((uint32_t)e[v], (uint32_t)(e[v] >> 32));
             ok[v] = en[v].x != EMPTY && may(en[v].y, tags, g);
             raw[v] = ok[v] ? l[en[v].x] : (typename T::S)0;
             b[v] = ok[v] && r.bias ? r.bias[en[v].x] : 0.0f;
         }
         uint32_t c[EACH] = {};
-        recall(g, r, en, s, c);
+        if (r.len) look_up(en, s, c);
+        for (uint32_t k0 = THREADS * RECALL; k0 < r.len; k0 += THREADS * RECALL) {
+            remember(r, k0, token);
+            block_sync<THREADS>();
+            put_down(g, r, k0, token, s);
+            look_up(en, s, c);
+        }
 #pragma unroll
         for (int v = 0; v < EACH; ++v) {
             float y = penalised(T::up(raw[v]), c[v], r);
@@ -1152,32 +1166,47 @@ __device__ inline Written written(const int32_t* begin, const int32_t* len, uint
 // it up, where a row begins, and its text.  (Rows beyond LINES_DIRECT are added up by the scan of the caption offsets instead.)
 // A wave holds LINE_AHEAD times 64 tokens at once, so that 256 tokens cost two rounds of memory latency: the tokens, and their texts, which stand beside
 // their sizes in 16 bytes up to a length of 15.  Bound by the gathers (64 cache lines a wave's load) and by LDS: 8192 rows of up to 300 tokens (7 MB of
-// tokens, 13 of text: 4.5 us at a copy's rate) take 10 us for the sizes and 17 for the texts.
+// tokens, 13 of text: 4.5 us at a copy's rate) take 6 us for the sizes (10 without the table of lengths in LDS) and 17 for the texts.
 constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, LINE_AHEAD = 4, SIZE_AHEAD = 8;
 constexpr uint64_t LINES_DIRECT = 65536;
 
+// TABLE: the block first brings the lengths of all tokens into LDS, four bits each.  A token's length costs a cache line otherwise.
+template <bool TABLE>
 __global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0,
                                                              uint64_t rows, uint32_t* sizes, unsigned long long* sums) {
     __shared__ uint32_t of_row[LINE_ROWS];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const uint64_t row = (block0 + blockIdx.x) * LINE_ROWS + wave;
-    uint32_t n = 0;
-    if (row < rows) {
-        const Written w = written(begin, len, width, row);
-        const auto t = glob(tokens) + row * stride;
-        const auto bytes = glob(g.bytes);
-        for (uint32_t k0 = w.first; k0 < w.last; k0 += SIZE_AHEAD * 64) {
-            uint32_t id[SIZE_AHEAD], of[SIZE_AHEAD];
+    const Written w = row < rows ? written(begin, len, width, row) : Written{0, 0};
+    const auto t = glob(tokens) + row * stride;
+    const auto bytes = glob(g.bytes);
+    uint32_t n = 0, id[SIZE_AHEAD];
+    auto load = [&](uint32_t k0) {
 #pragma unroll
-            for (uint32_t q = 0; q < SIZE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
-#pragma unroll
-            for (uint32_t q = 0; q < SIZE_AHEAD; ++q) of[q] = id[q] < g.n_tokens ? (uint32_t)bytes[id[q]] : 0u;
-#pragma unroll
-            for (uint32_t q = 0; q < SIZE_AHEAD; ++q) n += of[q] == LONG_TOKEN ? glob((const uint32_t*)g.record)[id[q] * 4ull + 1] : of[q];
-        }
-        n = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
-        if (lane == 0) sizes[row] = n;
+        for (uint32_t q = 0; q < SIZE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
+    };
+    load(w.first);
+    if constexpr (TABLE) {
+        const uint32_t pieces = (g.n_tokens + 31) / 32;
+        for (uint32_t i = threadIdx.x; i < pieces; i += LINE_THREADS) ((uint4*)dynamic_lds)[i] = g.quarter[i];
+        __syncthreads();
     }
+    for (uint32_t k0 = w.first; k0 < w.last; k0 += SIZE_AHEAD * 64) {
+        if (k0 != w.first) load(k0);
+        uint32_t of[SIZE_AHEAD];
+#pragma unroll
+        for (uint32_t q = 0; q < SIZE_AHEAD; ++q) {
+            if constexpr (TABLE) of[q] = id[q] < g.n_tokens ? dynamic_lds[id[q] >> 3] >> (id[q] % 8 * 4) & 15u : 0u;
+            else of[q] = id[q] < g.n_tokens ? (uint32_t)bytes[id[q]] : 0u;
+        }
+#pragma unroll
+        for (uint32_t q = 0; q < SIZE_AHEAD; ++q) {
+            if (TABLE && of[q] == 15) of[q] = bytes[id[q]];
+            n += of[q] == LONG_TOKEN ? glob((const uint32_t*)g.record)[id[q] * 4ull + 1] : of[q];
+        }
+    }
+    n = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+    if (lane == 0 && row < rows) sizes[row] = n;
     if (!sums) return;
     if (lane == 0) of_row[wave] = n;
     __syncthreads();
@@ -1427,14 +1456,23 @@ hipError_t launch_grammar_step(const DevGrammar& g, const tp_logits& io, const f
     });
 }
 
+// The lengths in LDS: up to 64 KB of them, so that two blocks share a compute unit, and where there are blocks for every unit and tokens enough to pay for the table.
+// Without / with it, of 131072 tokens: 8192 rows of up to 300 tokens 9.5 / 6.1 us, of 128 5.9 / 6.1; 4096 rows of 300 6.2 / 5.2, 2048 rows 5.1 / 4.8 at 300 and
+// 3.9 / 4.8 at 128; of 32768 tokens: 8192 rows of 300 5.5 / 4.7, of 128 4.4 / 4.6.
+static bool line_sizes_by_table(const DevGrammar& g, uint64_t rows, uint32_t width) {
+    return g.n_tokens <= 131072 && rows >= 256 * LINE_ROWS && width >= 192;
+}
+
 hipError_t launch_grammar_lines(const DevGrammar& g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t rows,
                                 uint8_t* arena, uint64_t capacity, uint64_t* offsets, void* workspace, hipStream_t s) {
     uint32_t* sizes = (uint32_t*)workspace;
     unsigned long long* sums = (unsigned long long*)((uint8_t*)workspace + (rows + 4) / 4 * 16);
     const uint64_t blocks = (rows + LINE_ROWS - 1) / LINE_ROWS;
     const bool direct = rows <= LINES_DIRECT;
+    const bool table = line_sizes_by_table(g, rows, width);
     hipError_t e = in_ranges(blocks, [&](uint64_t b, unsigned n) {
-        hipLaunchKernelGGL(k_line_sizes, dim3(n), dim3(LINE_THREADS), 0, s, g, tokens, stride, width, begin, len, b, rows, sizes, direct ? sums : nullptr);
+        if (table) hipLaunchKernelGGL(k_line_sizes<true>, dim3(n), dim3(LINE_THREADS), (g.n_tokens + 31) / 32 * 16, s, g, tokens, stride, width, begin, len, b, rows, sizes, direct ? sums : nullptr);
+        else hipLaunchKernelGGL(k_line_sizes<false>, dim3(n), dim3(LINE_THREADS), 0, s, g, tokens, stride, width, begin, len, b, rows, sizes, direct ? sums : nullptr);
     });
     if (e != hipSuccess) return e;
     if (!direct) e = launch_scan_u32(sizes, rows, offsets, (uint64_t*)sums, nullptr, nullptr, s);
