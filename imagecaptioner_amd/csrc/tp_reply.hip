@@ -212,12 +212,22 @@ __device__ inline float temperature_of(const float* temperature, const float* un
 __device__ inline float countable(float x) { return x == x ? x : NEG_INF; }
 // the z of the weights, never a NaN; temper: the temperature, 1 where the largest is chosen
 __device__ inline float z_of(float x, float temper) { return countable(x / temper); }
-// x of at least `low`; the builtins would first make an ordinary number of every operand
-__device__ inline float at_least(float x, float low) {
-    float r;
-    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(x), "v"(low));
-    return r;
-}
+// The same quotient of many x by two operations.  hi + lo is 1 / temper to 48 bits, hi below it, so that x * hi + x * lo is off by 2^-46 before the one
+// rounding that matters; with lo above 0 an infinite x gives the infinity that it should.  A temper out of bounds gives NaNs, whoever has them divides.
+struct Inverse {
+    float hi, lo;
+    __device__ Inverse(float temper) {
+        hi = 1.0f / temper;
+        float rest = __builtin_fmaf(-hi, temper, 1.0f);
+        if (rest < 0.0f) {
+            hi = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, hi) - 1);
+            rest = __builtin_fmaf(-hi, temper, 1.0f);
+        }
+        lo = fmaxf(rest * hi, 1.17549435e-38f);
+        if (!(temper > 1e-30f && temper < 1e30f)) hi = __builtin_nanf("");
+    }
+    __device__ float z(float x) const { return __builtin_fmaf(x, hi, x * lo); }
+};
 __device__ inline float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -584,10 +594,9 @@ __device__ inline float segment_largest(const float (&x)[VECS][8], float temper,
 // The lane's sum of a segment's weights.  They are taken against `ref`, and only where they outgrow it, or there is none, against
 // the segment's own largest z, which is the wave's `ref` from then on: the shares that the join works with do not mind what they are
 // relative to, and the largest need not be found.  With `greedy` it is the segment's largest in any case.
-// A quotient x / T of the vectors is x * (1 / T), corrected by its exact remainder; what that cannot do (infinities, temperatures whose inverse is none) becomes
-// a NaN, and the segment is done again by divisions.  The x far below `ref`, -infinity among them, are lifted to where a weight is still 0.
+// A NaN among the weights has the segment done again, by divisions and without the NaNs.
 template <class T, bool TINY, class Next>
-__device__ inline float segment_part(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, float temper, float inverse, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
+__device__ inline float segment_part(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, float temper, const Inverse& inverse, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
                                           const uint32_t* value, Next&& next) {
     float x[VECS][8];
     uint32_t i0, i1;
@@ -601,15 +610,11 @@ __device__ inline float segment_part(const RowRules& r, uint32_t n, uint32_t g, 
     if (greedy || ref == NEG_INF) ref = segment_largest(x, temper, value, i0, i1);
     Scale scale(ref);
     float sum = 0.0f;
-    const float low = (ref - 200.0f - fabsf(ref) * 0x1p-10f) * temper;
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
         float w[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float y = at_least(x[v][j], low), q = y * inverse;
-            w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(__builtin_fmaf(__builtin_fmaf(-q, temper, y), inverse, q), LOG2E, -scale.c));
-        }
+        for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(inverse.z(x[v][j]), LOG2E, -scale.c));
         sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     }
     if (i1 > i0) sum = (float)((double)sum + repeated(scale));
@@ -753,7 +758,8 @@ __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_
     __shared__ float largest[CHOICE_WAVES];
     const uint64_t row = row0 + blockIdx.y;
     const uint32_t chunks = gridDim.x, window = segs * CHOICE_WAVES * SEGMENT, w0 = blockIdx.x * window, n = a.vocab - w0, segments = reply_segments(a.vocab);
-    const float t = temperature_of(temperature, uniform, row), temper = t > 0.0f ? t : 1.0f, inverse = 1.0f / temper;
+    const float t = temperature_of(temperature, uniform, row), temper = t > 0.0f ? t : 1.0f;
+    const Inverse inverse(temper);
     const RowRules r = row_rules(a, row);
     const auto from = logit_row<T>(a, row) + w0;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * CHOICE_WAVES, reply_segments(n));
