@@ -551,7 +551,7 @@ struct Window {
 // of 0.5 .. 1.2, one row of 5000 got another token, always the border's other side.
 //
 // What bounds it: 512 rows of 131072 bfloat16 (134 MB, 26 us at a copy's rate) with 256 tokens of history and a bias take 45 us: the vector units
-// spend some 300 instructions a segment, a third of them in the quotients and a quarter in the powers; the block's start (rules, history and repeated tokens: 6 us) and the join of
+// spend some 260 instructions a segment (powers: 16, four times as long), 29 us of work; the block's start (rules, history and repeated tokens: 6 us) and the join of
 // the row (4 us) are chains of latency that no other block hides, since all rows are at work at once.
 using OneSegment = Window<1, 1>;
 constexpr int CHOICE_WAVES = 16, MOST_SEGS = 8;                               // waves of a block, segments of a wave at the most
@@ -1126,8 +1126,8 @@ struct Step {
 
 // A block per row.  Most places of a tag line have a handful of tokens, and the places where a tag begins thousands: a list of up to 64
 // is the work of one wave, which needs no barrier, and the block's other waves are done at once.  Bound by latency: 256 rows over
-// 131072 tokens and lists of up to 4781 take 16 us, one row 14, of which the bytes (1.3 MB, 0.3 us) are next to nothing; rules and list, entries, their
-// logits, the history's table, the sums and the choice each wait for what comes before.
+// 131072 tokens and lists of up to 4781 take 15.5 us, of which the bytes (1.3 MB, 0.3 us) are next to nothing; rules and list, entries, their
+// logits, the sums and the choice each wait for what comes before.
 constexpr int STEP_THREADS = 1024;
 using LongStep = Step<STEP_THREADS, 8, 1>;
 using ShortStep = Step<64, 1, 4>;
