@@ -22,11 +22,31 @@ COMMON = ["-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unus
 DEVICE = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
+# The torch side of the reply calls: a Python module against the torch that is installed, host code only.
+TORCH_SOURCE = os.path.join(CSRC, "tp_torch.cpp")
+TORCH_LIB = os.path.join(HERE, "_tp_torch.so")
+
+
+def _build_torch_module(verbose):
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+           "-I" + sysconfig.get_paths()["include"]]
+    for d in ("include", os.path.join("include", "torch", "csrc", "api", "include")):
+        cmd += ["-isystem", os.path.join(root, d)]
+    cmd += [TORCH_SOURCE, "-o", TORCH_LIB, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+
+
 def _stale():
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(TORCH_LIB):
         return True
-    t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_LIB))
+    return os.path.getmtime(TORCH_SOURCE) > t or any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS)
 
 
 def build(force=False, verbose=False, prof=False):
@@ -39,7 +59,9 @@ def build(force=False, verbose=False, prof=False):
         return _build(LIB.replace(".so", "_%s.so" % name), "_%s.o" % name, [f for f in flags.split(",") if f], verbose, kernels_only=True)
     if not force and not _stale():
         return LIB
-    return _build(LIB, ".o", [], verbose)
+    lib = _build(LIB, ".o", [], verbose)
+    _build_torch_module(verbose)
+    return lib
 
 
 def _build(lib, obj_suffix, extra, verbose, kernels_only=False):

@@ -14,146 +14,53 @@ torch tensors of that device, on torch's current stream, without waiting for it,
 Nothing here has a gradient: the calls shape what a model answers while it answers.
 """
 import ctypes as C
-import struct
 
 import numpy as np
 
 from ._abi import TP_E_CAPACITY, VERDICT_DTYPE, tp_counters, tp_device_io, tp_grammar_config, tp_grammar_info
 from .tagpipe import BatchResult, TagPipeError, load_library
 
-# A decoding loop makes these calls once per token, and the host's part of a small call takes longer than the GPU's: arguments are
-# checked with as few tensor queries as will do, and tp_logits is packed in one go (the layout of _abi.tp_logits).
-_LOGITS = struct.Struct("@IiQIIPQPQPPPPPPQPPQPIIP")
+_native_module = None
 _torch_module = None
-_TYPES = None
+
+
+def _native():
+    """The module that checks the tensors, makes the outputs and calls the library (csrc/tp_torch.cpp)."""
+    global _native_module, _torch_module
+    if _native_module is None:
+        import torch
+        L = load_library()
+        try:
+            from . import _tp_torch
+        except ImportError as e:
+            raise TagPipeError(-3, "the torch module is not built or does not fit this torch (run `python -m imagecaptioner_amd.build`): %s" % e) from e
+
+        def failed(rc):
+            raise TagPipeError(rc, L.tp_last_error().decode("utf-8", "replace"))
+        _tp_torch.bind(*(C.cast(f, C.c_void_p).value for f in (L.tp_shape_logits, L.tp_choose_workspace, L.tp_choose_tokens, L.tp_grammar_mask, L.tp_grammar_step,
+                                                              L.tp_lines_workspace, L.tp_grammar_lines)), failed)
+        _native_module, _torch_module = _tp_torch, torch
+    return _native_module
 
 
 def _torch():
-    global _torch_module, _TYPES
-    if _torch_module is None:
-        import torch
-        _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-        _torch_module = torch
+    _native()
     return _torch_module
 
 
-def _stream(torch, device):
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)                 # the same number without a Stream object around it
-    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
-
-
-def _refuse(name, t, device, dtype, shape):
-    if t.requires_grad and _torch_module.is_grad_enabled():
-        raise ValueError("%s requires a gradient, which this call does not have: detach it" % name)
-    raise ValueError("%s must be a %s tensor of the shape %s on cuda:%d, dense along its last axis, got %s %s with strides %s on %s" % (
-        name, dtype, shape, device, t.dtype, tuple(t.shape), t.stride(), t.device))
-
-
-def _vec(name, t, device, dtype, rows):
-    """A dense vector's data pointer."""
-    if t.dtype is not dtype or t.get_device() != device or t.shape != (rows,) or not t.is_contiguous() or (t.requires_grad and _torch_module.is_grad_enabled()):
-        _refuse(name, t, device, dtype, "(%d,)" % rows)
-    return t.data_ptr()
-
-
-def _table(name, t, device, dtype, rows, columns):
-    """A table's data pointer, rows, columns and elements between rows (its columns where there is one row at most); rows or columns -1: any."""
-    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2 or (t.requires_grad and _torch_module.is_grad_enabled()):
-        _refuse(name, t, device, dtype, "(%d, %d)" % (rows, columns))
-    r, c = t.shape
-    stride, dense = t.stride()
-    if (rows != -1 and r != rows) or (columns != -1 and c != columns) or (c > 1 and dense != 1):
-        _refuse(name, t, device, dtype, "(%d, %d)" % (rows, columns))
-    return t.data_ptr(), r, c, stride if r > 1 else c
-
-
-def logit_rules(device, type_, rows, vocab, logits, stride, *, history=None, history_len=None, prompt_len=None, repetition=None, frequency=None, presence=None,
-                bias=None, bias_row=None, mask=None, mask_row=None):
-    """A packed tp_logits.
-
-    history int32 [rows, n] with history_len int32 [rows] (every row is full without it); entries before prompt_len int32 [rows] count as
-    repeated but not for frequency and presence.  repetition, frequency, presence: float32 [rows].
-    bias float32 [n, vocab] (or [vocab]) with bias_row int32 [rows]: which one a row takes, -1 none; row 0 for all without it.
-    mask int32 [n, (vocab + 31) // 32] (or one row) with mask_row likewise: token t is allowed when bit t % 32 of word t // 32 is set."""
-    torch = _torch()
-    i32, f32 = torch.int32, torch.float32
-    h = h_cap = h_stride = h_len = prompt = b = b_stride = b_row = n_bias = m = m_stride = m_row = n_masks = 0
-    if history is not None:
-        h, _, h_cap, h_stride = _table("history", history, device, i32, rows, -1)
-        if history_len is not None:
-            h_len = _vec("history_len", history_len, device, i32, rows)
-        if prompt_len is not None:
-            prompt = _vec("prompt_len", prompt_len, device, i32, rows)
-        if not h:                                            # no rows, or rows of no room: there is no history, whatever the lengths say
-            h_len = prompt = 0
-    elif history_len is not None or prompt_len is not None:
-        raise ValueError("history_len or prompt_len without a history")
-    if bias is not None:
-        b, n_bias, _, b_stride = _table("bias", bias if bias.dim() == 2 else bias[None], device, f32, -1, vocab)
-        if bias_row is not None:
-            b_row = _vec("bias_row", bias_row, device, i32, rows)
-        if not n_bias:
-            raise ValueError("bias has no rows")
-    elif bias_row is not None:
-        raise ValueError("bias_row without a bias")
-    if mask is not None:
-        m, n_masks, _, m_stride = _table("mask", mask if mask.dim() == 2 else mask[None], device, i32, -1, (vocab + 31) // 32)
-        if mask_row is not None:
-            m_row = _vec("mask_row", mask_row, device, i32, rows)
-        if not n_masks:
-            raise ValueError("mask has no rows")
-    elif mask_row is not None:
-        raise ValueError("mask_row without a mask")
-    return _LOGITS.pack(_LOGITS.size, type_, rows, vocab, h_cap, logits, stride, h, h_stride, h_len, prompt,
-                        0 if repetition is None else _vec("repetition", repetition, device, f32, rows),
-                        0 if frequency is None else _vec("frequency", frequency, device, f32, rows),
-                        0 if presence is None else _vec("presence", presence, device, f32, rows),
-                        b, b_stride, b_row, m, m_stride, m_row, n_bias, n_masks, _stream(torch, device))
-
-
-def _with_logits(device, logits, rules):
-    """(packed tp_logits, rows, vocab)"""
-    _torch()
-    dtype = logits.dtype
-    if dtype not in _TYPES:
-        raise ValueError("logits must be a float32, float16 or bfloat16 tensor [rows, vocab], got %s" % dtype)
-    p, rows, vocab, stride = _table("logits", logits, device, dtype, -1, -1)
-    return logit_rules(device, _TYPES[dtype], rows, vocab, p, stride, **rules), rows, vocab
-
-
-def _choice_inputs(device, rows, temperature, uniform):
-    torch = _torch()
-    t = None if temperature is None else _vec("temperature", temperature, device, torch.float32, rows)
-    u = None if uniform is None else _vec("uniform", uniform, device, torch.float32, rows)
-    if t and not u:
-        raise ValueError("a temperature needs `uniform`, the random numbers of the choice")
-    return t, u
+def _stream(device):
+    raw = getattr(_torch_module._C, "_cuda_getCurrentRawStream", None)         # the same number without a Stream object around it
+    return raw(device) if raw is not None else _torch_module.cuda.current_stream(device).cuda_stream
 
 
 def shape_logits(pipe, logits, out, rules):
-    device = pipe._device
-    io, rows, vocab = _with_logits(device, logits, rules)
-    if out is None:
-        out = logits.new_empty((rows, vocab))
-        to, stride = out.data_ptr(), vocab
-    else:
-        to, _, _, stride = _table("out", out, device, logits.dtype, rows, vocab)
-        _torch().autograd.graph.increment_version(out)           # a backward pass that has kept what `out` held finds it changed
-    pipe._check(pipe._L.tp_shape_logits(pipe._h, io, to, stride))
-    return out
+    native, device = _native(), pipe._device
+    return native.shape(pipe._h, device, _stream(device), logits, out, rules)
 
 
 def choose_tokens(pipe, logits, temperature, uniform, rules):
-    torch = _torch()
-    device = pipe._device
-    io, rows, vocab = _with_logits(device, logits, rules)
-    t, u = _choice_inputs(device, rows, temperature, uniform)
-    need = pipe._L.tp_choose_workspace(rows, vocab)
-    workspace = logits.new_empty((need,), dtype=torch.uint8) if need else None   # torch's own pool keeps it apart per stream and per graph
-    tokens = logits.new_empty((rows,), dtype=torch.int32)
-    logprob = logits.new_empty((rows,), dtype=torch.float32)
-    pipe._check(pipe._L.tp_choose_tokens(pipe._h, io, t, u, tokens.data_ptr(), logprob.data_ptr(), workspace.data_ptr() if need else None, need))
-    return tokens, logprob
+    native, device = _native(), pipe._device
+    return native.choose(pipe._h, device, _stream(device), logits, temperature, uniform, rules)
 
 
 def _pack(texts):
@@ -188,7 +95,7 @@ class TagGrammar:
         self._check(self._L.tp_grammar_get_info(self._h, C.byref(self.info)))
         self.device = pipe._device
         self.end_place = self.info.n_prefixes + 1
-        self._words = (self.info.n_tokens + 31) // 32
+        self._n_tokens, self._longest, self._words = self.info.n_tokens, self.info.longest_token, (self.info.n_tokens + 31) // 32
 
     def _check(self, rc):
         if rc != 0:
@@ -210,60 +117,28 @@ class TagGrammar:
         torch = _torch()
         return torch.zeros(rows, 2, dtype=torch.int32, device="cuda:%d" % self.device)
 
-    def _states(self, states):
-        p, rows, _, stride = _table("states", states, self.device, _torch().int32, -1, 2)
-        if stride != 2:
-            raise ValueError("states must be dense")
-        return p, rows
-
     def mask(self, states, out=None):
         """tp_grammar_mask: the allowed-token masks of rows of states, int32 [rows, (n_tokens + 31) // 32]."""
-        p, rows = self._states(states)
-        words = self._words
-        if out is None:
-            out = states.new_empty((rows, words))
-            to, stride = out.data_ptr(), words
-        else:
-            to, _, _, stride = _table("out", out, self.device, states.dtype, rows, words)
-        self._check(self._L.tp_grammar_mask(self._h, p, rows, to, stride, _stream(_torch(), self.device)))
-        return out
+        native = _native()
+        return native.mask(self._h, self.device, _stream(self.device), states, self._words, out)
 
     def step(self, states, logits, *, temperature=None, uniform=None, append=False, **rules):
         """tp_grammar_step: (tokens int32 [rows], log-probabilities float32 [rows]); `states` move on in place, and with append=True the
-        tokens go to the end of `history` and `history_len` rises.  -1: the row's line is at its end, or nothing is left to choose."""
-        p, rows = self._states(states)
-        io, of_logits, _ = _with_logits(self.device, logits, rules)
-        if of_logits != rows:
-            raise ValueError("one state per row of logits")
-        t, u = _choice_inputs(self.device, rows, temperature, uniform)
-        tokens = states.new_empty((rows,))
-        logprob = states.new_empty((rows,), dtype=_torch().float32)
-        self._check(self._L.tp_grammar_step(self._h, io, t, u, p, tokens.data_ptr(), logprob.data_ptr(), bool(append)))
-        return tokens, logprob
+        tokens go to the end of `history` and `history_len` rises.  -1: the row's line is at its end, or nothing is left to choose.  `rules` are
+        those of TagPipe.shape_logits, without a mask."""
+        native = _native()
+        return native.step(self._h, self.device, _stream(self.device), states, logits, temperature, uniform, append, rules)
 
     def advance(self, states, tokens, *, history=None, history_len=None, append=False):
         """tp_grammar_step by the caller's own tokens (int32 [rows]): `states` move on in place; to place -1 where a token is not allowed."""
-        p, rows = self._states(states)
-        io = logit_rules(self.device, 0, rows, self.info.n_tokens, 0, 0, history=history, history_len=history_len)
-        self._check(self._L.tp_grammar_step(self._h, io, None, None, p, _vec("tokens", tokens, self.device, states.dtype, rows), None, bool(append)))
+        native = _native()
+        native.advance(self._h, self.device, _stream(self.device), states, self._n_tokens, tokens, append, {"history": history, "history_len": history_len})
 
     def lines(self, tokens, lengths=None, begin=None, arena=None):
         """tp_grammar_lines: (arena uint8, offsets int64 [rows + 1]) of rows of tokens int32 [rows, n], from begin to below lengths (int32
         [rows]).  A given arena bounds what is written: compare offsets[rows] with its size."""
-        torch = _torch()
-        i32 = torch.int32
-        p, rows, n, stride = _table("tokens", tokens, self.device, i32, -1, -1)
-        le = None if lengths is None else _vec("lengths", lengths, self.device, i32, rows)
-        be = None if begin is None else _vec("begin", begin, self.device, i32, rows)
-        if arena is None:
-            arena = tokens.new_empty((rows * n * self.info.longest_token + 16,), dtype=torch.uint8)
-        to = _vec("arena", arena, self.device, torch.uint8, arena.numel())
-        offsets = tokens.new_empty((rows + 1,), dtype=torch.int64) if rows else tokens.new_zeros((1,), dtype=torch.int64)
-        need = self._L.tp_lines_workspace(rows)
-        workspace = tokens.new_empty((need,), dtype=torch.uint8)
-        self._check(self._L.tp_grammar_lines(self._h, p, stride, n, be, le, rows, to, arena.numel(), offsets.data_ptr(), workspace.data_ptr(), need,
-                                             _stream(torch, self.device)))
-        return arena, offsets
+        native = _native()
+        return native.lines(self._h, self.device, _stream(self.device), tokens, lengths, begin, arena, self._longest)
 
 
 # An arena for rows of nothing but the longest token is made up to this many bytes; beyond it (a token list may hold a token of a hundred
@@ -294,7 +169,7 @@ def run_tokens(pipe, grammar, tokens, lengths, begin):
         io.arena, io.offsets, io.n_files = arena.data_ptr(), offsets.data_ptr(), rows
         io.captions, io.caption_capacity, io.caption_offsets = captions.data_ptr(), capacity, caption_offsets.data_ptr()
         io.verdicts, io.histogram, io.counters = verdicts.data_ptr(), histogram.data_ptr(), counters.data_ptr()
-        io.fired, io.facet_choice, io.stream = fired.data_ptr(), facets.data_ptr(), _stream(torch, pipe._device)
+        io.fired, io.facet_choice, io.stream = fired.data_ptr(), facets.data_ptr(), _stream(pipe._device)
         try:
             total = pipe.run_lines_device(io)
             break

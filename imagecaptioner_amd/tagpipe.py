@@ -481,7 +481,12 @@ class TagPipe:
     # ---- writing the replies (torch tensors on the context's device; see replies.py) ----------------
     def shape_logits(self, logits, *, out=None, **rules):
         """tp_shape_logits: penalties for repeated tokens, biases and allowed-token masks on logits [rows, vocab] (float32, float16 or
-        bfloat16).  `rules` are those of replies.logit_rules.  `out` may be `logits` itself (in place); a new tensor otherwise."""
+        bfloat16).  `out` may be `logits` itself (in place); a new tensor otherwise.  The rules, all of them optional:
+
+        history int32 [rows, n] with history_len int32 [rows] (every row is full without it); entries before prompt_len int32 [rows] count as
+        repeated but not for frequency and presence.  repetition, frequency, presence: float32 [rows].
+        bias float32 [n, vocab] (or [vocab]) with bias_row int32 [rows]: which one a row takes, -1 none; row 0 for all without it.
+        mask int32 [n, (vocab + 31) // 32] (or one row) with mask_row likewise: token t is allowed when bit t % 32 of word t // 32 is set."""
         return replies.shape_logits(self, logits, out, rules)
 
     def choose_tokens(self, logits, *, temperature=None, uniform=None, **rules):

@@ -252,12 +252,35 @@ def test_null_handles_are_refused_by_the_library():
     L.tp_grammar_destroy(None)
 
 
-def test_packed_logits_have_the_structs_layout():
-    from imagecaptioner_amd.replies import _LOGITS
-    n = len(tp_logits._fields_)
-    assert _LOGITS.size == C.sizeof(tp_logits)
-    io = tp_logits.from_buffer_copy(_LOGITS.pack(*range(1, n + 1)))
-    assert [getattr(io, f) for f, _ in tp_logits._fields_] == list(range(1, n + 1))
+def test_the_torch_module_refuses_without_a_device():
+    """Everything is checked before the library is called: with tensors of the host there is nothing else to do."""
+    import torch
+
+    from imagecaptioner_amd.replies import _native
+    native = _native()
+    x, i = torch.zeros(2, 40), torch.zeros(2, dtype=torch.int32)
+    states = torch.zeros(2, 2, dtype=torch.int32)
+    for text, call in (("logits must be a Float tensor", lambda: native.shape(None, 0, 0, x, None, {})), ("logits must be a tensor", lambda: native.shape(None, 0, 0, 7, None, {})),
+                       ("float32, float16 or bfloat16", lambda: native.choose(None, 0, 0, x.double(), None, None, {})), ("states must be", lambda: native.mask(None, 0, 0, states, 2, None)),
+                       ("states must be", lambda: native.step(None, 0, 0, states, x, None, None, False, {})), ("states must be", lambda: native.advance(None, 0, 0, states, 40, i, False, {})),
+                       ("tokens must be a Int tensor", lambda: native.lines(None, 0, 0, x, None, None, None, 5)), ("requires a gradient", lambda: native.shape(None, 0, 0, x.clone().requires_grad_(), None, {}))):
+        with pytest.raises(ValueError, match=text):
+            call()
+    with pytest.raises(TypeError):
+        native.shape(None, 0, 0, x, None)
+    # device -1 is the host's: the checks of the rules, up to the library's own refusal of a context that is none
+    from imagecaptioner_amd import TagPipeError
+    for error, text, rules in ((ValueError, "history_len or prompt_len without a history", dict(history_len=i)), (ValueError, "bias_row without a bias", dict(bias_row=i)),
+                               (ValueError, "mask must be", dict(mask=torch.zeros(2, 3, dtype=torch.int32))), (ValueError, "bias must be", dict(bias=torch.zeros(39))), (ValueError, "bias has 0 rows", dict(bias=torch.zeros(0, 40))),
+                               (ValueError, "history must be", dict(history=x)), (ValueError, r"history must be .*\(2, -1\)", dict(history=torch.zeros(3, 4, dtype=torch.int32))),
+                               (ValueError, r"repetition must be .*\(2,\)", dict(repetition=torch.ones(3))), (ValueError, "repetition must be .*not contiguous", dict(repetition=torch.ones(4)[::2])),
+                               (TypeError, "unexpected keyword argument 'penalty'", dict(penalty=i)), (TagPipeError, "null argument", dict(bias=None, mask=torch.zeros(2, dtype=torch.int32)))):
+        with pytest.raises(error, match=text):
+            native.shape(None, -1, 0, x, None, rules)
+    with pytest.raises(ValueError, match="a temperature needs"):
+        native.choose(None, -1, 0, x, torch.ones(2), None, {})
+    with pytest.raises(ValueError, match="one state per row"):
+        native.step(None, -1, 0, torch.zeros(3, 2, dtype=torch.int32), x, None, None, False, {})
 
 
 def test_struct_layouts_match_the_header(tmp_path):
