@@ -1170,21 +1170,19 @@ __device__ inline Written written(const int32_t* begin, const int32_t* len, uint
 
 // Sixteen rows a block, a wave each: first the bytes of every row's text and of the block's, then, each block adding the blocks before
 // it up, where a row begins, and its text.  (Rows beyond LINES_DIRECT are added up by the scan of the caption offsets instead.)
+// Up to LINES_ALONE rows one launch does both, every block finding the sizes of the rows before it as well: two launches / one, a pass, 8.7 / 5.4 us for 16 rows of 32 tokens,
+// 9.0 / 6.4 for 32 of 128, 11.5 / 11.6 for 64 of 300, 7.6 / 10.4 for 128 of 32.
 // A wave holds LINE_AHEAD times 64 tokens at once, so that 256 tokens cost two rounds of memory latency: the tokens, and their texts, which stand beside
 // their sizes in 16 bytes up to a length of 15.  Bound by the gathers (64 cache lines a wave's load) and by LDS: 8192 rows of up to 300 tokens (7 MB of
 // tokens, 13 of text: 4.5 us at a copy's rate) take 6 us for the sizes (10 without the table of lengths in LDS) and 17 for the texts.
 constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, LINE_AHEAD = 4, SIZE_AHEAD = 8;
-constexpr uint64_t LINES_DIRECT = 65536;
+constexpr uint64_t LINES_DIRECT = 65536, LINES_ALONE = 64;
 
-// TABLE: the block first brings the lengths of all tokens into LDS, four bits each.  A token's length costs a cache line otherwise.
-template <bool TABLE>
-__global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0,
-                                                             uint64_t rows, uint32_t* sizes, unsigned long long* sums) {
-    __shared__ uint32_t of_row[LINE_ROWS];
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const uint64_t row = (block0 + blockIdx.x) * LINE_ROWS + wave;
-    const Written w = row < rows ? written(begin, len, width, row) : Written{0, 0};
-    const auto t = glob(tokens) + row * stride;
+// The bytes of a row's text, by a wave.  `between` is called when the first tokens' loads are in flight.  TABLE: the lengths of all tokens stand in LDS, four bits each; a
+// token's length costs a cache line otherwise.
+template <bool TABLE, class F>
+__device__ inline uint32_t row_bytes(const DevGrammar& g, Glob<int32_t> t, const Written& w, F&& between) {
+    const uint32_t lane = threadIdx.x & 63;
     const auto bytes = glob(g.bytes);
     uint32_t n = 0, id[SIZE_AHEAD];
     auto load = [&](uint32_t k0) {
@@ -1192,11 +1190,7 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const
         for (uint32_t q = 0; q < SIZE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
     };
     load(w.first);
-    if constexpr (TABLE) {
-        const uint32_t pieces = (g.n_tokens + 31) / 32;
-        for (uint32_t i = threadIdx.x; i < pieces; i += LINE_THREADS) ((uint4*)dynamic_lds)[i] = g.quarter[i];
-        __syncthreads();
-    }
+    between();
     for (uint32_t k0 = w.first; k0 < w.last; k0 += SIZE_AHEAD * 64) {
         if (k0 != w.first) load(k0);
         uint32_t of[SIZE_AHEAD];
@@ -1211,7 +1205,23 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const
             n += of[q] == LONG_TOKEN ? glob((const uint32_t*)g.record)[id[q] * 4ull + 1] : of[q];
         }
     }
-    n = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+    return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n), 63);
+}
+
+template <bool TABLE>
+__global__ __launch_bounds__(LINE_THREADS) void k_line_sizes(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0,
+                                                             uint64_t rows, uint32_t* sizes, unsigned long long* sums) {
+    __shared__ uint32_t of_row[LINE_ROWS];
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint64_t row = (block0 + blockIdx.x) * LINE_ROWS + wave;
+    const Written w = row < rows ? written(begin, len, width, row) : Written{0, 0};
+    const uint32_t n = row_bytes<TABLE>(g, glob(tokens) + row * stride, w, [&] {
+        if constexpr (TABLE) {
+            const uint32_t pieces = (g.n_tokens + 31) / 32;
+            for (uint32_t i = threadIdx.x; i < pieces; i += LINE_THREADS) ((uint4*)dynamic_lds)[i] = g.quarter[i];
+            __syncthreads();
+        }
+    });
     if (lane == 0 && row < rows) sizes[row] = n;
     if (!sums) return;
     if (lane == 0) of_row[wave] = n;
@@ -1282,10 +1292,13 @@ struct Staged {
     }
 };
 
+// ALONE: no launch has found the sizes, the block finds those of its rows and of all rows before.
+template <bool ALONE>
 __global__ __launch_bounds__(LINE_THREADS) void k_line_text(DevGrammar g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t block0,
                                                             uint64_t rows, const uint32_t* sizes, const unsigned long long* sums, uint64_t* offsets, uint8_t* arena, uint64_t capacity) {
     __shared__ alignas(16) unsigned long long stage[LINE_ROWS][LINE_STAGE / 8 + 2];
     __shared__ unsigned long long before[LINE_ROWS];
+    __shared__ uint32_t here[LINE_ROWS];
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const uint64_t b = block0 + blockIdx.x, row = b * LINE_ROWS + wave;
     const bool mine = row < rows;
@@ -1302,21 +1315,26 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_text(DevGrammar g, const 
     };
     load(w.first);                                                              // in flight while the row's place is found
     uint64_t at = 0;
-    if (sums) {
+    if (ALONE || sums) {
         unsigned long long sum = 0;
-        for (uint64_t i = threadIdx.x; i < b; i += LINE_THREADS) sum += sums[i];
-        const uint32_t size = lane < LINE_ROWS && b * LINE_ROWS + lane < rows ? sizes[b * LINE_ROWS + lane] : 0u;
-        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+        if constexpr (ALONE) {
+            const uint32_t own = row_bytes<false>(g, t, w, [] {});
+            for (uint64_t q = wave; q < b * LINE_ROWS; q += LINE_ROWS) sum += row_bytes<false>(g, glob(tokens) + q * stride, written(begin, len, width, q), [] {});
+            if (lane == 0) here[wave] = own;
+        } else {
+            for (uint64_t i = threadIdx.x; i < b; i += LINE_THREADS) sum += sums[i];
+            for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+            if (wave == 0 && lane < LINE_ROWS) here[lane] = b * LINE_ROWS + lane < rows ? sizes[b * LINE_ROWS + lane] : 0u;
+        }
         if (lane == 0) before[wave] = sum;
         __syncthreads();
-        sum = lane < LINE_ROWS ? before[lane] : 0ull;                             // the blocks before, a wave's share a lane
-        sum += lane < wave ? size : 0u;                                           // and the block's rows before this one
+        sum = lane < LINE_ROWS ? before[lane] + (lane < wave ? here[lane] : 0u) : 0ull;   // the blocks before, a wave's share a lane, and the block's rows before this one
         for (int d = 8; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
         at = sum;                                                                 // of the first sixteen lanes
         at = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at);
         if (mine && lane == 0) {
             offsets[row] = at;
-            if (row == rows - 1) offsets[rows] = at + sizes[row];
+            if (row == rows - 1) offsets[rows] = at + here[wave];
         }
     } else if (mine) {
         at = offsets[row];
@@ -1475,6 +1493,10 @@ hipError_t launch_grammar_lines(const DevGrammar& g, const int32_t* tokens, uint
     unsigned long long* sums = (unsigned long long*)((uint8_t*)workspace + (rows + 4) / 4 * 16);
     const uint64_t blocks = (rows + LINE_ROWS - 1) / LINE_ROWS;
     const bool direct = rows <= LINES_DIRECT;
+    if (rows <= LINES_ALONE) {
+        hipLaunchKernelGGL(k_line_text<true>, dim3((unsigned)blocks), dim3(LINE_THREADS), 0, s, g, tokens, stride, width, begin, len, 0, rows, nullptr, nullptr, offsets, arena, capacity);
+        return hipGetLastError();
+    }
     const bool table = line_sizes_by_table(g, rows, width);
     hipError_t e = in_ranges(blocks, [&](uint64_t b, unsigned n) {
         if (table) hipLaunchKernelGGL(k_line_sizes<true>, dim3(n), dim3(LINE_THREADS), (g.n_tokens + 31) / 32 * 16, s, g, tokens, stride, width, begin, len, b, rows, sizes, direct ? sums : nullptr);
@@ -1484,7 +1506,7 @@ hipError_t launch_grammar_lines(const DevGrammar& g, const int32_t* tokens, uint
     if (!direct) e = launch_scan_u32(sizes, rows, offsets, (uint64_t*)sums, nullptr, nullptr, s);
     if (e != hipSuccess) return e;
     return in_ranges(blocks, [&](uint64_t b, unsigned n) {
-        hipLaunchKernelGGL(k_line_text, dim3(n), dim3(LINE_THREADS), 0, s, g, tokens, stride, width, begin, len, b, rows, sizes, direct ? sums : nullptr, offsets, arena, capacity);
+        hipLaunchKernelGGL(k_line_text<false>, dim3(n), dim3(LINE_THREADS), 0, s, g, tokens, stride, width, begin, len, b, rows, sizes, direct ? sums : nullptr, offsets, arena, capacity);
     });
 }
 

@@ -566,7 +566,7 @@ def lines_of(plain, rows, first, last):
     return [plain.text(row[a:b]) for row, a, b in zip(rows, first, last)]
 
 
-@pytest.mark.parametrize("rows,width", [(1, 1), (1, 300), (5, 64), (4, 65), (70, 131), (4100, 9), (4099, 200), (70001, 2)])
+@pytest.mark.parametrize("rows,width", [(1, 1), (1, 300), (5, 64), (4, 65), (64, 70), (65, 20), (70, 131), (4100, 9), (4099, 200), (70001, 2)])
 def test_lines(pipe, rows, width):
     g, plain, tokens = small_grammar(pipe)
     rng = np.random.default_rng(rows * width)
