@@ -182,6 +182,13 @@ __device__ inline double wave_scan(double v) {
     return v;
 }
 __device__ inline double wave_sum(double v) { return read_lane(wave_scan(v), 63); }
+// in the last of eight neighbouring lanes, their sum
+__device__ inline double eight_lanes_sum(double v) {
+    v += dpp<0x111, 0xF>(v);
+    v += dpp<0x112, 0xF>(v);
+    v += dpp<0x114, 0xF>(v);
+    return v;
+}
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------
 // z = x / T is rounded to 32 bits, as the formula says, by the quotient's own rounding: with 131072 tokens a border between two of them lies in every
@@ -791,10 +798,7 @@ __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_
     __syncthreads();
     if (threadIdx.x < last * 8) {                                             // eight threads a segment
         const float4 a0 = *(const float4*)(l.lane_sum + threadIdx.x * 8), a1 = *(const float4*)(l.lane_sum + threadIdx.x * 8 + 4);
-        double sum = (((double)a0.x + a0.y) + ((double)a0.z + a0.w)) + (((double)a1.x + a1.y) + ((double)a1.z + a1.w));
-        sum += dpp<0x111, 0xF>(sum);
-        sum += dpp<0x112, 0xF>(sum);
-        sum += dpp<0x114, 0xF>(sum);
+        const double sum = eight_lanes_sum((((double)a0.x + a0.y) + ((double)a0.z + a0.w)) + (((double)a1.x + a1.y) + ((double)a1.z + a1.w)));
         if (threadIdx.x % 8 == 7) {
             const uint32_t g = threadIdx.x / 8;
             if (chunks > 1) out[g] = ChoicePart{sum, here[g].best}; else here[g].sum = sum;
@@ -916,6 +920,7 @@ struct Step {
         alignas(16) uint32_t key[SLOTS];
         alignas(16) uint32_t cnt[SLOTS];
         double sum[SEGMENTS];
+        alignas(16) float weight[EACH == 1 ? 4 : PIECE];
         float max[WAVES];
         uint32_t first;
     };
@@ -1019,10 +1024,17 @@ struct Step {
     // the segments' sums of the weights against `best`, into LDS
     static __device__ void segment_sums(const float (&x)[EACH], float best, Lds& s) {
         const Scale scale(best);
+        if constexpr (EACH == 1) {
+            const double w = wave_sum(best > NEG_INF ? (double)scale.weight(x[0]) : 0.0);
+            if ((threadIdx.x & 63) == 0) s.sum[threadIdx.x >> 6] = w;
+        } else {                                                              // eight threads a segment, eight neighbours each: three steps of 64 bits instead of 48
+            static_assert(EACH == 8, "");
 #pragma unroll
-        for (int v = 0; v < EACH; ++v) {
-            const double w = wave_sum(best > NEG_INF ? (double)scale.weight(x[v]) : 0.0);
-            if ((threadIdx.x & 63) == 0) s.sum[v * WAVES + (threadIdx.x >> 6)] = w;
+            for (int v = 0; v < EACH; ++v) s.weight[v * THREADS + threadIdx.x] = best > NEG_INF ? scale.weight(x[v]) : 0.0f;
+            block_sync<THREADS>();
+            const float4 a0 = *(const float4*)(s.weight + threadIdx.x * 8), a1 = *(const float4*)(s.weight + threadIdx.x * 8 + 4);
+            const double w = eight_lanes_sum((((double)a0.x + a0.y) + ((double)a0.z + a0.w)) + (((double)a1.x + a1.y) + ((double)a1.z + a1.w)));
+            if (threadIdx.x % 8 == 7) s.sum[threadIdx.x / 8] = w;
         }
         block_sync<THREADS>();
     }
