@@ -649,11 +649,8 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
                          float* logprob, uint32_t distinct, typename Tables::Lds& l, uint32_t* value) {
     constexpr bool HERE = Tables::TOKENS > SEGMENT;
     const uint32_t lane = threadIdx.x & 63;
-    auto from_memory = [&](uint32_t c) { return c < segments ? p[c] : ChoicePart{0.0, NEG_INF}; };
-    const ChoicePart first_parts = from_memory(lane), second_parts = from_memory(64 + lane);   // read once
-    auto part = [&](uint32_t c0) { return c0 == 0 ? first_parts : c0 == 64 ? second_parts : from_memory(c0 + lane); };
     float best = NEG_INF;
-    for (uint32_t c0 = 0; c0 < segments; c0 += 64) best = fmaxf(best, part(c0).best);
+    for (uint32_t c = lane; c < segments; c += 64) best = fmaxf(best, p[c].best);
     best = wave_max(best);
     if (!(best > NEG_INF)) {
         if (lane == 0) {
@@ -664,31 +661,28 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     }
     const float temper = t > 0.0f ? t : 1.0f;
     const Scale scale(best);
-    auto share = [&](const ChoicePart& q) { return q.sum * scale.of(q.best); };
+    auto share = [&](uint32_t c) { return c < segments ? p[c].sum * scale.of(p[c].best) : 0.0; };
     double sum = 0.0;
-    for (uint32_t c0 = 0; c0 < segments; c0 += 64) sum += share(part(c0));
+    for (uint32_t c = lane; c < segments; c += 64) sum += share(c);
     sum = wave_sum(sum);
     // Greedy: the first segment that has the largest z.  Sampled: the first whose cumulative share exceeds the target; where there is none (rounding,
     // or a `uniform` of 1 or more) the last of a share above 0, and so within the segment.
     double target = t > 0.0f ? (double)uniform[row] * sum : 0.0, carry = 0.0, before = 0.0;
     uint32_t segment = 0;
-    ChoicePart of_segment{0.0, NEG_INF};
     bool found = false;
     for (uint32_t c0 = 0; c0 < segments && !found; c0 += 64) {
-        const ChoicePart q = part(c0);
-        const double w = share(q), incl = carry + wave_scan(w);
+        const double w = share(c0 + lane), incl = carry + wave_scan(w);
         const uint64_t live = __ballot(w > 0.0);
-        const uint64_t over = t > 0.0f ? __ballot(w > 0.0 && incl > target) : __ballot(q.best == best);
+        const uint64_t over = t > 0.0f ? __ballot(w > 0.0 && incl > target) : __ballot(c0 + lane < segments && p[c0 + lane].best == best);
         if (over || (live && t > 0.0f)) {
             found = over != 0;
             const int to = found ? __builtin_ctzll(over) : 63 - __builtin_clzll(live);
             segment = c0 + (uint32_t)to;
-            of_segment = ChoicePart{read_lane(q.sum, to), read_lane(q.best, to)};
             before = read_lane(incl - w, to);
         }
         carry = read_lane(incl, 63);
     }
-    const Scale within(of_segment.best);
+    const Scale within(p[segment].best);
     target = (target - before) / scale.of(within.best);
     const uint32_t w0 = segment * SEGMENT, n = a.vocab - w0, l0 = HERE ? w0 : 0;             // l0: the segment's start within the tables
     const auto from = logit_row<T>(a, row) + w0;
@@ -756,7 +750,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     }
     // The token's own segment is now known to 64 bits: where the token has nearly all the weight, its logarithm is that of a number next to 1, and the
     // segment's sum in 32 bits would have rounded the rest away.
-    sum += (run - of_segment.sum) * scale.of(within.best);
+    sum += (run - p[segment].sum) * scale.of(within.best);
     if (lane == 0) {
         tokens[row] = (int32_t)(w0 + at);
         if (logprob) logprob[row] = scale.log_share(x_at, sum);
