@@ -1205,10 +1205,11 @@ __device__ inline Written written(const int32_t* begin, const int32_t* len, uint
 // it up, where a row begins, and its text.  (Rows beyond LINES_DIRECT are added up by the scan of the caption offsets instead.)
 // Up to LINES_ALONE rows one launch does both, every block finding the sizes of the rows before it as well: two launches / one, a pass, 8.7 / 5.4 us for 16 rows of 32 tokens,
 // 9.0 / 6.4 for 32 of 128, 11.5 / 11.6 for 64 of 300, 7.6 / 10.4 for 128 of 32.
-// A wave holds LINE_AHEAD times 64 tokens at once, so that 256 tokens cost two rounds of memory latency: the tokens, and their texts, which stand beside
+// A wave takes 64 tokens at a time, the next 64's texts and the 64 tokens behind those in flight (256 at a time, loaded together: 8192 rows of 300 in 22.2 us a pass
+// instead of 20.4, for their registers and their bursts); a text stands beside
 // their sizes in 16 bytes up to a length of 15.  Bound by the gathers (64 cache lines a wave's load) and by LDS: 8192 rows of up to 300 tokens (7 MB of
-// tokens, 13 of text: 4.5 us at a copy's rate) take 6 us for the sizes (10 without the table of lengths in LDS) and 17 for the texts.
-constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, LINE_AHEAD = 4, SIZE_AHEAD = 8;
+// tokens, 13 of text: 4.5 us at a copy's rate) take 6 us for the sizes (10 without the table of lengths in LDS) and 15 for the texts.
+constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, SIZE_AHEAD = 5;
 constexpr uint64_t LINES_DIRECT = 65536, LINES_ALONE = 64;
 
 // The bytes of a row's text, by a wave.  `between` is called when the first tokens' loads are in flight.  TABLE: the lengths of all tokens stand in LDS, four bits each; a
@@ -1338,15 +1339,10 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_text(DevGrammar g, const 
     const Written w = mine ? written(begin, len, width, row) : Written{0, 0};
     const auto t = glob(tokens) + row * stride;
     const auto record = glob((const Words4*)g.record);
-    Words4 rec[LINE_AHEAD];
-    auto load = [&](uint32_t k0) {                                               // 256 tokens of the row, 64 apart in a lane
-        uint32_t id[LINE_AHEAD];
-#pragma unroll
-        for (uint32_t q = 0; q < LINE_AHEAD; ++q) id[q] = k0 + q * 64 + lane < w.last ? (uint32_t)t[k0 + q * 64 + lane] : 0xFFFFFFFFu;
-#pragma unroll
-        for (uint32_t q = 0; q < LINE_AHEAD; ++q) rec[q] = id[q] < g.n_tokens ? record[id[q]] : Words4{0, 0, 0, 0};
-    };
-    load(w.first);                                                              // in flight while the row's place is found
+    auto token = [&](uint32_t k0) { return k0 + lane < w.last ? (uint32_t)t[k0 + lane] : 0xFFFFFFFFu; };
+    auto text_of = [&](uint32_t id) { return id < g.n_tokens ? record[id] : Words4{0, 0, 0, 0}; };
+    Words4 next = text_of(token(w.first));                                       // in flight while the row's place is found
+    uint32_t id = token(w.first + 64);
     uint64_t at = 0;
     if (ALONE || sums) {
         unsigned long long sum = 0;
@@ -1379,31 +1375,29 @@ __global__ __launch_bounds__(LINE_THREADS) void k_line_text(DevGrammar g, const 
     s.word = stage[wave];
     s.end = out + capacity;
     s.start(out + at, lane);
-    for (uint32_t k0 = w.first; k0 < w.last; k0 += LINE_AHEAD * 64) {
-        if (k0 != w.first) load(k0);
-#pragma unroll
-        for (uint32_t q = 0; q < LINE_AHEAD; ++q) {
-            if (k0 + q * 64 >= w.last) break;
-            const uint32_t kind = rec[q][3] >> 24, n = kind == LONG_TOKEN ? rec[q][1] : kind;
-            const uint32_t incl = wave_scan(n), all = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63), to = incl - n;
-            if (all <= LINE_STAGE - 16) {
-                s.flush(lane);
-                const uint32_t d = s.n + to;                                  // a flush leaves at most 15 bytes
-                if (kind != LONG_TOKEN) {
-                    s.put(d, (unsigned long long)rec[q][1] << 32 | rec[q][0], n < 8 ? n : 8);
-                    if (n > 8) s.put(d + 8, (unsigned long long)rec[q][3] << 32 | rec[q][2], n - 8);
-                } else {
-                    for (uint32_t j = 0; j < n; j += 8)                       // the texts are followed by eight bytes of room
-                        s.put(d + j, *(const Bytes8 __attribute__((address_space(1)))*)(text + rec[q][0] + j), n - j < 8 ? n - j : 8);
-                }
-                s.n += all;
-            } else {                                                          // texts longer than the stage: a lane stores its token's
-                s.finish(lane);
-                const OutBytes d = s.piece + s.n + to;
-                for (uint32_t j = 0; j < n; ++j)
-                    if (d + j < s.end) d[j] = kind == LONG_TOKEN ? text[rec[q][0] + j] : (uint8_t)((j < 8 ? j < 4 ? rec[q][0] : rec[q][1] : j < 12 ? rec[q][2] : rec[q][3]) >> (8 * (j & 3)));
-                s.start(s.piece + s.n + all, lane);
+    for (uint32_t k0 = w.first; k0 < w.last; k0 += 64) {
+        const Words4 rec = next;
+        next = text_of(id);
+        id = token(k0 + 128);
+        const uint32_t kind = rec[3] >> 24, n = kind == LONG_TOKEN ? rec[1] : kind;
+        const uint32_t incl = wave_scan(n), all = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63), to = incl - n;
+        if (all <= LINE_STAGE - 16) {
+            s.flush(lane);
+            const uint32_t d = s.n + to;                                      // a flush leaves at most 15 bytes
+            if (kind != LONG_TOKEN) {
+                s.put(d, (unsigned long long)rec[1] << 32 | rec[0], n < 8 ? n : 8);
+                if (n > 8) s.put(d + 8, (unsigned long long)rec[3] << 32 | rec[2], n - 8);
+            } else {
+                for (uint32_t j = 0; j < n; j += 8)                           // the texts are followed by eight bytes of room
+                    s.put(d + j, *(const Bytes8 __attribute__((address_space(1)))*)(text + rec[0] + j), n - j < 8 ? n - j : 8);
             }
+            s.n += all;
+        } else {                                                              // texts longer than the stage: a lane stores its token's
+            s.finish(lane);
+            const OutBytes d = s.piece + s.n + to;
+            for (uint32_t j = 0; j < n; ++j)
+                if (d + j < s.end) d[j] = kind == LONG_TOKEN ? text[rec[0] + j] : (uint8_t)((j < 8 ? j < 4 ? rec[0] : rec[1] : j < 12 ? rec[2] : rec[3]) >> (8 * (j & 3)));
+            s.start(s.piece + s.n + all, lane);
         }
     }
     s.finish(lane);
