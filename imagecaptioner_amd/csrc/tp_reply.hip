@@ -421,7 +421,7 @@ struct History {
 constexpr int SHAPE_WAVES = 8;
 constexpr uint32_t SHAPE_TOKENS = SHAPE_WAVES * SEGMENT;
 
-template <class T, bool TINY>
+template <class T, bool TINY, bool MASKED>
 __global__ __launch_bounds__(SHAPE_WAVES * 64) __attribute__((amdgpu_waves_per_eu(8))) void k_shape(tp_logits a, uint64_t row0, void* out, uint64_t out_stride) {
     using S = typename T::S;
     using V = typename At<S>::W __attribute__((address_space(1)));
@@ -431,7 +431,8 @@ __global__ __launch_bounds__(SHAPE_WAVES * 64) __attribute__((amdgpu_waves_per_e
     const uint32_t w0 = blockIdx.x * SHAPE_TOKENS, n = a.vocab - w0;
     const uint32_t g = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), at = lane_at(g);
     auto* o = (S __attribute__((address_space(1)))*)((S*)out + row * out_stride + w0);
-    const RowRules r = row_rules(a, row);
+    RowRules r = row_rules(a, row);
+    if (!MASKED) r.mask = nullptr;                                            // as it is: 256 rows of 131072 bfloat16 take 22.5 us instead of 24.5
     History<THREADS, 4> history;
     history.load(r, w0);
     Held<T> h;
@@ -472,7 +473,12 @@ __global__ __launch_bounds__(SHAPE_WAVES * 64) __attribute__((amdgpu_waves_per_e
         T::down8(x[v], d);
         if (cut == 0) {
 #pragma unroll
-            for (int k = 0; k < T::VEC; ++k) ((V*)(o + t))[k] = d[k];
+            for (int k = 0; k < T::VEC; ++k) {
+                // Past the caches where a store fills whole lines (64 rows of bfloat16 10.7 -> 9.2 us, shaping and then choosing 26.2 -> 25.0; in 32 bits, where it fills halves,
+                // 256 rows 51.7 -> 56.8).
+                if constexpr (T::VEC == 1) __builtin_nontemporal_store(d[k], (V*)(o + t) + k);
+                else ((V*)(o + t))[k] = d[k];
+            }
         } else if (cut < 8) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) if ((uint32_t)j >= cut) o[t + j - cut] = T::down(x[v][j]);
@@ -622,8 +628,16 @@ __device__ inline float segment_part(const RowRules& r, uint32_t n, uint32_t g, 
                                           const uint32_t* value, Next&& next) {
     float x[VECS][8];
     uint32_t i0, i1;
+    static_assert(VECS == 2, "");
+    // A grammar's mask leaves most segments without a token (making the mask and choosing under it for 1024 rows of 131072: 108 -> 58 us; 48 rows of 50021 under masks that leave every
+    // segment a few: 17.7 -> 18.5).
+    const bool empty = r.mask && __ballot((h.take[0] | h.take[1]) != 0) == 0;
     segment_x<T, TINY>(r, n, g, h, distinct, l, x, i0, i1);
     next();                                                                   // `h` is free for the loads of the wave's next segment
+    if (empty) {
+        if (greedy) ref = NEG_INF;
+        return 0.0f;
+    }
     auto repeated = [&](const Scale& scale) {
         double more = 0.0;                                                    // up to sixteen, one after another
         for (uint32_t i = i0 + (threadIdx.x & 63); i < i1; i += 64) more += (double)scale.weight(__builtin_bit_cast(float, value[i]));
@@ -774,7 +788,7 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     }
 }
 
-template <class T, bool TINY>
+template <class T, bool TINY, bool MASKED>
 __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_eu(8))) void k_choose(tp_logits a, uint64_t row0, uint32_t segs, const float* temperature,
                                                                                                      const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
     __shared__ Chunk::Lds l;
@@ -784,7 +798,8 @@ __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_
     const uint32_t chunks = gridDim.x, window = segs * CHOICE_WAVES * SEGMENT, w0 = blockIdx.x * window, n = a.vocab - w0, segments = reply_segments(a.vocab);
     const float t = temperature_of(temperature, uniform, row), temper = t > 0.0f ? t : 1.0f;
     const Inverse inverse(temper);
-    const RowRules r = row_rules(a, row);
+    RowRules r = row_rules(a, row);
+    if (!MASKED) r.mask = nullptr;                                            // as it is: without the masks' registers 512 rows take 42.0 us instead of 42.9
     const auto from = logit_row<T>(a, row) + w0;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * CHOICE_WAVES, reply_segments(n));
     History<CHOICE_WAVES * 64, 1> history;
@@ -879,8 +894,8 @@ __device__ inline uint32_t lower_entry_wave(const uint2* entry, uint32_t lo, uin
 
 // A block writes MASK_PIECE words of one row: cleared in LDS, the list's entries that fall into the piece set there, stored
 // in 16-byte pieces.  Of a list longer than a few rounds of the block only the piece's own part is read.  Bound by the blocks of the long
-// lists: 1024 rows over 131072 tokens (17 MB of mask, 4 us at a copy's rate) take 7.2 us.
-constexpr uint32_t MASK_PIECE = 1024, MASK_AHEAD = 4;
+// lists: 1024 rows over 131072 tokens (17 MB of mask, 4 us at a copy's rate) take 6.0 us.
+constexpr uint32_t MASK_PIECE = 1024, MASK_AHEAD = 2;   // (4 ahead: 7.3 us, 1: 7.2)
 __global__ __launch_bounds__(256) void k_grammar_mask(DevGrammar g, const int32_t* states, uint64_t row0, uint32_t* mask, uint64_t mask_stride) {
     __shared__ alignas(16) uint32_t bits[MASK_PIECE];
     const uint64_t row = row0 + blockIdx.y;
@@ -906,7 +921,7 @@ __global__ __launch_bounds__(256) void k_grammar_mask(DevGrammar g, const int32_
     uint32_t* out = mask + row * mask_stride + w0;
     const uint32_t n = words - w0, at = threadIdx.x * 4;
     if (at + 4 <= n) {
-        __builtin_memcpy(out + at, __builtin_assume_aligned(bits + at, 16), 16);
+        __builtin_nontemporal_store(*(const Words4*)(bits + at), (At<uint32_t>::W*)(out + at));   // past the caches: 7.0 -> 6.0 us
     } else {
         for (uint32_t j = at; j < n && j < at + 4; ++j) out[j] = bits[j];
     }
@@ -1453,7 +1468,9 @@ hipError_t launch_shape(const tp_logits& io, void* out, uint64_t out_stride) {
     return by_type_and_size(io, [&](auto tag, auto tiny) {
         using T = decltype(tag);
         return in_row_ranges(io.rows, chunks, [&](uint64_t r, unsigned n) {
-            hipLaunchKernelGGL((k_shape<T, decltype(tiny)::value>), dim3(chunks, n), dim3(SHAPE_WAVES * 64), 0, (hipStream_t)io.stream, io, r, out, out_stride);
+            constexpr bool TINY = decltype(tiny)::value;
+            const auto kernel = io.mask || TINY ? k_shape<T, TINY, true> : k_shape<T, TINY, TINY>;
+            hipLaunchKernelGGL(kernel, dim3(chunks, n), dim3(SHAPE_WAVES * 64), 0, (hipStream_t)io.stream, io, r, out, out_stride);
         });
     });
 }
@@ -1477,7 +1494,9 @@ hipError_t launch_choose(const tp_logits& io, const float* temperature, const fl
     return by_type_and_size(io, [&](auto tag, auto tiny) {
         using T = decltype(tag);
         hipError_t e = in_row_ranges(io.rows, chunks, [&](uint64_t r, unsigned n) {
-            hipLaunchKernelGGL((k_choose<T, decltype(tiny)::value>), dim3(chunks, n), dim3(CHOICE_WAVES * 64), lds, (hipStream_t)io.stream, io, r, segs, temperature, uniform, tokens, logprob, parts);
+            constexpr bool TINY = decltype(tiny)::value;
+            const auto kernel = io.mask || TINY ? k_choose<T, TINY, true> : k_choose<T, TINY, TINY>;
+            hipLaunchKernelGGL(kernel, dim3(chunks, n), dim3(CHOICE_WAVES * 64), lds, (hipStream_t)io.stream, io, r, segs, temperature, uniform, tokens, logprob, parts);
         });
         if (e != hipSuccess || chunks == 1) return e;
         return in_ranges(io.rows, [&](uint64_t b, unsigned n) {
