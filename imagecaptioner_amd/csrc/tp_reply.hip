@@ -1527,8 +1527,8 @@ hipError_t launch_grammar_step(const DevGrammar& g, const tp_logits& io, const f
 }
 
 // The lengths in LDS: up to 64 KB of them, so that two blocks share a compute unit, and where there are blocks for every unit and tokens enough to pay for the table.
-// Without / with it, of 131072 tokens: 8192 rows of up to 300 tokens 9.5 / 6.1 us, of 128 5.9 / 6.1; 4096 rows of 300 6.2 / 5.2, 2048 rows 5.1 / 4.8 at 300 and
-// 3.9 / 4.8 at 128; of 32768 tokens: 8192 rows of 300 5.5 / 4.7, of 128 4.4 / 4.6.
+// Without / with it, us a pass, of 131072 tokens: 8192 rows of 300 tokens 22.9 / 19.9, of 192 16.4 / 15.3, of 128 13.8 / 13.7; 4096 rows of 300 15.5 / 14.4, of 128
+// 10.5 / 10.8; 2048 rows of 300 13.0 / 12.7; of 32768 tokens: 8192 rows of 300 19.4 / 18.1, of 128 12.3 / 12.4.
 static bool line_sizes_by_table(const DevGrammar& g, uint64_t rows, uint32_t width) {
     return g.n_tokens <= 131072 && rows >= 256 * LINE_ROWS && width >= 192;
 }
