@@ -504,9 +504,10 @@ int tp_format_review_rows(const tp_ctx* ctx, const tp_result* res, int format, c
  * Conventions.  Every pointer in these structs and argument lists is a device pointer on the context's device unless
  * it is said to be host memory.  Work is enqueued on `stream` (a hipStream_t, NULL = default stream); no call
  * allocates, copies to the host or waits, so all but tp_grammar_create may be captured into a HIP graph.  The caller's
- * current device is left as it was.  Equal arguments give equal bits, call after call.  A workspace holds nothing between calls and needs no initial contents, but calls that may
- * overlap (two streams, two graphs replayed at once) need one each.  Outputs must not overlap inputs except where a
- * call says so.  Zero rows: nothing is done.  A grammar does not refer to the context it was made from.
+ * current device is left as it was.  Equal arguments give equal bits, call after call.  A workspace holds nothing
+ * between calls and needs no initial contents, but calls that may overlap (two streams, two graphs replayed at once)
+ * need one each.  Outputs must not overlap inputs except where a call says so.  Zero rows: nothing is done.  A grammar
+ * does not refer to the context it was made from.
  */
 #define TP_T_F32  0
 #define TP_T_F16  1
@@ -553,12 +554,14 @@ int tp_shape_logits(tp_ctx* ctx, const tp_logits* io, void* out, uint64_t out_st
 
 /*
  * The token of every row.  z = x / temperature[r] where temperature[r] > 0, else z = x.  Without a temperature (NULL
- * array, 0, negative, NaN) the token is the largest x, ties to the lowest token.  With one it is the lowest token whose
- * cumulative weight exceeds uniform[r] * (the sum of all weights), weights exp(z - max z) in token order; uniform[r] in
- * [0, 1), NULL: as temperature NULL.  Values of uniform outside [0, 1) give the first or last token of a weight above 0.
- * z and the weights are 32-bit numbers; the weights are summed 16 at a time in 32 bits and in 64 from there on.  A z of NaN counts as -infinity.  Where +infinity stands, the tokens that have it share the weight.
- * logprob[r] = z - max z - ln(sum of weights) of the chosen token.  A row without a z above -infinity gets token -1 and
- * log-probability -infinity.  logprob may be NULL.  workspace: tp_choose_workspace bytes (host function), aligned to 16.
+ * array, 0, negative, NaN) the token is the largest x, ties to the lowest token.  With one it is the lowest token
+ * whose cumulative weight exceeds uniform[r] * (the sum of all weights), weights exp(z - max z) in token order;
+ * uniform[r] in [0, 1), NULL: as temperature NULL.  Values of uniform outside [0, 1) give the first or last token of a
+ * weight above 0. z and the weights are 32-bit numbers; the weights are summed 16 at a time in 32 bits and in 64 from
+ * there on.  A z of NaN counts as -infinity.  Where +infinity stands, the tokens that have it share the weight.
+ * logprob[r] = z - max z - ln(sum of weights) of the chosen token.  A row without a z above -infinity gets token -1
+ * and log-probability -infinity.  logprob may be NULL.  workspace: tp_choose_workspace bytes (host function), aligned
+ * to 16.
  */
 uint64_t tp_choose_workspace(uint64_t rows, uint32_t vocab);
 int tp_choose_tokens(tp_ctx* ctx, const tp_logits* io, const float* temperature, const float* uniform, int32_t* tokens, float* logprob,
@@ -620,9 +623,10 @@ int tp_grammar_step(const tp_grammar* g, const tp_logits* io, const float* tempe
 /*
  * The texts of rows of tokens, back to back: row r's is arena[offsets[r] .. offsets[r + 1]).  Row r's tokens are
  * tokens[r * stride + k], from begin[r] (NULL: 0) to below len[r] (NULL: width; both taken as 0 below 0 and as width
- * above it); one outside [0, n_tokens) has no text.  A row's text must stay below 4 GiB.  Nothing is written at or behind
- * `capacity`: offsets[rows] is the size needed, and a caller that cannot bound it compares the two.  16 zero bytes behind
- * the last text are written where they fit, so that the arena can go to tp_run_lines_device as it is.  workspace: tp_lines_workspace bytes (host function), aligned to 16.
+ * above it); one outside [0, n_tokens) has no text.  A row's text must stay below 4 GiB.  Nothing is written at or
+ * behind `capacity`: offsets[rows] is the size needed, and a caller that cannot bound it compares the two.  16 zero
+ * bytes behind the last text are written where they fit, so that the arena can go to tp_run_lines_device as it is.
+ * workspace: tp_lines_workspace bytes (host function), aligned to 16.
  */
 uint64_t tp_lines_workspace(uint64_t rows);
 int tp_grammar_lines(const tp_grammar* g, const int32_t* tokens, uint64_t stride, uint32_t width, const int32_t* begin, const int32_t* len, uint64_t rows,
