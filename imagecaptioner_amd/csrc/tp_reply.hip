@@ -195,12 +195,13 @@ __device__ inline double eight_lanes_sum(double v) {
 // hundred-thousandth of the weight, and unrounded quotients chose another token than the rounded ones in one row of 700.
 // A token's weight is 2^(z * LOG2E - c), c = best * LOG2E rounded once for the tokens that are summed together: one fused multiply-add and one power.  c is no
 // more than a common scale, known exactly to whoever joins sums of different c, so that a weight is off by LOG2E's rounding and the fma's, each half a step
-// relative in the exponent, and by the power's own step.  Where c overflows, neighbouring numbers already lie so far apart that only the largest z weighs anything.
+// relative in the exponent, and by the power's own step.  From |c| = 2^30 on, neighbouring numbers lie so far apart that only the largest z weighs anything, and c's own rounding
+// (32 at the most below it) would grow out of the powers' range.
 constexpr float LOG2E = 1.44269504088896341f;
 struct Scale {
     float c, best;
     bool equal;                   // weigh by equality with the largest
-    __device__ Scale(float best_) : c(best_ * LOG2E), best(best_), equal(!(fabsf(best_ * LOG2E) < __builtin_inff())) {}
+    __device__ Scale(float best_) : c(best_ * LOG2E), best(best_), equal(!(fabsf(best_ * LOG2E) < 0x1p30f)) {}
     __device__ float weight(float z) const { return equal ? (z == best ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f(__builtin_fmaf(z, LOG2E, -c)); }
     // what a sum of the weights of another scale counts for in this one's
     __device__ double of(float other_best) const { return equal || !(other_best > NEG_INF) ? (other_best == best ? 1.0 : 0.0) : (double)__builtin_amdgcn_exp2f(other_best * LOG2E - c); }

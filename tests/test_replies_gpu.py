@@ -276,6 +276,61 @@ def test_choose_ties_and_specials(pipe, vocab):
     assert token.tolist() == [0, 0, int(0.5 * vocab), vocab - 1]        # cumulative weights k + 1 > u * vocab: exact in 64 bits
 
 
+@pytest.mark.parametrize("vocab", [7, 4000, 140000])
+def test_extreme_temperatures(pipe, vocab):
+    """z = x / T in 32 bits: far above 1 every token weighs the same, far below the largest x is alone, and where the quotients overflow those that do share the weight."""
+    rng = np.random.default_rng(vocab)
+    l = rng.permutation(vocab).astype(np.float32) / 64 + 1.0
+    l[rng.random(vocab) < 0.3] *= -1
+    flat, sharp, over = [1e29, 1e31, 3e38, np.inf], [1e-29, 1e-31, 1e-33], [1e-40, 2e-45]
+    temperature = np.array(flat + sharp + over, np.float32)
+    uniform = rng.random(len(temperature)).astype(np.float32)
+    rows = len(temperature)
+    logits = dev(np.repeat(l[None], rows, 0))
+    for rules, left in ((dict(), np.ones(vocab, bool)), (dict(mask=dev(np.packbits(np.pad(np.arange(vocab) % 3 == 1, (0, -vocab % 32)), bitorder="little").view(np.int32)[None])), np.arange(vocab) % 3 == 1)):
+        token, logprob = pipe.choose_tokens(logits, temperature=dev(temperature), uniform=dev(uniform), **rules)
+        at = np.nonzero(left)[0]
+        up = np.nonzero(left & (l > 0))[0]
+        for r in range(rows):
+            of = at if r < len(flat) else up if r >= len(flat) + len(sharp) else [at[np.argmax(l[at])]]
+            k = int(np.searchsorted(of, int(token[r])))
+            assert of[k] == int(token[r]) and abs(k - float(uniform[r]) * len(of)) <= 1, (r, int(token[r]))       # cumulative weights are whole numbers: exact
+            assert abs(float(logprob[r]) + math.log(len(of))) <= 2 * HALF32 * math.log(max(len(of), 2)), r
+
+
+@pytest.mark.parametrize("vocab", [7, 4000, 140000])
+def test_large_logits(pipe, vocab):
+    """Whole multiples of every size of unit, which no operation before the weights rounds."""
+    rng = np.random.default_rng(vocab)
+    units = [2.0 ** p for p in (-3, 0, 5, 10, 16, 20, 23, 24, 26, 28, 29, 30, 31, 40, 64, 100, 120)]
+    l = np.concatenate([rng.integers(lo, hi, (len(units), vocab)) * np.array(units)[:, None] for lo, hi in ((-6, 7), (100, 108), (-108, -100))])
+    rows = len(l)
+    temperature, uniform = np.where(np.arange(rows) % 2, 1.0, 0.5).astype(np.float32), rng.random(rows).astype(np.float32)
+    token, logprob = (v.cpu().numpy() for v in pipe.choose_tokens(dev(l, torch.float32), temperature=dev(temperature), uniform=dev(uniform)))
+    assert np.isfinite(logprob).all()
+    check_choice(token, logprob, list(l), [np.zeros(vocab)] * rows, temperature, uniform)
+
+
+@pytest.mark.parametrize("name", sorted(TYPES))
+@pytest.mark.parametrize("rows,vocab", [(40, 50021), (3, 300001), (260, 140000)])
+def test_choose_under_masks_that_empty_segments(pipe, name, rows, vocab):
+    rng = np.random.default_rng(rows)
+    logits, l = make_logits(rng, rows, vocab, TYPES[name])
+    rules = Rules(rng, rows, vocab, history=60, bias=1, mask=5, density=2e-4)
+    allowed = bits_of(rules.mask[0], vocab).nonzero()[0]
+    rules.history[:, ::4] = rng.choice(allowed, size=rules.history[:, ::4].shape)                                  # repeated and allowed
+    rules.mask[1], rules.mask[2] = 0, 0
+    rules.mask[1, -1] = 1                                                 # one token near the end, in a segment behind empty ones
+    rules.mask[2, 3] = 1 << 7
+    rules.args.update(history=dev(rules.history), mask=dev(rules.mask))
+    temperature, uniform = choice_numbers(rng, rows)
+    some = list(range(rows)) if rows < 100 else list(range(0, rows, 20))
+    for tu in (dict(temperature=dev(temperature), uniform=dev(uniform)), dict()):
+        token, logprob = (v.cpu().numpy() for v in pipe.choose_tokens(logits, **tu, **rules.args))
+        xs, sizes, _ = zip(*(rules.plain(l[r], r) for r in some))
+        check_choice(token[some], logprob[some], xs, sizes, temperature[some] if tu else None, uniform[some] if tu else None)
+
+
 @pytest.mark.parametrize("name", sorted(TYPES))
 def test_signalling_nans(pipe, name):
     """NaNs of either kind among the logits, in every position of a lane's eight, hide no larger number beside them."""
@@ -484,6 +539,19 @@ def test_grammar_step_on_long_lists(wide_grammar):
         rules = Rules(rng, len(states), len(tokens), **kw)
         check_step(g, plain, tokens, states, "bf16", rules, l, logits, temperature, uniform)
         check_step(g, plain, tokens, states, "bf16", rules, l, logits, None, None)
+
+
+def test_grammar_step_of_large_logits(pipe, wide_grammar):
+    for g, plain, tokens in (small_grammar(pipe), wide_grammar):
+        rng = np.random.default_rng(29)
+        units = np.array([2.0 ** p for p in (-3, 0, 10, 24, 29, 30, 64, 120)])
+        states = np.zeros((len(units), 2), np.int32)
+        l = rng.integers(100, 108, (len(units), len(tokens))) * units[:, None]
+        temperature, uniform = np.ones(len(units), np.float32), rng.random(len(units)).astype(np.float32)
+        rules = Rules(rng, len(units), len(tokens))
+        token, logprob = (v.cpu().numpy() for v in g.step(dev(states), dev(l, torch.float32), temperature=dev(temperature), uniform=dev(uniform)))
+        allowed = plain.allowed((0, 0))
+        check_choice(token, logprob, [np.where(allowed, x, -np.inf) for x in l], [np.zeros(len(tokens))] * len(units), temperature, uniform)
 
 
 def test_step_is_choose_under_the_grammars_mask(pipe, wide_grammar):
