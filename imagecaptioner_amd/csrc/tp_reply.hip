@@ -1479,7 +1479,8 @@ hipError_t launch_shape(const tp_logits& io, void* out, uint64_t out_stride) {
 // Segments a wave of the choice takes, one after another.  Where a window holds the row (131072 tokens) its history is read once and
 // no second launch joins it: taken for rows of up to 64 segments, and where there are rows for every compute unit.  A unit works on a segment for
 // about 0.15 us, though, and fewer long rows than units leave the others idle (one row of 131072: 22 us in one block, 7 + 7 in eight and the join): they are split.
-// (48 rows of 50021, 49 segments: 17.5 us a pass in a block each, 19.4 in four and the join.)
+// (A block each / in blocks of 16 segments and the join, us a pass: one row of 32768 12.4 / 14.5, of 50021 14.6 / 14.8, of 65536 15.6 / 14.7; 48 rows of 50021 17.3 / 17.1,
+// 128 17.2 / 19.3, 200 of 32768 14.0 / 20.1.)
 // A window must also keep its repeated tokens in 64 KB of LDS.
 static uint32_t window_segments(const tp_logits& io) {
     uint32_t segs = 1;
