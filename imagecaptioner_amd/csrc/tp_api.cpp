@@ -1899,6 +1899,7 @@ tp_grammar* tp_grammar_create(tp_ctx* ctx, const tp_grammar_config* cfg) {
         g->dev.n_places = h.info.n_prefixes + 2;
         g->dev.min_tags = h.min_tags;
         g->dev.max_tags = h.max_tags;
+        g->dev.longest_list = h.info.longest_list;
         made = g.release();
         return (int)TP_OK;
     });

@@ -21,7 +21,7 @@ struct DevGrammar {
                                   //   `text`, its bytes, and LONG_TOKEN in the last byte
     const uint8_t* text;          // the tokens' bytes, and eight behind them
     uint32_t n_tokens, n_places;  // places 0 .. n_places - 1 (the end among them)
-    uint32_t min_tags, max_tags;
+    uint32_t min_tags, max_tags, longest_list;
 };
 
 // Loads the kernels' code on the current device, so that the first call of one may already be a captured one.

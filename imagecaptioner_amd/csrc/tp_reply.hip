@@ -946,8 +946,8 @@ __device__ inline bool has_room(const tp_logits& a, uint64_t row, int append) { 
 // THREADS * EACH.  Only the listed tokens' logits are read.  The history goes through a hash table in LDS, a part of THREADS * RECALL entries at a time,
 // in which every entry of the list looks its token up.  (Looking every history token up in the sorted list takes a binary search of
 // dependent LDS reads: 3.4 of the 8.5 us that a list of 4781 took.)  A list longer than THREADS * EACH is worked on in pieces,
-// twice: for the largest x and the sum, and for the place.
-template <int THREADS, int EACH, int RECALL>
+// twice: for the largest x and the sum, and for the place.  ONE: there is none.
+template <int THREADS, int EACH, int RECALL, bool ONE>
 struct Step {
     static constexpr uint32_t PIECE = THREADS * EACH;
     static constexpr int WAVES = THREADS / 64, SEGMENTS = WAVES * EACH;      // a wave's 64 entries of one round are a segment, in token order
@@ -1086,7 +1086,7 @@ struct Step {
     static __device__ void run(const DevGrammar& g, const tp_logits& a, const RowRules& r, uint64_t row, const List& q, const float* temperature, const float* uniform, int32_t* states,
                                int32_t* tokens, float* logprob, int append, Lds& s) {
         const float t = temperature_of(temperature, uniform, row), temper = t > 0.0f ? t : 1.0f;
-        const bool one = q.hi - q.lo <= PIECE, room = has_room(a, row, append);
+        const bool one = ONE || q.hi - q.lo <= PIECE, room = has_room(a, row, append);
         const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
         uint2 en[EACH];
         float x[EACH], best = NEG_INF;
@@ -1177,21 +1177,23 @@ struct Step {
 // is the work of one wave, which needs no barrier, and the block's other waves are done at once.  Bound by latency: 256 rows over
 // 131072 tokens and lists of up to 4781 take 15.5 us, of which the bytes (1.3 MB, 0.3 us) are next to nothing; rules and list, entries, their
 // logits, the sums and the choice each wait for what comes before.
-constexpr int STEP_THREADS = 1024;
-using LongStep = Step<STEP_THREADS, 8, 1>;
-using ShortStep = Step<64, 1, 4>;
+// The block is as large as the grammar's longest list asks for: 256 threads up to 2048 entries, 512 up to 4096, 1024 beyond.  A unit holds as many more rows, and a row's start
+// costs fewer idle waves: 4096 rows with lists of up to 759 take 22.6 us in 256 threads, 39.0 in 512, 89.8 in 1024, up to 2259 47.4 in 512 and 102 in 1024 (and 43.9 in
+// 256, in two pieces, but 256 rows 19.0 instead of 11.4).
+using ShortStep = Step<64, 1, 4, true>;
 
-template <class T>
-__global__ __launch_bounds__(STEP_THREADS) void k_grammar_step(DevGrammar g, tp_logits a, uint64_t row0, const float* temperature, const float* uniform,
+template <class T, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_grammar_step(DevGrammar g, tp_logits a, uint64_t row0, const float* temperature, const float* uniform,
                                                                int32_t* states, int32_t* tokens, float* logprob, int append) {
-    __shared__ union { LongStep::Lds l; ShortStep::Lds s; } lds;
+    using LongStep = Step<THREADS, 8, 1024 / THREADS, THREADS < 1024>;
+    __shared__ union { typename LongStep::Lds l; ShortStep::Lds s; } lds;
     const uint64_t row = row0 + blockIdx.x;
     const RowRules r = row_rules(a, row);
     const List q = list_of(g, states, row);
     const bool many = q.hi - q.lo > ShortStep::PIECE;
     __syncthreads();                                                         // every wave has read the state before one moves it
     if (many) {
-        LongStep::run<T>(g, a, r, row, q, temperature, uniform, states, tokens, logprob, append, lds.l);
+        LongStep::template run<T>(g, a, r, row, q, temperature, uniform, states, tokens, logprob, append, lds.l);
     } else if (threadIdx.x < 64) {
         ShortStep::run<T>(g, a, r, row, q, temperature, uniform, states, tokens, logprob, append, lds.s);
     }
@@ -1523,7 +1525,9 @@ hipError_t launch_grammar_step(const DevGrammar& g, const tp_logits& io, const f
     return by_type(io.type, [&](auto tag) {
         using T = decltype(tag);
         return in_ranges(io.rows, [&](uint64_t b, unsigned n) {
-            hipLaunchKernelGGL(k_grammar_step<T>, dim3(n), dim3(STEP_THREADS), 0, (hipStream_t)io.stream, g, io, b, temperature, uniform, states, tokens, logprob, append);
+            const int threads = g.longest_list <= 2048 ? 256 : g.longest_list <= 4096 ? 512 : 1024;
+            const auto kernel = threads == 256 ? k_grammar_step<T, 256> : threads == 512 ? k_grammar_step<T, 512> : k_grammar_step<T, 1024>;
+            hipLaunchKernelGGL(kernel, dim3(n), dim3(threads), 0, (hipStream_t)io.stream, g, io, b, temperature, uniform, states, tokens, logprob, append);
         });
     });
 }

@@ -541,6 +541,21 @@ def test_grammar_step_on_long_lists(wide_grammar):
         check_step(g, plain, tokens, states, "bf16", rules, l, logits, None, None)
 
 
+@pytest.mark.parametrize("count,lo,hi", [(800, 1500, 2048), (1800, 2049, 4096), (3500, 4097, 8192)])
+def test_grammar_step_by_the_longest_list(pipe, count, lo, hi):
+    g, plain, tokens = words_grammar(pipe, count, 20011)
+    assert lo <= g.info.longest_list <= hi, g.info.longest_list
+    rng = np.random.default_rng(count)
+    states = np.array([(0, 0)] * 9 + [(plain.after_comma, 2), (plain.place[plain.tags[11]], 4), (0, 41), (plain.place[plain.tags[5][:1]], 3)], np.int32)
+    logits, l = make_logits(rng, len(states), len(tokens), torch.float16, scale=1.0)
+    temperature, uniform = choice_numbers(rng, len(states))
+    uniform[3:9], temperature[3:9] = [0.1, 0.3, 0.5, 0.7, 0.9, 1.5], 1.2
+    for kw in (dict(), dict(history=1300, bias=1)):                       # 1024 entries of history go into a table at once
+        rules = Rules(rng, len(states), len(tokens), **kw)
+        check_step(g, plain, tokens, states, "f16", rules, l, logits, temperature, uniform)
+        check_step(g, plain, tokens, states, "f16", rules, l, logits, None, None)
+
+
 def test_grammar_step_of_large_logits(pipe, wide_grammar):
     for g, plain, tokens in (small_grammar(pipe), wide_grammar):
         rng = np.random.default_rng(29)
