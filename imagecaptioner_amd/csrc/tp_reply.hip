@@ -584,11 +584,12 @@ struct Window {
 // the row (4 us) are chains of latency that no other block hides, since all rows are at work at once.
 using OneSegment = Window<1, 1>;
 constexpr int CHOICE_WAVES = 16, MOST_SEGS = 8;                               // waves of a block, segments of a wave at the most
-using Chunk = Window<CHOICE_WAVES, MOST_SEGS>;
+// Waves of a block where a row has no more segments: 4096 rows of 1000 tokens 80.3 -> 28.7 us a pass, of 4096 82.7 -> 38.2, 512 rows of 4096 12.7 -> 11.6, one row 9.9 -> 10.0.
+constexpr int FEW_WAVES = 4;
 
 // x of a segment without its repeated tokens, which are value[i0 .. i1)
-template <class T, bool TINY>
-__device__ inline void segment_x(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, uint32_t distinct, const Chunk::Lds& l, float (&x)[VECS][8], uint32_t& i0, uint32_t& i1) {
+template <class T, bool TINY, class Lds>
+__device__ inline void segment_x(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, uint32_t distinct, const Lds& l, float (&x)[VECS][8], uint32_t& i0, uint32_t& i1) {
     uint32_t take[VECS];
     i0 = i1 = 0;
 #pragma unroll
@@ -624,8 +625,8 @@ __device__ inline float segment_largest(const float (&x)[VECS][8], float temper,
 // the segment's own largest z, which is the wave's `ref` from then on: the shares that the join works with do not mind what they are
 // relative to, and the largest need not be found.  With `greedy` it is the segment's largest in any case.
 // A NaN among the weights has the segment done again, by divisions and without the NaNs.
-template <class T, bool TINY, class Next>
-__device__ inline float segment_part(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, float temper, const Inverse& inverse, bool greedy, float& ref, uint32_t distinct, const Chunk::Lds& l,
+template <class T, bool TINY, class Lds, class Next>
+__device__ inline float segment_part(const RowRules& r, uint32_t n, uint32_t g, const Held<T>& h, float temper, const Inverse& inverse, bool greedy, float& ref, uint32_t distinct, const Lds& l,
                                           const uint32_t* value, Next&& next) {
     float x[VECS][8];
     uint32_t i0, i1;
@@ -789,28 +790,30 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
     }
 }
 
-template <class T, bool TINY, bool MASKED>
-__global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_eu(8))) void k_choose(tp_logits a, uint64_t row0, uint32_t segs, const float* temperature,
-                                                                                                     const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
-    __shared__ Chunk::Lds l;
-    __shared__ ChoicePart here[CHOICE_WAVES * MOST_SEGS];
-    __shared__ float largest[CHOICE_WAVES];
+template <class T, bool TINY, bool MASKED, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(8))) void k_choose(tp_logits a, uint64_t row0, uint32_t segs, const float* temperature,
+                                                                                              const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
+    constexpr int SEGS = WAVES == CHOICE_WAVES ? MOST_SEGS : 1;
+    using Chunk = Window<WAVES, SEGS>;
+    __shared__ typename Chunk::Lds l;
+    __shared__ ChoicePart here[WAVES * SEGS];
+    __shared__ float largest[WAVES];
     const uint64_t row = row0 + blockIdx.y;
-    const uint32_t chunks = gridDim.x, window = segs * CHOICE_WAVES * SEGMENT, w0 = blockIdx.x * window, n = a.vocab - w0, segments = reply_segments(a.vocab);
+    const uint32_t chunks = gridDim.x, window = segs * WAVES * SEGMENT, w0 = blockIdx.x * window, n = a.vocab - w0, segments = reply_segments(a.vocab);
     const float t = temperature_of(temperature, uniform, row), temper = t > 0.0f ? t : 1.0f;
     const Inverse inverse(temper);
     RowRules r = row_rules(a, row);
     if (!MASKED) r.mask = nullptr;                                            // as it is: without the masks' registers 512 rows take 42.0 us instead of 42.9
     const auto from = logit_row<T>(a, row) + w0;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * CHOICE_WAVES, reply_segments(n));
-    History<CHOICE_WAVES * 64, 1> history;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * WAVES, reply_segments(n));
+    History<WAVES * 64, CHOICE_WAVES / WAVES> history;
     history.load(r, w0);
     Held<T> h;
     uint32_t bits[VECS];
     load_mask(r, w0, n, wave, bits);
     if (wave < last) load_segment<T, TINY, true>(r, from, w0, n, wave, bits, h);
-    load_mask(r, w0, n, wave + CHOICE_WAVES, bits);
-    const uint32_t distinct = Chunk::repeated<T>(r, temper, history, from, w0, std::min(n, window), l, dynamic_lds);
+    load_mask(r, w0, n, wave + WAVES, bits);
+    const uint32_t distinct = Chunk::template repeated<T>(r, temper, history, from, w0, std::min(n, window), l, dynamic_lds);
     ChoicePart* out = parts + row * segments + w0 / SEGMENT;
     float ref = NEG_INF;
     if (t > 0.0f) {                                                           // the largest of the waves' first segments, a number near the row's largest: small exponents round less
@@ -822,12 +825,12 @@ __global__ __launch_bounds__(CHOICE_WAVES * 64) __attribute__((amdgpu_waves_per_
         }
         if ((threadIdx.x & 63) == 0) largest[wave] = ref;
         __syncthreads();
-        ref = wave_max(largest[threadIdx.x % CHOICE_WAVES]);
+        ref = wave_max(largest[threadIdx.x % WAVES]);
     }
-    for (uint32_t g = wave; g < last; g += CHOICE_WAVES) {
+    for (uint32_t g = wave; g < last; g += WAVES) {
         const float sum = segment_part<T, TINY>(r, n, g, h, temper, inverse, t == 0.0f, ref, distinct, l, dynamic_lds, [&] {
-            if (g + CHOICE_WAVES < last) load_segment<T, TINY, true>(r, from, w0, n, g + CHOICE_WAVES, bits, h);
-            load_mask(r, w0, n, g + 2 * CHOICE_WAVES, bits);
+            if (g + WAVES < last) load_segment<T, TINY, true>(r, from, w0, n, g + WAVES, bits, h);
+            load_mask(r, w0, n, g + 2 * WAVES, bits);
         });
         l.lane_sum[g * 64 + (threadIdx.x & 63)] = sum;
         if ((threadIdx.x & 63) == 0) here[g].best = ref;
@@ -1493,14 +1496,18 @@ static uint32_t window_segments(const tp_logits& io) {
 }
 
 hipError_t launch_choose(const tp_logits& io, const float* temperature, const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
-    const uint32_t segs = window_segments(io), window = segs * CHOICE_WAVES * SEGMENT, chunks = (io.vocab + window - 1) / window;
+    const bool few = reply_segments(io.vocab) <= FEW_WAVES;
+    const uint32_t segs = few ? 1 : window_segments(io), window = segs * (few ? FEW_WAVES : CHOICE_WAVES) * SEGMENT, chunks = (io.vocab + window - 1) / window;
     const uint32_t lds = io.history ? std::min(io.history_cap, window) * 4 : 0, lds_one = io.history ? std::min(io.history_cap, SEGMENT) * 4 : 0;
     return by_type_and_size(io, [&](auto tag, auto tiny) {
         using T = decltype(tag);
         hipError_t e = in_row_ranges(io.rows, chunks, [&](uint64_t r, unsigned n) {
-            constexpr bool TINY = decltype(tiny)::value;
-            const auto kernel = io.mask || TINY ? k_choose<T, TINY, true> : k_choose<T, TINY, TINY>;
-            hipLaunchKernelGGL(kernel, dim3(chunks, n), dim3(CHOICE_WAVES * 64), lds, (hipStream_t)io.stream, io, r, segs, temperature, uniform, tokens, logprob, parts);
+            auto launch = [&](auto kernel, int waves) {
+                hipLaunchKernelGGL(kernel, dim3(chunks, n), dim3(waves * 64), lds, (hipStream_t)io.stream, io, r, segs, temperature, uniform, tokens, logprob, parts);
+            };
+            if constexpr (decltype(tiny)::value) launch(k_choose<T, true, true, FEW_WAVES>, FEW_WAVES);
+            else if (few) launch(io.mask ? k_choose<T, false, true, FEW_WAVES> : k_choose<T, false, false, FEW_WAVES>, FEW_WAVES);
+            else launch(io.mask ? k_choose<T, false, true, CHOICE_WAVES> : k_choose<T, false, false, CHOICE_WAVES>, CHOICE_WAVES);
         });
         if (e != hipSuccess || chunks == 1) return e;
         return in_ranges(io.rows, [&](uint64_t b, unsigned n) {

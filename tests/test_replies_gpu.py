@@ -197,7 +197,7 @@ def check_choice(token, logprob, xs, sizes, temperature, uniform):
         assert abs(lp - want) <= 2 * e + 2 * share + 2 * HALF32 * abs(want), (r, lp, want)
 
 
-@pytest.mark.parametrize("rows,vocab", [(2, 50021), (3, 9000), (1, 200001), (520, 17000)])
+@pytest.mark.parametrize("rows,vocab", [(2, 50021), (3, 9000), (5, 3000), (1, 200001), (520, 17000)])
 def test_long_histories(pipe, rows, vocab):
     """More history than a launch keeps of it at once, most of it distinct."""
     rng = np.random.default_rng(rows)
