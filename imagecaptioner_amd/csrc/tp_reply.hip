@@ -579,13 +579,17 @@ struct Window {
 // 32 bits (five roundings, one more where repeated tokens are among them), everything above in 64.  Against the formula with 64-bit sums, 131072 tokens and temperatures
 // of 0.5 .. 1.2, one row of 5000 got another token, always the border's other side.
 //
-// What bounds it: 512 rows of 131072 bfloat16 (134 MB, 26 us at a copy's rate) with 256 tokens of history and a bias take 45 us: the vector units
+// What bounds it: 512 rows of 131072 bfloat16 (134 MB, 26 us at a copy's rate) with 256 tokens of history and a bias take 41 us: the vector units
 // spend some 260 instructions a segment (powers: 16, four times as long), 29 us of work; the block's start (rules, history and repeated tokens: 6 us) and the join of
 // the row (4 us) are chains of latency that no other block hides, since all rows are at work at once.
 using OneSegment = Window<1, 1>;
-constexpr int CHOICE_WAVES = 16, MOST_SEGS = 8;                               // waves of a block, segments of a wave at the most
-// Waves of a block where a row has no more segments: 4096 rows of 1000 tokens 80.3 -> 28.7 us a pass, of 4096 82.7 -> 38.2, 512 rows of 4096 12.7 -> 11.6, one row 9.9 -> 10.0.
-constexpr int FEW_WAVES = 4;
+// A block has eight waves of up to 16 segments.  Two blocks share a unit, for their LDS, and so a wave may have 128 registers: with sixteen waves of 64, which had to
+// store some of them and copied others, 512 rows of 131072 took 42.0 us instead of 41.1, 48 rows of 50021 under masks 18.5 instead of 17.5, one row of 131072 13.9 instead of 12.8.
+// Where there are more rows than units and they have up to 16 segments, blocks of four waves: more rows at work at once hide each other's start and join (sixteen waves / four:
+// 4096 rows of 16384 115 / 49 us, 512 of 8000 13.8 / 11.7; with eight waves 300 rows of 16384 14.2 / 13.5, 256 rows 11.6 / 12.1).  So they are for up to four
+// segments in any case: the other waves would have nothing to do.
+constexpr int CHOICE_WAVES = 8, MOST_SEGS = 16;                               // waves of a block, segments of a wave at the most
+constexpr int FEW_WAVES = 4, FEW_SEGS = 4;
 
 // x of a segment without its repeated tokens, which are value[i0 .. i1)
 template <class T, bool TINY, class Lds>
@@ -791,9 +795,9 @@ __device__ void join_row(const tp_logits& a, const RowRules& r, uint64_t row, ui
 }
 
 template <class T, bool TINY, bool MASKED, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(8))) void k_choose(tp_logits a, uint64_t row0, uint32_t segs, const float* temperature,
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(4))) void k_choose(tp_logits a, uint64_t row0, uint32_t segs, const float* temperature,
                                                                                               const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
-    constexpr int SEGS = WAVES == CHOICE_WAVES ? MOST_SEGS : 1;
+    constexpr int SEGS = WAVES == CHOICE_WAVES ? MOST_SEGS : FEW_SEGS;
     using Chunk = Window<WAVES, SEGS>;
     __shared__ typename Chunk::Lds l;
     __shared__ ChoicePart here[WAVES * SEGS];
@@ -806,7 +810,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(8)))
     if (!MASKED) r.mask = nullptr;                                            // as it is: without the masks' registers 512 rows take 42.0 us instead of 42.9
     const auto from = logit_row<T>(a, row) + w0;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), last = std::min(segs * WAVES, reply_segments(n));
-    History<WAVES * 64, CHOICE_WAVES / WAVES> history;
+    History<WAVES * 64, 16 / WAVES> history;
     history.load(r, w0);
     Held<T> h;
     uint32_t bits[VECS];
@@ -836,11 +840,11 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(8)))
         if ((threadIdx.x & 63) == 0) here[g].best = ref;
     }
     __syncthreads();
-    if (threadIdx.x < last * 8) {                                             // eight threads a segment
-        const float4 a0 = *(const float4*)(l.lane_sum + threadIdx.x * 8), a1 = *(const float4*)(l.lane_sum + threadIdx.x * 8 + 4);
+    for (uint32_t i = threadIdx.x; i < last * 8; i += WAVES * 64) {           // eight threads a segment
+        const float4 a0 = *(const float4*)(l.lane_sum + i * 8), a1 = *(const float4*)(l.lane_sum + i * 8 + 4);
         const double sum = eight_lanes_sum((((double)a0.x + a0.y) + ((double)a0.z + a0.w)) + (((double)a1.x + a1.y) + ((double)a1.z + a1.w)));
-        if (threadIdx.x % 8 == 7) {
-            const uint32_t g = threadIdx.x / 8;
+        if (i % 8 == 7) {
+            const uint32_t g = i / 8;
             if (chunks > 1) out[g] = ChoicePart{sum, here[g].best}; else here[g].sum = sum;
         }
     }
@@ -1484,22 +1488,22 @@ hipError_t launch_shape(const tp_logits& io, void* out, uint64_t out_stride) {
 }
 
 // Segments a wave of the choice takes, one after another.  Where a window holds the row (131072 tokens) its history is read once and
-// no second launch joins it: taken for rows of up to 64 segments, and where there are rows for every compute unit.  A unit works on a segment for
-// about 0.15 us, though, and fewer long rows than units leave the others idle (one row of 131072: 22 us in one block, 7 + 7 in eight and the join): they are split.
-// (A block each / in blocks of 16 segments and the join, us a pass: one row of 32768 12.4 / 14.5, of 50021 14.6 / 14.8, of 65536 15.6 / 14.7; 48 rows of 50021 17.3 / 17.1,
-// 128 17.2 / 19.3, 200 of 32768 14.0 / 20.1.)
+// no second launch joins it; but a unit works on a segment for some 0.15 us, and fewer long rows than units leave the others idle: they are split.
+// Split / not, us a pass: one row of 20000 14.8 / 11.3, of 32768 14.5 / 12.9, of 50021 14.5 / 14.7, of 65536 14.2 / 16.7, 128 rows of 50021 19.0 / 16.3;
+// one row of 131072 14.7 / 24.1, 48 17.9 / 26.0, 128 23.1 / 26.2, 200 29.8 / 26.6.
 // A window must also keep its repeated tokens in 64 KB of LDS.
 static uint32_t window_segments(const tp_logits& io) {
     uint32_t segs = 1;
-    const bool whole = reply_segments(io.vocab) <= 64 || io.rows >= 256;
+    const bool whole = reply_segments(io.vocab) <= 64 || io.rows >= 160;
     while (segs < MOST_SEGS && segs * CHOICE_WAVES * SEGMENT < io.vocab && (whole || io.rows * ((io.vocab + 2 * segs * CHOICE_WAVES * SEGMENT - 1) / (2 * segs * CHOICE_WAVES * SEGMENT)) >= 256)) segs *= 2;
     while (segs > 1 && io.history && std::min(io.history_cap, segs * CHOICE_WAVES * SEGMENT) > 16384) segs /= 2;
     return segs;
 }
 
 hipError_t launch_choose(const tp_logits& io, const float* temperature, const float* uniform, int32_t* tokens, float* logprob, ChoicePart* parts) {
-    const bool few = reply_segments(io.vocab) <= FEW_WAVES;
-    const uint32_t segs = few ? 1 : window_segments(io), window = segs * (few ? FEW_WAVES : CHOICE_WAVES) * SEGMENT, chunks = (io.vocab + window - 1) / window;
+    const uint32_t segments = reply_segments(io.vocab);
+    const bool few = segments <= FEW_WAVES || (segments <= FEW_WAVES * FEW_SEGS && io.rows > 256);
+    const uint32_t segs = few ? (segments + FEW_WAVES - 1) / FEW_WAVES : window_segments(io), window = segs * (few ? FEW_WAVES : CHOICE_WAVES) * SEGMENT, chunks = (io.vocab + window - 1) / window;
     const uint32_t lds = io.history ? std::min(io.history_cap, window) * 4 : 0, lds_one = io.history ? std::min(io.history_cap, SEGMENT) * 4 : 0;
     return by_type_and_size(io, [&](auto tag, auto tiny) {
         using T = decltype(tag);

@@ -226,7 +226,7 @@ def choice_numbers(rng, rows):
 
 
 @pytest.mark.parametrize("name", sorted(TYPES))
-@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 7), (9, 100), (4, 8192), (5, 8193), (6, 50021), (33, 20000), (2, 300001)])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 7), (9, 100), (4, 8192), (5, 8193), (260, 9000), (6, 50021), (33, 20000), (2, 300001)])
 def test_choose(pipe, name, rows, vocab):
     rng = np.random.default_rng(rows + vocab)
     logits, l = make_logits(rng, rows, vocab, TYPES[name])
