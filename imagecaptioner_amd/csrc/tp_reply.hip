@@ -267,7 +267,7 @@ __device__ inline bool block_any(bool v) {
 // ---- a row in segments ----------------------------------------------------------------------------------------------------------
 constexpr uint32_t SEGMENT = REPLY_SEGMENT;
 constexpr int VECS = (int)(SEGMENT / (64 * 8));
-extern __shared__ uint32_t dynamic_lds[];
+extern __shared__ __attribute__((aligned(16))) uint32_t dynamic_lds[];
 
 // A wave's segment of a row: two vectors of eight tokens a lane, the lane's second 512 tokens behind its first.  A vector that the row's end cuts is loaded
 // from eight tokens before the end instead, so that every lane loads alike; its first `cut` tokens belong to the vector before and
