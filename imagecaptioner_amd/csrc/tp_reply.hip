@@ -293,13 +293,14 @@ __device__ inline void load_mask(const RowRules& r, uint32_t w0, uint32_t n, uin
 }
 
 // `n`: tokens from the window's start to the row's end
-// ONCE: the loads do not ask the caches to keep the logits, which nobody reads again, so that a shared bias keeps its place there (choosing for 512 rows
-// of 131072 with one: 47 -> 45 us).  Shaping, which writes what it reads, is slower that way (256 rows of 131071 in 32 bits: 51 -> 57 us).
-template <class T, bool TINY, bool ONCE>
+// The loads go through the caches, where logits that a product has just written still are: choosing for 512 rows of 131072, some of it there, takes 38.8 us instead of the 41.6 of loads
+// past them, for 512 of 50021 22.3 instead of 24.3; where nothing is, 41.9 instead of 41.2.
+// BIAS_LAST: behind the logits where those wait for nothing (choosing for 512 rows: 43.8 -> 42.9 us), before them in shaping (256 rows: 53.0 -> 51.9).
+template <class T, bool TINY, bool BIAS_LAST>
 __device__ inline void load_segment(const RowRules& r, Glob<typename T::S> row, uint32_t w0, uint32_t n, uint32_t segment, const uint32_t (&bits)[VECS], Held<T>& h) {
     using S = typename T::S;
     const uint32_t at = lane_at(segment);
-    if (r.bias && !TINY && !ONCE) {
+    if (r.bias && !TINY && !BIAS_LAST) {
 #pragma unroll
         for (int v = 0; v < VECS; ++v) {
             auto* from = (Vec<uint32_t>*)(r.bias + w0 + (int32_t)std::min((int32_t)(at + v * 512), (int32_t)n - 8));
@@ -332,8 +333,7 @@ __device__ inline void load_segment(const RowRules& r, Glob<typename T::S> row, 
 #pragma unroll
                 for (int g = 0; g < T::VEC; ++g) {
                     auto* from = (Vec<S>*)(row + (int32_t)std::min((int32_t)t, (int32_t)n - 8)) + g;
-                    if constexpr (ONCE) h.d[v][g] = __builtin_nontemporal_load(from);
-                    else h.d[v][g] = *from;
+                    h.d[v][g] = *from;
                 }
         }
     } else {
@@ -344,13 +344,11 @@ __device__ inline void load_segment(const RowRules& r, Glob<typename T::S> row, 
 #pragma unroll
             for (int g = 0; g < T::VEC; ++g) {
                 auto* from = (Vec<S>*)(row + (int32_t)std::min((int32_t)t, (int32_t)n - 8)) + g;
-                if constexpr (ONCE) h.d[v][g] = __builtin_nontemporal_load(from);
-                else h.d[v][g] = *from;
+                h.d[v][g] = *from;
             }
         }
     }
-    // Behind the logits where those wait for nothing (choose for 512 rows: 43.8 -> 42.9 us), before them in shaping (256 rows: 53.0 -> 51.9).
-    if (r.bias && ONCE) {
+    if (r.bias && BIAS_LAST) {
 #pragma unroll
         for (int v = 0; v < VECS; ++v) {
             auto* from = (Vec<uint32_t>*)(r.bias + w0 + (int32_t)std::min((int32_t)(at + v * 512), (int32_t)n - 8));
@@ -579,7 +577,7 @@ struct Window {
 // 32 bits (five roundings, one more where repeated tokens are among them), everything above in 64.  Against the formula with 64-bit sums, 131072 tokens and temperatures
 // of 0.5 .. 1.2, one row of 5000 got another token, always the border's other side.
 //
-// What bounds it: 512 rows of 131072 bfloat16 (134 MB, 26 us at a copy's rate) with 256 tokens of history and a bias take 41 us: the vector units
+// What bounds it: 512 rows of 131072 bfloat16 (134 MB, 26 us at a copy's rate) with 256 tokens of history and a bias take 42 us: the vector units
 // spend some 260 instructions a segment (powers: 16, four times as long), 29 us of work; the block's start (rules, history and repeated tokens: 6 us) and the join of
 // the row (4 us) are chains of latency that no other block hides, since all rows are at work at once.
 using OneSegment = Window<1, 1>;
