@@ -3,6 +3,7 @@
 hipcc cross-compiles without a GPU.  The library is written next to the
 sources so that it travels with the tree; it is never installed elsewhere.
 """
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -59,13 +60,15 @@ def build(force=False, verbose=False, prof=False):
         return _build(LIB.replace(".so", "_%s.so" % name), "_%s.o" % name, [f for f in flags.split(",") if f], verbose, kernels_only=True)
     if not force and not _stale():
         return LIB
-    lib = _build(LIB, ".o", [], verbose)
-    _build_torch_module(verbose)
+    with concurrent.futures.ThreadPoolExecutor(1) as beside:
+        torch_module = beside.submit(_build_torch_module, verbose)
+        lib = _build(LIB, ".o", [], verbose)
+        torch_module.result()
     return lib
 
 
 def _build(lib, obj_suffix, extra, verbose, kernels_only=False):
-    objs = []
+    objs, cmds = [], []
     for src in SOURCES:
         obj = os.path.join(CSRC, os.path.splitext(src)[0] + obj_suffix)
         if kernels_only and not src.endswith(".hip"):       # experiments only touch the kernels: reuse the main build's host objects
@@ -76,11 +79,12 @@ def _build(lib, obj_suffix, extra, verbose, kernels_only=False):
             cmd += ["-x", "hip"] + DEVICE
         else:
             cmd += ["-x", "c++", "-D__HIP_PLATFORM_AMD__", "-I" + os.path.join(ROCM, "include")]
-        cmd += ["-c", os.path.join(CSRC, src), "-o", obj]
+        cmds.append(cmd + ["-c", os.path.join(CSRC, src), "-o", obj])
         if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.check_call(cmd)
+            print(" ".join(cmds[-1]), flush=True)
         objs.append(obj)
+    with concurrent.futures.ThreadPoolExecutor(len(cmds)) as pool:                 # the kernels' two files take a minute each
+        list(pool.map(subprocess.check_call, cmds))
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-o", lib] + objs
     if verbose:
         print(" ".join(cmd), flush=True)
