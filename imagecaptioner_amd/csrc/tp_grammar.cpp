@@ -169,9 +169,24 @@ const char* check_lines(const int32_t* tokens, uint64_t stride, uint32_t width, 
 std::vector<std::string> reply_tags(const HostTables& ht) {
     // a phrase or a fence inside a force-allowed tag would make the whole line look bad, and one with a comma is cut up
     const uint32_t want = FL_VALID | FL_LEN2 | (ht.known_found ? FL_KNOWN : 0u), without = FL_DROP | FL_PHRASE | FL_FENCE | FL_SPLIT;
+    // What the ingest judges is not the string but what NormalizeTag makes of it, an alias's target among others, and it normalises three times: the line's parts
+    // (Program.cs:599-601), the candidates (:622-631) and the selected tags (:693-697).  The caption's tags are normalised further, to where the string stays the same (or a circle
+    // of aliases closes): all of those must be known too.
+    constexpr int SELECTED = 3, FURTHER = 64;
+    auto kept = [&](uint32_t id) {
+        for (int hop = 1; hop <= FURTHER; ++hop) {
+            const uint32_t to = ht.next[id], f = ht.flags[to];
+            if (hop == 1 && (!(f & FL_LEN2) || (f & FL_SPLIT))) return false;
+            if (hop <= SELECTED && ((f & FL_DROP) || (hop > 1 && !(f & FL_VALID)))) return false;
+            if (hop >= SELECTED && ht.known_found && !(f & FL_KNOWN)) return false;
+            if (hop >= SELECTED && to == id) break;
+            id = to;
+        }
+        return true;
+    };
     std::vector<std::string> tags;
     for (uint32_t i = 0; i < ht.scalars.n_public; ++i)
-        if ((ht.flags[i] & want) == want && !(ht.flags[i] & without)) tags.push_back(ht.strings[i]);
+        if ((ht.flags[i] & want) == want && !(ht.flags[i] & without) && kept(i)) tags.push_back(ht.strings[i]);
     return tags;
 }
 

@@ -25,7 +25,7 @@ struct HostGrammar {
 
 struct HostTables;
 // The tags the line ingest keeps: valid and not dropped, and with a vocabulary file a member of it (where the vocabulary is not
-// strict another table string would be kept too, but the caller's list does not have it).
+// strict another table string would be kept too, but the caller's list does not have it); and the same of what NormalizeTag makes of them.
 std::vector<std::string> reply_tags(const HostTables& ht);
 
 // Throws ConfigError.  tags: the texts a tag may have, in any order, with repeats, before '_' becomes ' '.
