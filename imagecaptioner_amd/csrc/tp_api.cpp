@@ -1863,7 +1863,7 @@ tp_grammar* tp_grammar_create(tp_ctx* ctx, const tp_grammar_config* cfg) {
         if (cfg->tags) {
             for (uint64_t t = 0; t < cfg->n_tags; ++t) tags.emplace_back((const char*)cfg->tags + cfg->tag_offsets[t], (size_t)(cfg->tag_offsets[t + 1] - cfg->tag_offsets[t]));
         } else {
-            tags = reply_tags(ctx->ht);
+            tags = reply_tags(ctx->ht, cfg->spaces != 0);
         }
         HostGrammar h;
         compile_grammar(*cfg, std::move(tags), h);

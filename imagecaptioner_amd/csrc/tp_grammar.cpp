@@ -40,6 +40,11 @@ struct PrefixTree {
 bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 size_t type_bytes(int32_t t) { return t == TP_T_F32 ? 4 : 2; }
 uint64_t mask_words(uint32_t vocab) { return ((uint64_t)vocab + 31) / 32; }
+// a tag as a line of the grammar spells it
+std::string spelled(std::string tag, bool spaces) {
+    if (spaces) std::replace(tag.begin(), tag.end(), '_', ' ');
+    return tag;
+}
 // rows * stride elements of `bytes` stay below 2^62
 bool fits(uint64_t rows, uint64_t stride, uint64_t bytes) { return stride == 0 || rows <= ((uint64_t)1 << 62) / bytes / stride; }
 
@@ -166,8 +171,9 @@ const char* check_lines(const int32_t* tokens, uint64_t stride, uint32_t width, 
     return nullptr;
 }
 
-std::vector<std::string> reply_tags(const HostTables& ht) {
-    // a phrase or a fence inside a force-allowed tag would make the whole line look bad, and one with a comma is cut up
+std::vector<std::string> reply_tags(const HostTables& ht, bool spaces) {
+    // A phrase or a fence inside a force-allowed tag would make the whole line look bad, and one with a comma is cut up.  FL_PHRASE is the string's as it stands, and most
+    // phrases hold a blank: with `spaces` other tags come to hold one ("unable_to_stand").
     const uint32_t want = FL_VALID | FL_LEN2 | (ht.known_found ? FL_KNOWN : 0u), without = FL_DROP | FL_PHRASE | FL_FENCE | FL_SPLIT;
     // What the ingest judges is not the string but what NormalizeTag makes of it, an alias's target among others, and it normalises three times: the line's parts
     // (Program.cs:599-601), the candidates (:622-631) and the selected tags (:693-697).  The caption's tags are normalised further, to where the string stays the same (or a circle
@@ -186,7 +192,7 @@ std::vector<std::string> reply_tags(const HostTables& ht) {
     };
     std::vector<std::string> tags;
     for (uint32_t i = 0; i < ht.scalars.n_public; ++i)
-        if ((ht.flags[i] & want) == want && !(ht.flags[i] & without) && kept(i)) tags.push_back(ht.strings[i]);
+        if ((ht.flags[i] & want) == want && !(ht.flags[i] & without) && kept(i) && !(spaces && holds_phrase(spelled(ht.strings[i], true)))) tags.push_back(ht.strings[i]);
     return tags;
 }
 
@@ -195,7 +201,7 @@ void compile_grammar(const tp_grammar_config& cfg, std::vector<std::string> tags
     out.min_tags = cfg.min_tags;
     out.max_tags = cfg.max_tags;
     for (std::string& t : tags) {
-        if (cfg.spaces) std::replace(t.begin(), t.end(), '_', ' ');
+        t = spelled(std::move(t), cfg.spaces != 0);
         if (t.empty() || t.front() == ' ' || t.back() == ' ') throw ConfigError("a tag of the grammar is empty, or begins or ends with a space");
         for (char ch : t) if (ch == ',' || (uint8_t)ch < 0x20) throw ConfigError("a tag of the grammar holds a comma or a control character");
     }

@@ -26,7 +26,8 @@ struct HostGrammar {
 struct HostTables;
 // The tags the line ingest keeps: valid and not dropped, and with a vocabulary file a member of it (where the vocabulary is not
 // strict another table string would be kept too, but the caller's list does not have it); and the same of what NormalizeTag makes of them.
-std::vector<std::string> reply_tags(const HostTables& ht);
+// With `spaces`, those that a line may hold with ' ' for every '_'.
+std::vector<std::string> reply_tags(const HostTables& ht, bool spaces = false);
 
 // Throws ConfigError.  tags: the texts a tag may have, in any order, with repeats, before '_' becomes ' '.
 void compile_grammar(const tp_grammar_config& cfg, std::vector<std::string> tags, HostGrammar& out);

@@ -683,6 +683,8 @@ struct Interner {
 
 }  // namespace
 
+bool holds_phrase(const std::string& text) { return Loader::has_looks_bad_phrase(lowered(from_utf8((const uint8_t*)text.data(), text.size()))); }
+
 bool less_ordinal_ignore_case(const std::string& a, const std::string& b) {
     return folded(from_utf8((const uint8_t*)a.data(), a.size())) < folded(from_utf8((const uint8_t*)b.data(), b.size()));
 }

@@ -64,6 +64,9 @@ void compile_tables(const tp_config& cfg, HostTables& out, const std::vector<std
 // derives the final-set form the wave-per-file kernel starts from.
 void set_fallback(const HostTables& ht, DevTables& dt, const uint32_t* ids, uint32_t n);
 
+// Whether a text (UTF-8) holds one of the LooksBad phrases (Program.cs:56-58, 1144).
+bool holds_phrase(const std::string& text);
+
 // a < b under StringComparer.OrdinalIgnoreCase (UTF-16 code units, upper-cased the invariant way), both UTF-8.
 bool less_ordinal_ignore_case(const std::string& a, const std::string& b);
 

@@ -571,7 +571,8 @@ int tp_choose_tokens(tp_ctx* ctx, const tp_logits* io, const float* temperature,
  * The grammar of a tag line over a model's token list:  tag ", " tag ", " ... tag <end>,  between min_tags and max_tags
  * tags.  A tag is one the pipeline keeps: with a vocabulary file a member of it that ShouldDropTag lets pass
  * (Program.cs:1121-1133), without one any such string of the context's tables, and in either case only if the ingest also
- * keeps (and, with a vocabulary file, knows) what NormalizeTag makes of it, an alias's target for instance.  Or a tag is
+ * keeps (and, with a vocabulary file, knows) what NormalizeTag makes of it, an alias's target for instance, and if a line
+ * that holds it as it is written does not look bad: with `spaces` "unable_to_stand" would (Program.cs:1144).  Or a tag is
  * one of the caller's own `tags`, which are taken as they are: whether the pipeline keeps them is not looked at.
  * Tags may repeat (tp_logits' penalties are there for that).  A token may be any piece of text; one that holds two
  * commas is never allowed.

@@ -24,7 +24,7 @@ HostGrammar* rsim_compile(const tp_grammar_config* cfg, const tp_config* tables)
         } else {
             HostTables ht;
             compile_tables(*tables, ht);
-            tags = reply_tags(ht);
+            tags = reply_tags(ht, cfg->spaces != 0);
         }
         std::unique_ptr<HostGrammar> g(new HostGrammar());
         compile_grammar(*cfg, tags, *g);

@@ -97,3 +97,16 @@ def test_shipped_tables(sim):  # noqa: F811
     assert len(tags) > 5000
     for t in sorted(tags)[::7]:
         assert kept_by_the_ingest(oracle, t), t
+
+
+PHRASES = ["unable_to_stand", "has_an_airplane", "i_cannot", "hawaii_can't_swim", "cannot_provide_hat", "i'm_not_able", "i_won't"]
+
+
+@pytest.mark.parametrize("spaces", [0, 1])
+def test_no_phrase_behind_underscores(sim, spaces):  # noqa: F811
+    """Most phrases of a refusal hold blanks: a tag that spells one with them has the whole line refused."""
+    words = ["solo", "smile", "long_hair", "sorry_face", "unable"]
+    assert check_tags(sim, words + PHRASES, spaces)[1] == {"sorry_face"} | (set(PHRASES) if spaces else set())
+    oracle = Oracle(Config(vocabulary="\n".join(words + PHRASES).encode()))
+    for t in PHRASES:
+        assert bool(oracle.normalize_raw_tag_line(", ".join([written(t, spaces), "solo", "smile"]))) == (not spaces), t
