@@ -190,9 +190,11 @@ std::vector<std::string> reply_tags(const HostTables& ht, bool spaces) {
         }
         return true;
     };
+    // A blank at a tag's end would be trimmed off with the comma's, and another tag read.  (None begins with '_'.)
+    auto spellable = [&](const std::string& s) { return !spaces || (s.back() != '_' && !holds_phrase(spelled(s, true))); };
     std::vector<std::string> tags;
     for (uint32_t i = 0; i < ht.scalars.n_public; ++i)
-        if ((ht.flags[i] & want) == want && !(ht.flags[i] & without) && kept(i) && !(spaces && holds_phrase(spelled(ht.strings[i], true)))) tags.push_back(ht.strings[i]);
+        if ((ht.flags[i] & want) == want && !(ht.flags[i] & without) && kept(i) && spellable(ht.strings[i])) tags.push_back(ht.strings[i]);
     return tags;
 }
 
@@ -202,8 +204,8 @@ void compile_grammar(const tp_grammar_config& cfg, std::vector<std::string> tags
     out.max_tags = cfg.max_tags;
     for (std::string& t : tags) {
         t = spelled(std::move(t), cfg.spaces != 0);
-        if (t.empty() || t.front() == ' ' || t.back() == ' ') throw ConfigError("a tag of the grammar is empty, or begins or ends with a space");
-        for (char ch : t) if (ch == ',' || (uint8_t)ch < 0x20) throw ConfigError("a tag of the grammar holds a comma or a control character");
+        if (t.empty() || t.front() == ' ' || t.back() == ' ') throw ConfigError("a tag of the grammar is empty, or begins or ends with a space: \"" + t + "\"");
+        for (char ch : t) if (ch == ',' || (uint8_t)ch < 0x20) throw ConfigError("a tag of the grammar holds a comma or a control character: \"" + t + "\"");
     }
     std::sort(tags.begin(), tags.end(), [](const std::string& a, const std::string& b) {
         const int c = std::memcmp(a.data(), b.data(), std::min(a.size(), b.size()));

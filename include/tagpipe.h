@@ -572,7 +572,8 @@ int tp_choose_tokens(tp_ctx* ctx, const tp_logits* io, const float* temperature,
  * tags.  A tag is one the pipeline keeps: with a vocabulary file a member of it that ShouldDropTag lets pass
  * (Program.cs:1121-1133), without one any such string of the context's tables, and in either case only if the ingest also
  * keeps (and, with a vocabulary file, knows) what NormalizeTag makes of it, an alias's target for instance, and if a line
- * that holds it as it is written does not look bad: with `spaces` "unable_to_stand" would (Program.cs:1144).  Or a tag is
+ * that holds it as it is written does not look bad: with `spaces` "unable_to_stand" would (Program.cs:1144), and a tag that
+ * ends in '_' cannot be written.  Or a tag is
  * one of the caller's own `tags`, which are taken as they are: whether the pipeline keeps them is not looked at.
  * Tags may repeat (tp_logits' penalties are there for that).  A token may be any piece of text; one that holds two
  * commas is never allowed.

@@ -110,3 +110,14 @@ def test_no_phrase_behind_underscores(sim, spaces):  # noqa: F811
     oracle = Oracle(Config(vocabulary="\n".join(words + PHRASES).encode()))
     for t in PHRASES:
         assert bool(oracle.normalize_raw_tag_line(", ".join([written(t, spaces), "solo", "smile"]))) == (not spaces), t
+
+
+def test_a_tag_that_cannot_be_written_with_spaces(sim):  # noqa: F811
+    """A blank at a tag's end is trimmed off: the context's tags that end in one are left out, a caller's are refused by name."""
+    words = ["solo_", "solo", "smile", "hat_(a)_", "hat_(a)"]
+    assert check_tags(sim, words, 0)[1] == set()
+    g = compiled(sim, BYTES, 256, tables=Config(vocabulary="\n".join(words).encode()), spaces=1)
+    assert not isinstance(g, str) and grammar_tags(g) == {"solo", "smile", "hat (a)"}
+    refusal = compiled(sim, BYTES, 256, tags=words, spaces=1)
+    assert "ends with a space" in refusal and '"hat (a) "' in refusal or '"solo "' in refusal, refusal
+    assert '"so,lo"' in compiled(sim, BYTES, 256, tags=["so,lo"])
