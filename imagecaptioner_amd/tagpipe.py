@@ -495,7 +495,8 @@ class TagPipe:
         return replies.choose_tokens(self, logits, temperature, uniform, rules)
 
     def tag_grammar(self, tokens, end_token, *, min_tags=3, max_tags=42, spaces=False, tags=None):
-        """tp_grammar_create: the tag lines of this context's tables (or of `tags`) over a model's token list (texts, bytes or str)."""
+        """tp_grammar_create: the tag lines of this context's tables (or of `tags`, as they are) over a model's token list (texts, bytes or str).  min_tags and
+        max_tags count written tags: of repeats the ingest keeps one."""
         return replies.TagGrammar(self, tokens, end_token, min_tags, max_tags, spaces, tags)
 
     def run_tokens(self, grammar, tokens, lengths=None, begin=None):

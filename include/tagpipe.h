@@ -493,7 +493,7 @@ int tp_format_review_rows(const tp_ctx* ctx, const tp_result* res, int format, c
  * Writing the replies.  The line ingest above parses a language model's answer (Program.cs:574-587); a caller whose
  * captioning model runs on the same GPU has that model's logits in device memory, one row per reply and one column per
  * token.  The functions below write the answer under the rules the pipeline will read it by, token by token, so that
- * no refusal, no unknown tag and no cut-off line has to be dropped afterwards:
+ * no refusal and no unknown tag has to be dropped afterwards (tp_grammar_create says what they do not rule out):
  *
  *   tp_shape_logits   penalties for repeated tokens, a bias and a mask of allowed tokens on the logits
  *   tp_choose_tokens  the same without writing the logits: the token that is chosen, and its log-probability
@@ -575,8 +575,13 @@ int tp_choose_tokens(tp_ctx* ctx, const tp_logits* io, const float* temperature,
  * that holds it as it is written does not look bad: with `spaces` "unable_to_stand" would (Program.cs:1144), and a tag that
  * ends in '_' cannot be written.  Or a tag is
  * one of the caller's own `tags`, which are taken as they are: whether the pipeline keeps them is not looked at.
- * Tags may repeat (tp_logits' penalties are there for that).  A token may be any piece of text; one that holds two
- * commas is never allowed.
+ * A token may be any piece of text; one that holds two commas is never allowed.
+ * min_tags and max_tags count the tags as they are written.  Tags may repeat, or be normalised to the same one
+ * (tp_logits' penalties are there for that), and the ingest keeps one of them (Program.cs:602).  So a caption may have fewer
+ * tags than min_tags, and it falls back where fewer than three different ones are selected, the trigger and 1girl among
+ * them (Program.cs:297).  Of more than 42 selected tags, the trigger, 1girl and the profile's always-add tags included, the last are
+ * left out (Program.cs:38).  And with min_tags below 3 a line of one or two tags and more than 40 characters is refused as a
+ * whole (Program.cs:1145-1146).  A line that has not come to its end may stop inside a tag.
  * Refused (TP_E_CONFIG): no tags; a token list without a token of its own for every single byte that the lines use,
  * because a line could then come to a place with no way on.  All pointers are host memory and are not kept.
  *
@@ -592,7 +597,7 @@ typedef struct tp_grammar_config {
     const uint8_t*  tokens;        /* token t is tokens[token_offsets[t] .. token_offsets[t + 1]); an empty one is never allowed */
     const uint64_t* token_offsets; /* n_tokens + 1 */
     int32_t  end_token;            /* ends a line; its text counts as empty */
-    uint32_t min_tags, max_tags;   /* 1 <= min_tags <= max_tags <= 65535; three tags is what a line needs not to fall back (Program.cs:297) */
+    uint32_t min_tags, max_tags;   /* 1 <= min_tags <= max_tags <= 65535; three written tags (two commas) are what no line is refused for (Program.cs:1145) */
     uint32_t spaces;               /* 1: the '_' of a tag is written ' ' (NormalizeTag takes it back, Program.cs:1153) */
     const uint8_t*  tags;          /* the caller's own tags, laid out like the tokens; NULL: the context's */
     const uint64_t* tag_offsets;   /* n_tags + 1 */

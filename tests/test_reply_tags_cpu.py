@@ -1,5 +1,6 @@
 """The tags a grammar takes from a context's tables against what the line ingest keeps of them, as the oracle says it: host code, no GPU."""
 import json
+import random
 
 import pytest
 
@@ -121,3 +122,35 @@ def test_a_tag_that_cannot_be_written_with_spaces(sim):  # noqa: F811
     refusal = compiled(sim, BYTES, 256, tags=words, spaces=1)
     assert "ends with a space" in refusal and '"hat (a) "' in refusal or '"solo "' in refusal, refusal
     assert '"so,lo"' in compiled(sim, BYTES, 256, tags=["so,lo"])
+
+
+ALIASES = {"soles": "foot_sole", "blond_hair": "blonde_hair", "hood": "watermark", "cap": "hats"}
+WORDS = ["1girl", "solo", "soles", "foot_sole", "blond_hair", "blonde_hair", "blue_eyes", "hood", "cap", "hats", "unable_to_stand", "long_hair", "smile", "a_", "school_uniform", "blue_sky"]
+
+
+@pytest.mark.parametrize("spaces", [0, 1])
+def test_finished_lines_are_taken(sim, spaces):  # noqa: F811
+    """Lines of at least three of the grammar's tags, repeats among them: none is refused, and every different tag is selected and known."""
+    cfg = Config(vocabulary="\n".join(WORDS).encode(), lexicon=lexicon(ALIASES), trigger="solo")
+    oracle, rng = Oracle(cfg), random.Random(11)
+    tags = sorted(grammar_tags(compiled(sim, BYTES, 256, tables=cfg, spaces=spaces)))
+    assert set(WORDS) - {t.replace(" ", "_") for t in tags} == {"hood", "soles"} | ({"unable_to_stand", "a_"} if spaces else set())   # the vocabulary has read "soles" as "foot_sole"
+    lines = [[rng.choice(tags) for _ in range(rng.randint(3, 12))] for _ in range(300)]
+    got = oracle.run_texts([", ".join(line) for line in lines], detail=True)
+    assert got.counters["line_rejected"] == 0 and not got.verdicts["n_dropped"].any()
+    for line, v, d in zip(lines, got.verdicts, got.details):
+        kept = {oracle.normalize_tag(t) for t in line}
+        selected = oracle.select_tags_from_line(", ".join(line))
+        assert v["n_candidates"] == len(kept) and set(selected) == kept | {"1girl", "solo"} and len(selected) == v["n_selected"]
+        assert not kept & set(d["unknown"])
+        assert bool(v["flags"] & 0x08) == (len(selected) < 3)                    # the fallback
+
+
+def test_what_a_finished_line_may_still_be(sim):  # noqa: F811
+    """What the header does not promise: repeats count as written tags, two tags of more than 40 characters are refused, and a caption ends at 42 tags."""
+    words = ["1girl", "sgrui", "blue_eyes", "a" * 25, "b" * 25] + ["w%d" % k for k in range(60)]
+    oracle = Oracle(Config(vocabulary="\n".join(words).encode()))
+    assert oracle.select_tags_from_line("blue_eyes, blue_eyes, blue_eyes") == ["sgrui", "1girl", "blue_eyes"]
+    assert oracle.run_texts(["1girl, sgrui, 1girl", "%s, %s" % (words[3], words[4]), "%s, 1girl" % words[3], "%s, %s, 1girl" % (words[3], words[4])]).verdicts["flags"].tolist() == [0x09, 0x19, 0x01, 0x01]
+    long = oracle.select_tags_from_line(", ".join(words[5:47]))
+    assert len(long) == 42 and long[:2] == ["sgrui", "1girl"] and len(set(long) & set(words[5:47])) == 40
