@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -42,13 +43,18 @@ void check(int rc) {
     throw Refused{};
 }
 
+// whether something is to be differentiated by this tensor: backwards, or forwards (it carries a tangent)
+bool differentiated(const at::Tensor& t) {
+    return (t.requires_grad() && c10::GradMode::is_enabled()) || (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined());
+}
+
 [[noreturn]] void refuse(const char* name, PyObject* o, int device, at::ScalarType dtype, int64_t rows, int64_t columns) {
     if (!THPVariable_Check(o)) {
         PyErr_Format(PyExc_ValueError, "%s must be a tensor, got %R", name, (PyObject*)Py_TYPE(o));
         throw Refused{};
     }
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (t.requires_grad() && c10::GradMode::is_enabled()) {
+    if (differentiated(t)) {
         PyErr_Format(PyExc_ValueError, "%s requires a gradient, which this call does not have: detach it", name);
         throw Refused{};
     }
@@ -66,7 +72,7 @@ void check(int rc) {
 bool usable(PyObject* o, int device, at::ScalarType dtype, int64_t dim) {
     if (!THPVariable_Check(o)) return false;
     const at::Tensor& t = THPVariable_Unpack(o);
-    return t.scalar_type() == dtype && t.get_device() == device && t.layout() == at::kStrided && t.dim() == dim && !(t.requires_grad() && c10::GradMode::is_enabled());
+    return t.scalar_type() == dtype && t.get_device() == device && t.layout() == at::kStrided && t.dim() == dim && !differentiated(t);
 }
 
 // A dense vector's data.
