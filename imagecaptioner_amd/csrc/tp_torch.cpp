@@ -48,6 +48,9 @@ bool differentiated(const at::Tensor& t) {
     return (t.requires_grad() && c10::GradMode::is_enabled()) || (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined());
 }
 
+// whether the values are not what stands in memory: a view that negates them (as the imaginary part of a conjugate does), or zeros without memory
+bool lazy(const at::Tensor& t) { return t.is_neg() || t._is_zerotensor(); }
+
 [[noreturn]] void refuse(const char* name, PyObject* o, int device, at::ScalarType dtype, int64_t rows, int64_t columns) {
     if (!THPVariable_Check(o)) {
         PyErr_Format(PyExc_ValueError, "%s must be a tensor, got %R", name, (PyObject*)Py_TYPE(o));
@@ -56,6 +59,10 @@ bool differentiated(const at::Tensor& t) {
     const at::Tensor& t = THPVariable_Unpack(o);
     if (differentiated(t)) {
         PyErr_Format(PyExc_ValueError, "%s requires a gradient, which this call does not have: detach it", name);
+        throw Refused{};
+    }
+    if (lazy(t)) {
+        PyErr_Format(PyExc_ValueError, "%s does not stand in memory as its values are (a negated view, or zeros without memory): clone or resolve it", name);
         throw Refused{};
     }
     std::string shape = "(" + std::to_string(rows) + (columns == -2 ? ",)" : ", " + std::to_string(columns) + ")");
@@ -72,7 +79,7 @@ bool differentiated(const at::Tensor& t) {
 bool usable(PyObject* o, int device, at::ScalarType dtype, int64_t dim) {
     if (!THPVariable_Check(o)) return false;
     const at::Tensor& t = THPVariable_Unpack(o);
-    return t.scalar_type() == dtype && t.get_device() == device && t.layout() == at::kStrided && t.dim() == dim && !differentiated(t);
+    return t.scalar_type() == dtype && t.get_device() == device && t.layout() == at::kStrided && t.dim() == dim && !differentiated(t) && !lazy(t);
 }
 
 // A dense vector's data.

@@ -47,3 +47,21 @@ def test_tangents_are_refused():
                 choose(**args)
         with pytest.raises(ValueError, match="out requires a gradient"):
             shape_into(dual(torch.ones(ROWS, VOCAB)))
+
+
+def test_values_that_do_not_stand_in_memory_are_refused():
+    """The imaginary part of a conjugate is a view with the opposite sign in memory; torch's efficient zeros have no memory at all."""
+    for k, v in arguments().items():
+        lazy = [torch._efficientzerotensor(v.shape, dtype=v.dtype)]
+        if v.is_floating_point():
+            lazy.append(torch._neg_view(v))
+        for t in lazy:
+            args = arguments()
+            args[k] = t
+            with pytest.raises(ValueError, match=k + " does not stand in memory"):
+                choose(**args)
+            args[k] = t.resolve_neg().clone() if t.is_neg() else torch.zeros(t.shape, dtype=t.dtype)
+            with pytest.raises(TagPipeError, match="null argument"):
+                choose(**args)
+    with pytest.raises(ValueError, match="out does not stand in memory"):
+        shape_into(torch._neg_view(torch.ones(ROWS, VOCAB)))
