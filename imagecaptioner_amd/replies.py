@@ -134,15 +134,24 @@ class TagGrammar:
         native = _native()
         native.advance(self._h, self.device, _stream(self.device), states, self._n_tokens, tokens, append, {"history": history, "history_len": history_len})
 
+    def _capturing(self):
+        with _torch_module.cuda.device(self.device):
+            return _torch_module.cuda.is_current_stream_capturing()
+
     def lines(self, tokens, lengths=None, begin=None, arena=None):
         """tp_grammar_lines: (arena uint8, offsets int64 [rows + 1]) of rows of tokens int32 [rows, n], from begin to below lengths (int32
-        [rows]).  A given arena bounds what is written: compare offsets[rows] with its size."""
+        [rows]).  A given arena bounds what is written: compare offsets[rows] with its size.  Without one it is made for rows of nothing but the
+        longest token, up to MOST_ARENA bytes; beyond those the texts' sizes are found first, for which the call waits (a captured call cannot, and
+        makes the large one)."""
         native = _native()
+        if arena is None and isinstance(tokens, _torch_module.Tensor) and tokens.numel() * self._longest > MOST_ARENA and not self._capturing():
+            _, offsets = self.lines(tokens, lengths, begin, arena=tokens.new_empty((0,), dtype=_torch_module.uint8))
+            arena = tokens.new_empty((int(offsets[-1]) + 16,), dtype=_torch_module.uint8)
         return native.lines(self._h, self.device, _stream(self.device), tokens, lengths, begin, arena, self._longest)
 
 
-# An arena for rows of nothing but the longest token is made up to this many bytes; beyond it (a token list may hold a token of a hundred
-# spaces) the texts' sizes are found first, at the price of doing the work twice.
+# Most bytes of an arena that is made for the largest texts there could be: a token list may hold a token of a hundred spaces, or of a megabyte.  Finding the
+# sizes first does the work twice.
 MOST_ARENA = 1 << 30
 
 
@@ -150,11 +159,7 @@ def run_tokens(pipe, grammar, tokens, lengths, begin):
     torch = _torch()
     if grammar.device != pipe._device:
         raise ValueError("the grammar is on another device than the context")
-    arena = None
-    if tokens.numel() * grammar.info.longest_token > MOST_ARENA:
-        _, offsets = grammar.lines(tokens, lengths, begin, arena=tokens.new_empty((0,), dtype=torch.uint8))
-        arena = tokens.new_empty((int(offsets[-1]) + 16,), dtype=torch.uint8)
-    arena, offsets = grammar.lines(tokens, lengths, begin, arena)
+    arena, offsets = grammar.lines(tokens, lengths, begin)
     rows, info, device = tokens.shape[0], pipe.info, tokens.device
 
     def zeros(n, dtype):
