@@ -1,8 +1,12 @@
-"""The text of written tokens where its bound is far from its size, on the GPU."""
+"""The text of written tokens where its bound is far from its size, and as the first work of a process, on the GPU."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
-from helpers import Config
+from helpers import ROOT, Config
 from reply_plain import TAGS, PlainGrammar
 
 torch = pytest.importorskip("torch")
@@ -57,3 +61,35 @@ def test_a_captured_call_makes_the_large_arena(pipe, monkeypatch):
         assert torch.equal(offsets, eager_offsets) and arena.numel() == 70 * 9 + 16
         assert bytes(arena[:640].cpu().numpy()) == bytes(eager[:640].cpu().numpy()) == bytes([letter]) * 630 + b"\0" * 10
         assert plain.text(t[0].tolist()) * 70 == bytes(arena[:630].cpu().numpy())
+
+
+FIRST = """
+import numpy as np, torch
+from imagecaptioner_amd import Config, TagPipe
+pipe = TagPipe(Config(vocabulary=b"solo\\nsmile\\nhat"))
+tokens = [bytes([b]) for b in range(256)] + [b""]
+g = pipe.tag_grammar(tokens, 256)
+rows = 70001                                          # so many are placed by the scan of the caption offsets
+t = torch.as_tensor(np.random.default_rng(5).integers(97, 123, (rows, 2)).astype(np.int32), device="cuda")
+states, logits = torch.zeros(5, 2, device="cuda", dtype=torch.int32), torch.randn(5, 257, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):                         # nothing of the reply calls has run before
+    arena, offsets = g.lines(t)
+    mask = g.mask(states)
+    shaped = pipe.shape_logits(logits, mask=mask, mask_row=torch.arange(5, device="cuda", dtype=torch.int32))
+    token, logprob = g.step(states, logits)
+for _ in range(3):
+    states.zero_()
+    t.copy_(t.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bytes(arena[:2 * rows].cpu().numpy()) == t.cpu().numpy().astype(np.uint8).tobytes()
+    assert np.array_equal(offsets.cpu().numpy(), np.arange(rows + 1) * 2)
+    assert torch.equal(token, shaped.argmax(1).int()) and (shaped > -1e30).sum(1).tolist() == [2] * 5    # 's' and 'h' begin a line
+print("captured first calls replay")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    done = subprocess.run([sys.executable, "-c", FIRST], cwd=ROOT, env=dict(os.environ, PYTHONPATH=ROOT), capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "captured first calls replay" in done.stdout, done.stderr[-2000:]
