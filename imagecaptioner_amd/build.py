@@ -2,9 +2,13 @@
 
 hipcc cross-compiles without a GPU.  The library is written next to the
 sources so that it travels with the tree; it is never installed elsewhere.
+Beside it stands the torch module of the reply calls (_tp_torch.so), where
+there is a torch to build it against.
 """
 import concurrent.futures
+import importlib.util
 import os
+import shutil
 import subprocess
 import sys
 
@@ -24,8 +28,22 @@ DEVICE = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 # The torch side of the reply calls: a Python module against the torch that is installed, host code only.
-TORCH_SOURCE = os.path.join(CSRC, "tp_torch.cpp")
+TORCH_SOURCES = ["tp_torch.cpp", os.path.join("..", "..", "include", "tagpipe.h")]
 TORCH_LIB = os.path.join(HERE, "_tp_torch.so")
+CXX = os.environ.get("CXX", "g++")
+
+
+def _torch_module_missing():
+    """Why the torch module cannot be built here, or None.  The C library does without it (a C# program needs nothing else); the reply calls of
+    replies.py say so when one is made."""
+    spec = importlib.util.find_spec("torch")                    # without importing it
+    if spec is None or not spec.origin:
+        return "torch is not installed"
+    if not os.path.isdir(os.path.join(os.path.dirname(spec.origin), "include", "torch", "csrc")):
+        return "torch is installed without its headers"
+    if shutil.which(CXX) is None:
+        return "there is no C++ compiler %s" % CXX
+    return None
 
 
 def _build_torch_module(verbose):
@@ -33,21 +51,26 @@ def _build_torch_module(verbose):
 
     import torch
     root = os.path.dirname(torch.__file__)
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
            "-I" + sysconfig.get_paths()["include"]]
     for d in ("include", os.path.join("include", "torch", "csrc", "api", "include")):
         cmd += ["-isystem", os.path.join(root, d)]
-    cmd += [TORCH_SOURCE, "-o", TORCH_LIB, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    cmd += [os.path.join(CSRC, TORCH_SOURCES[0]), "-o", TORCH_LIB, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
 
 
+def _older(lib, sources):
+    return not os.path.exists(lib) or any(os.path.getmtime(os.path.join(CSRC, f)) > os.path.getmtime(lib) for f in sources)
+
+
 def _stale():
-    if not os.path.exists(LIB) or not os.path.exists(TORCH_LIB):
-        return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_LIB))
-    return os.path.getmtime(TORCH_SOURCE) > t or any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in SOURCES + HEADERS)
+    return _older(LIB, SOURCES + HEADERS)
+
+
+def _torch_module_stale():
+    return _older(TORCH_LIB, TORCH_SOURCES)
 
 
 def build(force=False, verbose=False, prof=False):
@@ -58,13 +81,16 @@ def build(force=False, verbose=False, prof=False):
     if variant:
         name, flags = variant.split(":", 1)
         return _build(LIB.replace(".so", "_%s.so" % name), "_%s.o" % name, [f for f in flags.split(",") if f], verbose, kernels_only=True)
-    if not force and not _stale():
-        return LIB
+    missing = _torch_module_missing()
+    if missing and (force or verbose):
+        print("%s: the library is built without the torch module of the reply calls" % missing, flush=True)
     with concurrent.futures.ThreadPoolExecutor(1) as beside:
-        torch_module = beside.submit(_build_torch_module, verbose)
-        lib = _build(LIB, ".o", [], verbose)
-        torch_module.result()
-    return lib
+        torch_module = beside.submit(_build_torch_module, verbose) if not missing and (force or _torch_module_stale()) else None
+        if force or _stale():
+            _build(LIB, ".o", [], verbose)
+        if torch_module:
+            torch_module.result()
+    return LIB
 
 
 def _build(lib, obj_suffix, extra, verbose, kernels_only=False):
