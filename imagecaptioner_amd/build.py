@@ -8,6 +8,7 @@ there is a torch to build it against.
 import concurrent.futures
 import importlib.util
 import os
+import runpy
 import shutil
 import subprocess
 import sys
@@ -46,12 +47,19 @@ def _torch_module_missing():
     return None
 
 
+def _torch_name():
+    """The installed torch, as `torch.__version__ torch.version.git_version`, without importing it."""
+    spec = importlib.util.find_spec("torch")
+    v = runpy.run_path(os.path.join(os.path.dirname(spec.origin), "version.py"))
+    return "%s %s" % (v["__version__"], v["git_version"])
+
+
 def _build_torch_module(verbose):
     import sysconfig
 
     import torch
     root = os.path.dirname(torch.__file__)
-    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+    cmd = [CXX, '-DTP_TORCH_NAME="%s"' % _torch_name(), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
            "-I" + sysconfig.get_paths()["include"]]
     for d in ("include", os.path.join("include", "torch", "csrc", "api", "include")):
         cmd += ["-isystem", os.path.join(root, d)]
@@ -70,7 +78,10 @@ def _stale():
 
 
 def _torch_module_stale():
-    return _older(TORCH_LIB, TORCH_SOURCES)
+    if _older(TORCH_LIB, TORCH_SOURCES):
+        return True
+    with open(TORCH_LIB, "rb") as f:                             # it names the torch it was built against (its layouts are compiled in)
+        return ("torch module for " + _torch_name()).encode() + b"\0" not in f.read()
 
 
 def build(force=False, verbose=False, prof=False):

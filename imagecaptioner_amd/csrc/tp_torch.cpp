@@ -460,6 +460,10 @@ PyMethodDef methods[] = {
     {"step", (PyCFunction)(void*)step, METH_FASTCALL, nullptr},       {"advance", (PyCFunction)(void*)advance, METH_FASTCALL, nullptr},
     {"lines", (PyCFunction)(void*)lines, METH_FASTCALL, nullptr},     {nullptr, nullptr, 0, nullptr},
 };
+// The torch whose headers this was compiled with: another one's tensors may be laid out otherwise, so whoever loads the module compares, and the build looks for the text
+// in the file.
+const char built_for[] = "torch module for " TP_TORCH_NAME;
+
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tp_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -467,5 +471,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tp_torch", nullptr, -1, methods, 
 PyMODINIT_FUNC PyInit__tp_torch() {
     for (int k = 0; k < RULES; ++k)
         if (!(rule_keys[k] = PyUnicode_InternFromString(rule_names[k]))) return nullptr;
-    return PyModule_Create(&module);
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", built_for) < 0) Py_CLEAR(m);
+    return m;
 }

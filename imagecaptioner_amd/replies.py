@@ -35,6 +35,10 @@ def _native():
         except ImportError as e:
             raise TagPipeError(-3, "the torch module is not built or does not fit this torch (run `python -m imagecaptioner_amd.build`): %s" % e) from e
 
+        here = "torch module for %s %s" % (torch.__version__, torch.version.git_version)
+        if _tp_torch.built_for != here:
+            raise TagPipeError(-3, "this is a %s, and the module is a %s (run `python -m imagecaptioner_amd.build`)" % (here, _tp_torch.built_for))
+
         def failed(rc):
             raise TagPipeError(rc, L.tp_last_error().decode("utf-8", "replace"))
         _tp_torch.bind(*(C.cast(f, C.c_void_p).value for f in (L.tp_shape_logits, L.tp_choose_workspace, L.tp_choose_tokens, L.tp_grammar_mask, L.tp_grammar_step,

@@ -13,7 +13,8 @@ def recorded(monkeypatch, tmp_path):
     ran = []
 
     def touch(path, what):
-        with open(path, "w"):
+        with open(path, "w") as f:
+            f.write("torch module for %s\0" % build._torch_name() if what == "torch module" else "")
             ran.append(what)
     monkeypatch.setattr(build, "LIB", str(tmp_path / "lib.so"))
     monkeypatch.setattr(build, "TORCH_LIB", str(tmp_path / "torch.so"))
@@ -53,3 +54,24 @@ def test_the_library_is_built_without_torch(recorded, monkeypatch, tmp_path, cap
     assert "without the torch module" in capsys.readouterr().out
     build.build()                                                # and it is not stale for the module's absence
     assert recorded == ["library"]
+
+
+def test_another_torch(recorded, monkeypatch):
+    """A module that was built against another torch is stale, and refused where it is loaded all the same."""
+    import torch
+
+    from imagecaptioner_amd import TagPipeError, replies
+    assert build._torch_name() == "%s %s" % (torch.__version__, torch.version.git_version)
+    build.build()
+    recorded.clear()
+    assert not build._torch_module_stale()
+    monkeypatch.setattr(build, "_torch_name", lambda: "9.9.9 abc")
+    assert build._torch_module_stale() and not build._stale()
+    build.build()
+    assert recorded == ["torch module"] and not build._torch_module_stale()
+    monkeypatch.setattr(replies, "_native_module", None)
+    assert replies._native().built_for.endswith(torch.version.git_version)
+    monkeypatch.setattr(replies, "_native_module", None)
+    monkeypatch.setattr(torch.version, "git_version", "abc")
+    with pytest.raises(TagPipeError, match="abc, and the module is a torch module for"):
+        replies._native()
