@@ -124,10 +124,6 @@ __device__ inline float penalised(float x, uint32_t c, const RowRules& r) {
 
 // ---- wave reductions --------------------------------------------------------------------------------------------------------
 // Every sum is taken in one fixed order, so that a call's results do not change from run to run.
-template <int CTRL, int ROWS>
-__device__ inline float dpp(float old, float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
-}
 __device__ inline float read_lane(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
 
 // One instruction a step (the waits are for the step before, whose result another lane reads); a NaN is passed over.
@@ -139,15 +135,6 @@ __device__ inline float wave_max(float v) {
         "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_bcast:15 row_mask:0xa bank_mask:0xf\n\t"
         "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_bcast:31 row_mask:0xc bank_mask:0xf\n\t"
         "s_nop 1" : "+v"(v));
-    return read_lane(v, 63);
-}
-__device__ inline float wave_sum(float v) {
-    v += dpp<0x111, 0xF>(0.0f, v);
-    v += dpp<0x112, 0xF>(0.0f, v);
-    v += dpp<0x114, 0xF>(0.0f, v);
-    v += dpp<0x118, 0xF>(0.0f, v);
-    v += dpp<0x142, 0xA>(0.0f, v);
-    v += dpp<0x143, 0xC>(0.0f, v);
     return read_lane(v, 63);
 }
 // sum of the lanes up to and including this one
