@@ -179,7 +179,7 @@ __device__ inline double eight_lanes_sum(double v) {
 
 // ---- weights ------------------------------------------------------------------------------------------------------------------
 // z = x / T is rounded to 32 bits, as the formula says, by the quotient's own rounding: with 131072 tokens a border between two of them lies in every
-// hundred-thousandth of the weight, and unrounded quotients chose another token than the rounded ones in one row of 700.
+// hundred-thousandth of the weight, and unrounded quotients choose another token than the rounded ones in one row of 1100 (28 of 30720).
 // A token's weight is 2^(z * LOG2E - c), c = best * LOG2E rounded once for the tokens that are summed together: one fused multiply-add and one power.  c is no
 // more than a common scale, known exactly to whoever joins sums of different c, so that a weight is off by LOG2E's rounding and the fma's, each half a step
 // relative in the exponent, and by the power's own step.  From |c| = 2^30 on, neighbouring numbers lie so far apart that only the largest z weighs anything, and c's own rounding
@@ -280,8 +280,9 @@ __device__ inline void load_mask(const RowRules& r, uint32_t w0, uint32_t n, uin
 }
 
 // `n`: tokens from the window's start to the row's end
-// The loads go through the caches, where logits that a product has just written still are: choosing for 512 rows of 131072, some of it there, takes 38.8 us instead of the 41.6 of loads
-// past them, for 512 of 50021 22.3 instead of 24.3; where nothing is, 41.9 instead of 41.2.
+// The loads go through the caches, where logits that a product has just written still are if it writes them to one place step after step, as a loop over an allocator's blocks does: choosing
+// for 512 rows of 131072 behind such a product takes 37 us instead of the 41 of loads past them, for 512 of 50021 23.0 instead of 23.7.  With three places in turn it takes 44.5
+// instead of 42, 23.2 instead of 23.9; where nothing is in the caches 42.2 instead of 41.2, 24.1 instead of 23.9.
 // BIAS_LAST: behind the logits where those wait for nothing (choosing for 512 rows: 43.8 -> 42.9 us), before them in shaping (256 rows: 53.0 -> 51.9).
 template <class T, bool TINY, bool BIAS_LAST>
 __device__ inline void load_segment(const RowRules& r, Glob<typename T::S> row, uint32_t w0, uint32_t n, uint32_t segment, const uint32_t (&bits)[VECS], Held<T>& h) {
@@ -561,8 +562,9 @@ struct Window {
 // The first launch reads the logits once and leaves of every segment the sum of its weights and the z that they are relative to.  The second joins a
 // row with one wave: the token's segment by a scan of the segments' shares, and the token in that segment, which
 // the wave shapes again (1024 tokens of the row).  A row of one window does both in the first launch.  A lane's sixteen weights of a segment are summed in
-// 32 bits (five roundings, one more where repeated tokens are among them), everything above in 64.  Against the formula with 64-bit sums, 131072 tokens and temperatures
-// of 0.5 .. 1.2, one row of 5000 got another token, always the border's other side.
+// 32 bits (five roundings, one more where repeated tokens are among them), everything above in 64: sums in 64 bits from the first weight on take 53.5 us instead of 42.0 for
+// 512 rows of 131072 (their LDS leaves one block a unit), 16.6 instead of 16.2 for 48 of 50021.  Against the formula with 64-bit sums, 131072 tokens and temperatures
+// of 0.5 .. 1.2, 7 rows of 30720 got another token, always the border's other side, and the border within 2e-8 of the weight from the random number.
 //
 // What bounds it: 512 rows of 131072 bfloat16 (134 MB, 26 us at a copy's rate) with 256 tokens of history and a bias take 42 us: the vector units
 // spend some 260 instructions a segment (powers: 16, four times as long), 29 us of work; the block's start (rules, history and repeated tokens: 6 us) and the join of
@@ -1221,6 +1223,7 @@ __device__ inline Written written(const int32_t* begin, const int32_t* len, uint
 // instead of 20.4, for their registers and their bursts); a text stands beside
 // their sizes in 16 bytes up to a length of 15.  Bound by the gathers (64 cache lines a wave's load) and by LDS: 8192 rows of up to 300 tokens (7 MB of
 // tokens, 13 of text: 4.5 us at a copy's rate) take 6 us for the sizes (10 without the table of lengths in LDS) and 15 for the texts.
+// A wave of the sizes holds SIZE_AHEAD times 64 tokens: 3, 4, 5, 6 and 8 are within 3 % of one another for 8192 rows of 128 to 1200 tokens (8 is 4 % ahead for 1000 rows of 2000).
 constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, SIZE_AHEAD = 5;
 constexpr uint64_t LINES_DIRECT = 65536, LINES_ALONE = 64;
 
@@ -1478,6 +1481,9 @@ hipError_t launch_shape(const tp_logits& io, void* out, uint64_t out_stride) {
 // no second launch joins it; but a unit works on a segment for some 0.15 us, and fewer long rows than units leave the others idle: they are split.
 // Split / not, us a pass: one row of 20000 14.8 / 11.3, of 32768 14.5 / 12.9, of 50021 14.5 / 14.7, of 65536 14.2 / 16.7, 128 rows of 50021 19.0 / 16.3;
 // one row of 131072 14.7 / 24.1, 48 17.9 / 26.0, 128 23.1 / 26.2, 200 29.8 / 26.6.
+// Up to 131072 tokens, that is: a window has no more (its tables' LDS), so longer rows are split in any case, and the powers of two split them unevenly.  The rule / the best of
+// windows of 32768, 65536, 81920, 98304 and 131072 tokens: one row of 151936 13.5 / 16.2, 48 18.6 / 18.4, 160 40.7 / 28.3 (65536), 512 76.7 / 58.0 (81920); of 262144 13.2 / 16.1,
+// 21.7 / 21.6, 40.1 / 34.5 (98304), 82 / 82.
 // A window must also keep its repeated tokens in 64 KB of LDS.
 static uint32_t window_segments(const tp_logits& io) {
     uint32_t segs = 1;
