@@ -1,13 +1,15 @@
-"""The text of written tokens where its bound is far from its size, and as the first work of a process, on the GPU."""
+"""The text of written tokens where its bound is far from its size and as the first work of a process, and replies under tables with aliases, on the GPU."""
 import os
+import random
 import subprocess
 import sys
 
 import numpy as np
 import pytest
 
-from helpers import ROOT, Config
-from reply_plain import TAGS, PlainGrammar
+from helpers import ROOT, Config, Oracle, assert_same_results
+from reply_plain import TAGS, PlainGrammar, token_list
+from test_reply_tags_cpu import ALIASES, WORDS, lexicon
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -93,3 +95,30 @@ print("captured first calls replay")
 def test_the_first_call_of_a_process_may_be_captured():
     done = subprocess.run([sys.executable, "-c", FIRST], cwd=ROOT, env=dict(os.environ, PYTHONPATH=ROOT), capture_output=True, text=True, timeout=100)
     assert done.returncode == 0 and "captured first calls replay" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("spaces", [False, True])
+def test_replies_under_aliases_are_taken(spaces):
+    """Tables with aliases to kept, unknown and dropped tags, and tags that spell a phrase with blanks: no finished reply is refused and none of its tags is lost."""
+    from imagecaptioner_amd import TagPipe
+    cfg = Config(vocabulary="\n".join(WORDS).encode(), lexicon=lexicon(ALIASES), trigger="solo")
+    pipe, oracle, rng = TagPipe(cfg), Oracle(cfg), random.Random(8)
+    tokens = token_list(rng, WORDS, 500, spaces)
+    g = pipe.tag_grammar(tokens, len(tokens) - 1, spaces=spaces, max_tags=9)
+    rows, steps, vocab = 300, 120, len(tokens)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    history, length = torch.zeros(rows, steps, device="cuda", dtype=torch.int32), torch.zeros(rows, device="cuda", dtype=torch.int32)
+    states, bias = g.start(rows), torch.zeros(vocab, device="cuda")
+    bias[vocab - 1] = 3.0                                                  # an end that comes
+    for _ in range(steps):
+        g.step(states, torch.randn(rows, vocab, generator=gen, device="cuda").mul_(2.0), temperature=torch.ones(rows, device="cuda"),
+               uniform=torch.rand(rows, generator=gen, device="cuda"), append=True, history=history, history_len=length, bias=bias)
+    ended = (states[:, 0] == g.end_place).cpu().numpy()
+    assert ended.mean() > 0.9
+    texts = [b"".join(tokens[t] for t in row[:n] if t != vocab - 1).decode() for row, n in zip(history.cpu().numpy(), length.cpu().numpy())]
+    got, want = pipe.run_tokens(g, history, length), oracle.run_texts(texts)
+    assert_same_results(got, want, pipe.histogram_dict(got.histogram), "replies under aliases")
+    assert not (got.verdicts["flags"][ended] & 0x10).any() and not got.verdicts["n_dropped"][ended].any()
+    for r in np.nonzero(ended)[0]:
+        kept = {oracle.normalize_tag(t) for t in texts[r].split(", ")}
+        assert len(texts[r].split(", ")) >= 3 and got.verdicts["n_candidates"][r] == len(kept) and got.verdicts["n_selected"][r] == len(kept | {"solo", "1girl"}), texts[r]
