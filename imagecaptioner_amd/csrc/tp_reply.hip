@@ -1222,7 +1222,7 @@ __device__ inline Written written(const int32_t* begin, const int32_t* len, uint
 // A wave takes 64 tokens at a time, the next 64's texts and the 64 tokens behind those in flight (256 at a time, loaded together: 8192 rows of 300 in 22.2 us a pass
 // instead of 20.4, for their registers and their bursts); a text stands beside
 // their sizes in 16 bytes up to a length of 15.  Bound by the gathers (64 cache lines a wave's load) and by LDS: 8192 rows of up to 300 tokens (7 MB of
-// tokens, 13 of text: 4.5 us at a copy's rate) take 6 us for the sizes (10 without the table of lengths in LDS) and 15 for the texts.
+// tokens, 13 of text: 4.5 us at a copy's rate) take 5 us for the sizes (10 without the table of lengths in LDS) and 15 to 17 for the texts.
 // A wave of the sizes holds SIZE_AHEAD times 64 tokens: 3, 4, 5, 6 and 8 are within 3 % of one another for 8192 rows of 128 to 1200 tokens (8 is 4 % ahead for 1000 rows of 2000).
 constexpr uint32_t LINE_ROWS = 16, LINE_THREADS = LINE_ROWS * 64, SIZE_AHEAD = 5;
 constexpr uint64_t LINES_DIRECT = 65536, LINES_ALONE = 64;

@@ -1,7 +1,8 @@
 // The torch side of the calls that write replies (replies.py): argument checks, outputs and the call, as the Python module _tp_torch.
 //
 // A decoding loop makes these calls once per token, and for few rows the host's part of one takes longer than the GPU's.  The same checks by Python
-// attribute accesses cost 3 to 5 us a call, and an output 1.4 us; here they cost 0.3 and 0.8 (a grammar step of one row: 12.2 us of host time before, 5.6 now).
+// attribute accesses cost 3 to 5 us a call, and an output 1.4 us; here they cost 0.3 and 0.8 (a grammar step of one row: 12.2 us of host time before, 5.6 to 6.3 now,
+// 0.1 of it for refusing tangents and views that negate).
 // The library's functions come as addresses from whoever has loaded it.
 #include <Python.h>
 

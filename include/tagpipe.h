@@ -573,15 +573,17 @@ int tp_choose_tokens(tp_ctx* ctx, const tp_logits* io, const float* temperature,
  * (Program.cs:1121-1133), without one any such string of the context's tables, and in either case only if the ingest also
  * keeps (and, with a vocabulary file, knows) what NormalizeTag makes of it, an alias's target for instance, and if a line
  * that holds it as it is written does not look bad: with `spaces` "unable_to_stand" would (Program.cs:1144), and a tag that
- * ends in '_' cannot be written.  Or a tag is
- * one of the caller's own `tags`, which are taken as they are: whether the pipeline keeps them is not looked at.
+ * ends in '_' cannot be written.  Or a tag is one of the caller's own `tags`, which are taken as they are: whether the
+ * pipeline keeps them is not looked at.
+ *
  * A token may be any piece of text; one that holds two commas is never allowed.
  * min_tags and max_tags count the tags as they are written.  Tags may repeat, or be normalised to the same one
  * (tp_logits' penalties are there for that), and the ingest keeps one of them (Program.cs:602).  So a caption may have fewer
  * tags than min_tags, and it falls back where fewer than three different ones are selected, the trigger and 1girl among
- * them (Program.cs:297).  Of more than 42 selected tags, the trigger, 1girl and the profile's always-add tags included, the last are
- * left out (Program.cs:38).  And with min_tags below 3 a line of one or two tags and more than 40 characters is refused as a
- * whole (Program.cs:1145-1146).  A line that has not come to its end may stop inside a tag.
+ * them (Program.cs:297).  Of more than 42 selected tags, the trigger, 1girl and the profile's always-add tags included,
+ * the last are left out (Program.cs:38).  And with min_tags below 3 a line of one or two tags and more than 40 characters
+ * is refused as a whole (Program.cs:1145-1146).  A line that has not come to its end may stop inside a tag.
+ *
  * Refused (TP_E_CONFIG): no tags; a token list without a token of its own for every single byte that the lines use,
  * because a line could then come to a place with no way on.  All pointers are host memory and are not kept.
  *
